@@ -7,7 +7,8 @@
  * asynchronous on the `stream` argument (a cudaStream_t passed as void*, NULL =
  * the legacy default stream).  Device-side faults that cannot be known at
  * launch time (a bounded wait that ran out, an out-of-range embedding id) are
- * latched in a per-context status word and reported by mu_check().
+ * latched in a per-context status word and reported by mu_check(); so are page ids, slots and
+ * request lengths that the paged-cache entry points find out of range.
  *
  * Threading: a context may be used from any host thread, by one thread at a time
  * (its error text and its SM budget are per-context state); kernels of different
@@ -37,7 +38,7 @@ enum mu_status {
   MU_ERR_UNSUPPORTED = 2, /* dtype / mode this build does not implement */
   MU_ERR_CUDA = 3,        /* a CUDA runtime / driver call failed */
   MU_ERR_TIMEOUT = 4,     /* a bounded device-side wait ran out */
-  MU_ERR_INDEX = 5,       /* embedding id out of range */
+  MU_ERR_INDEX = 5,       /* embedding id, cache page, slot or request length out of range */
   MU_ERR_NOMEM = 6,
   MU_ERR_SIZE = 7         /* size beyond a documented maximum */
 };
@@ -185,6 +186,66 @@ int mu_attention_static_scratch(int device, const void *q, const void *k, const 
                                 int B, int H, int T, int D, int causal, int kmode, int dtype,
                                 void *stream, int sync_and_check, char *err, size_t err_len);
 
+/* ---- paged 8-bit KV cache ---------------------------------------------------
+ * No counterpart in the reference, whose attention keeps no cache. A cache is a pool of pages that
+ * the caller owns: k_cache / v_cache [num_pages][Hkv][page_size][D] e4m3 (16-byte aligned) with
+ * k_scale / v_scale [num_pages][Hkv] float32 > 0; a stored value stands for e4m3 * scale. The slot of
+ * a token is page * page_size + offset. page_size is a multiple of 16 up to 1024, D at most 256.
+ * All lengths, tables and slots live on the device, so a decode step can be captured in a CUDA graph
+ * and replayed; sizes that the host passes are upper bounds.
+ *
+ * mu_page_map: one step's bookkeeping for B requests (at most MU_PAGE_MAP_MAX_REQUESTS), request r
+ * holding context_lens[r] tokens and gaining new_lens[r]. A request that needs more pages than
+ * ceil(context / page_size) gets the next ones of free_pages[0 .. n_free), in request order, written
+ * behind those it has in block_table[r * table_stride ..]; other entries are left as they are.
+ *   query_start[B+1]  prefix sum of new_lens      seq_lens[B]  context + new
+ *   slots[n_slots]    slot of each new token, requests one after another; -1 behind the last one
+ *   positions[n_slots] position of each new token in its request; 0 behind the last one
+ *   pages_taken[1]    pages taken from the front of free_pages
+ * Too few free pages, table columns or slots latch MU_ERR_NOMEM: entries and slots that have no page
+ * are -1, the rest is valid. A page id outside [0, num_pages) latches MU_ERR_INDEX and gives -1; a
+ * request with a negative length latches MU_ERR_INDEX and counts as empty. Outputs must not overlap
+ * inputs. */
+#define MU_PAGE_MAP_MAX_REQUESTS 16384
+int mu_page_map(mu_ctx *ctx, const int32_t *context_lens, const int32_t *new_lens,
+                const int32_t *free_pages, int n_free, int32_t *block_table, int table_stride, int B,
+                int page_size, int num_pages, int32_t *query_start, int32_t *seq_lens, int32_t *slots,
+                int32_t *positions, int n_slots, int32_t *pages_taken, void *stream);
+
+/* mu_kv_cache_append: stores K and V rows k[t * ld + h * D + d] (ld >= Hkv * D elements: column slabs of
+ * a fused projection work) of n_tokens tokens at slots[t]; slot -1 skips a token, a slot beyond the pool
+ * latches MU_ERR_INDEX and is skipped. Per page and head the scale is the smallest power of two
+ * s >= 2^-64 with amax <= 448 s over the page's finite values; a token that raises it has the page's
+ * earlier tokens (offsets below the new ones) requantised, which loses nothing but e4m3 subnormals.
+ * New tokens at offset 0 start a page afresh. Infinities saturate to +-448 s, NaN stays NaN.
+ * The new tokens of one page must be neighbours in the call, as mu_page_map lays them out; a page
+ * that comes up in two separate places of one call is written by both in no fixed order. A slot that is
+ * repeated among neighbours holds its last row. */
+int mu_kv_cache_append(mu_ctx *ctx, const void *k, const void *v, long long ld, const int32_t *slots,
+                       int n_tokens, void *k_cache, void *v_cache, float *k_scale, float *v_scale,
+                       int num_pages, int page_size, int Hkv, int D, int dtype, void *stream);
+
+/* mu_attention_paged: attention of n_tokens query rows q[t * q_ld + h * D + d] (Hq heads, a multiple of
+ * Hkv; query head h reads KV head h / (Hq / Hkv)) over the cache, scaled by 1/sqrt(D). Request b owns
+ * the rows query_start[b] .. query_start[b+1]; its keys are the first seq_lens[b] tokens of its pages, the
+ * new ones among them (append first). Single tokens, prompt chunks and mixtures go in one call. causal:
+ * row i of n sees the keys up to position seq_len - n + i; a row that sees none gives zeros. Rows of
+ * `out` behind query_start[B] are left as they are. Keys on a page id outside the pool, or beyond
+ * table_stride pages, are left out and latch MU_ERR_INDEX; so do contradictory row ranges, whose
+ * request is skipped. What lies in a page behind its request's last token is never read as a value.
+ * workspace (16-byte aligned, mu_attention_paged_workspace_bytes) holds pieces of long requests during the
+ * call only; calls that may overlap on the GPU need one each. At most MU_ATTENTION_PAGED_MAX_REQUESTS
+ * requests. */
+#define MU_ATTENTION_PAGED_MAX_REQUESTS 16384
+size_t mu_attention_paged_workspace_bytes(const mu_ctx *ctx, int n_tokens, int B, int Hq, int Hkv,
+                                          int D, int dtype);
+int mu_attention_paged(mu_ctx *ctx, const void *q, long long q_ld, void *out, long long out_ld,
+                       const void *k_cache, const void *v_cache, const float *k_scale,
+                       const float *v_scale, const int32_t *block_table, int table_stride,
+                       const int32_t *query_start, const int32_t *seq_lens, int B, int n_tokens, int Hq,
+                       int Hkv, int D, int num_pages, int page_size, int causal, int dtype,
+                       void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- normalisation / softmax ----------------------------------------------
  * ops::layer_norm (src/core/ops/normalization.cpp:125-224; host-only in the
  * reference) and Backend::softmax over the last dim (src/core/backend.hpp:243). */
@@ -298,6 +359,25 @@ int mu_fill_uniform(mu_ctx *ctx, void *out, long long n, float low, float high,
  * (demos/transformers/decoder_block_demo.py:112). First maximum wins. */
 int mu_argmax(mu_ctx *ctx, const void *x, int32_t *idx, long long rows, int cols, int dtype,
               void *stream);
+
+/* ---- sampling ---------------------------------------------------------------
+ * mu_argmax's counterpart for drawn tokens (the reference has neither): one token per row of
+ * logits[r * ld + i], i < cols (at most MU_SAMPLE_MAX_COLS), from the caller's uniform numbers
+ * uniform[rows] in [0, 1). With w_i = exp((x_i - max) / temperature):
+ *   top_k  keeps the k largest logits (equal ones: lowest index first); k <= 0 or >= cols: all
+ *   top_p  keeps of those, in that order, the shortest prefix with at least top_p of their weight;
+ *          >= 1: all, the first one always stays
+ *   min_p  keeps of those the ones with w_i >= min_p (at most 1); <= 0: all
+ * idx[r] = the first index, in index order, at which the running sum of the kept weights exceeds
+ * uniform * (their sum); prob[r] = its share of that sum. temperature, top_k, top_p, min_p are one value
+ * per row on the device, or NULL for none (temperature 1); prob may be NULL. A temperature <= 0 takes the
+ * first maximum. NaN counts as -inf; a row with nothing above -inf gives idx -1, prob 0; +inf leaves
+ * only infinite logits. Sums are exact (weights are integer multiples of 2^-42), so results do not
+ * depend on the launch shape. */
+#define MU_SAMPLE_MAX_COLS 1048576
+int mu_sample(mu_ctx *ctx, const void *logits, long long ld, const float *uniform,
+              const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+              int32_t *idx, float *prob, int rows, int cols, int dtype, void *stream);
 
 /* ---- all-reduce ------------------------------------------------------------
  * Backend::all_reduce (src/core/backend.hpp:199,473-477): elementwise SUM over the

@@ -64,6 +64,11 @@ SIGNATURES = {
     "mu_attention": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
     "mu_attention_static_scratch": (_i, [_i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _i,
                                          C.c_char_p, _sz]),
+    "mu_page_map": (_i, [_vp] * 4 + [_i, _vp] + [_i] * 4 + [_vp] * 4 + [_i, _vp, _vp]),
+    "mu_kv_cache_append": (_i, [_vp] * 3 + [_ll, _vp, _i] + [_vp] * 4 + [_i] * 5 + [_vp]),
+    "mu_attention_paged_workspace_bytes": (_sz, [_vp] + [_i] * 6),
+    "mu_attention_paged": (_i, [_vp, _vp, _ll, _vp, _ll] + [_vp] * 5 + [_i, _vp, _vp] + [_i] * 9 +
+                           [_vp, _sz, _vp]),
     "mu_conv2d": (_i, [_vp, _vp, _vp, _vp, _vp] + [_i] * 11 + [_vp]),
     "mu_max_pool2d": (_i, [_vp, _vp, _vp] + [_i] * 8 + [_vp]),
     "mu_global_avg_pool": (_i, [_vp, _vp, _vp] + [_i] * 5 + [_vp]),
@@ -72,6 +77,7 @@ SIGNATURES = {
     "mu_embedding": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "mu_eltwise": (_i, [_vp, _vp, _vp, _vp, _vp, _ll, _i, _i, _i, _vp]),
     "mu_argmax": (_i, [_vp, _vp, _vp, _ll, _i, _i, _vp]),
+    "mu_sample": (_i, [_vp, _vp, _ll] + [_vp] * 7 + [_i] * 3 + [_vp]),
     "mu_unary": (_i, [_vp, _i, _vp, _vp, _ll, _i, _vp]),
     "mu_leaky_relu": (_i, [_vp, _vp, _vp, _ll, C.c_float, _i, _vp]),
     "mu_broadcast_row": (_i, [_vp, _vp, _vp, _ll, _i, _i, _vp]),
@@ -263,6 +269,35 @@ class Context:
                                         int(causal), kmode, dtype, _ptr(workspace),
                                         workspace_bytes, _stream(stream)))
 
+    # -- paged 8-bit KV cache ----------------------------------------------------
+    def page_map(self, context_lens, new_lens, free_pages, n_free, block_table, table_stride, B, page_size,
+                 num_pages, query_start, seq_lens, slots, positions, n_slots, pages_taken, stream=None):
+        """Block tables, slots and positions of one step from the request lengths (all on the device)."""
+        self._rc(self._lib.mu_page_map(
+            self._h, _ptr(context_lens), _ptr(new_lens), _ptr(free_pages), n_free, _ptr(block_table),
+            table_stride, B, page_size, num_pages, _ptr(query_start), _ptr(seq_lens), _ptr(slots),
+            _ptr(positions), n_slots, _ptr(pages_taken), _stream(stream)))
+
+    def kv_cache_append(self, k, v, ld, slots, n_tokens, k_cache, v_cache, k_scale, v_scale, num_pages,
+                        page_size, Hkv, D, dtype, stream=None):
+        """Quantise K/V rows (``ld`` elements between tokens) into the e4m3 pages at ``slots``."""
+        self._rc(self._lib.mu_kv_cache_append(
+            self._h, _ptr(k), _ptr(v), ld, _ptr(slots), n_tokens, _ptr(k_cache), _ptr(v_cache),
+            _ptr(k_scale), _ptr(v_scale), num_pages, page_size, Hkv, D, dtype, _stream(stream)))
+
+    def attention_paged_workspace_bytes(self, n_tokens, B, Hq, Hkv, D, dtype) -> int:
+        return int(self._lib.mu_attention_paged_workspace_bytes(self._h, n_tokens, B, Hq, Hkv, D, dtype))
+
+    def attention_paged(self, q, q_ld, out, out_ld, k_cache, v_cache, k_scale, v_scale, block_table,
+                        table_stride, query_start, seq_lens, B, n_tokens, Hq, Hkv, D, num_pages, page_size,
+                        causal, dtype, workspace, workspace_bytes, stream=None):
+        """Attention of ragged query rows over the paged e4m3 cache."""
+        self._rc(self._lib.mu_attention_paged(
+            self._h, _ptr(q), q_ld, _ptr(out), out_ld, _ptr(k_cache), _ptr(v_cache), _ptr(k_scale),
+            _ptr(v_scale), _ptr(block_table), table_stride, _ptr(query_start), _ptr(seq_lens), B, n_tokens,
+            Hq, Hkv, D, num_pages, page_size, int(causal), dtype, _ptr(workspace), workspace_bytes,
+            _stream(stream)))
+
     # -- rows / elementwise ----------------------------------------------------
     def layer_norm(self, x, gamma, beta, y, rows, cols, dtype, eps=1e-5, stream=None):
         self._rc(self._lib.mu_layer_norm(self._h, _ptr(x), _ptr(gamma), _ptr(beta), _ptr(y), rows,
@@ -353,6 +388,13 @@ class Context:
 
     def argmax(self, x, idx, rows, cols, dtype, stream=None):
         self._rc(self._lib.mu_argmax(self._h, _ptr(x), _ptr(idx), rows, cols, dtype, _stream(stream)))
+
+    def sample(self, logits, ld, uniform, temperature, top_k, top_p, min_p, idx, prob, rows, cols, dtype,
+               stream=None):
+        """One token per row from ``uniform``; per-row temperature / top_k / top_p / min_p (None = off)."""
+        self._rc(self._lib.mu_sample(self._h, _ptr(logits), ld, _ptr(uniform), _ptr(temperature),
+                                     _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(idx), _ptr(prob), rows, cols,
+                                     dtype, _stream(stream)))
 
     def all_reduce_sum(self, comm, buf, n, dtype, stream=None):
         self._rc(self._lib.mu_all_reduce_sum(self._h, comm._h if comm else None, _ptr(buf), n, dtype,

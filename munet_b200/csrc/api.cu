@@ -335,6 +335,12 @@ int mu_check(mu_ctx *ctx, void *stream) {
   cudaMemset(ctx->d_status, 0, sizeof(int));
   if (st == 110)
     return fail(ctx, MU_ERR_INDEX, "Embedding index out of range");
+  if (st == 111)
+    return fail(ctx, MU_ERR_INDEX, "paged cache: page or slot out of range");
+  if (st == 112)
+    return fail(ctx, MU_ERR_NOMEM, "page map: free pages, block table or slots exhausted");
+  if (st == 113)
+    return fail(ctx, MU_ERR_INDEX, "paged cache: request lengths out of range");
   return fail(ctx, MU_ERR_TIMEOUT, "device-side bounded wait ran out (code %d)", st);
 }
 

@@ -1,0 +1,546 @@
+// Page bookkeeping of a paged KV cache and the write into its 8-bit pages.
+//
+// Layout: k_cache / v_cache [num_pages][Hkv][page_size][D] e4m3, k_scale / v_scale
+// [num_pages][Hkv] float32; value = e4m3 * scale. Keys of one head inside one page are contiguous,
+// so attention reads page_size * D bytes in a row. Slot of a token = page * page_size + offset.
+//
+// No counterpart in the reference (it has no KV cache); the argument checks, the latched device
+// status and the asynchronous streams are those of the other entry points.
+#include "../../include/munet_b200.h"
+#include "common.h"
+#include "ptx.cuh"
+#include <climits>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+namespace mu {
+
+// ---- page map -----------------------------------------------------------------------------------
+// One launch. Every CTA scans the request lengths itself (two prefix sums kept in shared memory: new
+// tokens and new pages), which costs less than a second launch or a grid-wide barrier; the grid then
+// shares out the new table entries and the tokens, each finding its request by binary search.
+// Entries of the block table that are read (pages a request holds already) and those that are written
+// (its new pages) never overlap, so no order between CTAs is needed.
+constexpr int PM_THREADS = 512;
+
+struct PageMapArgs {
+  const int *context_lens, *new_lens, *free_pages;
+  int n_free;
+  int *block_table;
+  int table_stride, B, page_size, num_pages;
+  int *query_start, *seq_lens, *slots, *positions;
+  int n_slots;
+  int *pages_taken;
+  int *status;
+};
+
+// Index of the first entry of ends[0..n) that is > v (n when there is none).
+__device__ __forceinline__ int upper_bound(const int *ends, int n, int v) {
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (ends[mid] > v)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  return lo;
+}
+
+struct ReqLens {
+  int ctx, add, old_pages, new_pages;
+  bool ok, fits;
+};
+// Lengths of one request; a negative one, or a sum beyond int32, counts as an empty request.
+__device__ __forceinline__ ReqLens req_lens(const PageMapArgs &a, int r) {
+  ReqLens q;
+  q.ctx = a.context_lens[r], q.add = a.new_lens[r];
+  const long long total = 1ll * q.ctx + q.add;
+  q.ok = q.ctx >= 0 && q.add >= 0 && total <= INT_MAX;
+  if (!q.ok)
+    q.ctx = q.add = 0;
+  const unsigned ps = a.page_size;
+  const int have = static_cast<int>((static_cast<unsigned>(q.ctx) + ps - 1) / ps);
+  const int want = static_cast<int>((static_cast<unsigned>(q.ctx) + static_cast<unsigned>(q.add) + ps - 1) / ps);
+  q.fits = want <= a.table_stride;
+  q.old_pages = min(have, a.table_stride);
+  q.new_pages = min(want, a.table_stride) - q.old_pages;
+  return q;
+}
+
+__global__ void __launch_bounds__(PM_THREADS) page_map_kernel(PageMapArgs a) {
+  extern __shared__ int sm[];
+  int *tok_end = sm, *page_end = sm + a.B; // inclusive prefix sums, saturated at INT_MAX
+  __shared__ long long warp_tok[PM_THREADS / 32], warp_page[PM_THREADS / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (a.B + PM_THREADS - 1) / PM_THREADS;
+  const int r0 = min(tid * per, a.B), r1 = min(r0 + per, a.B);
+  long long toks = 0, pages = 0;
+  bool bad = false, full = false;
+  for (int r = r0; r < r1; ++r) {
+    const ReqLens q = req_lens(a, r);
+    bad |= !q.ok, full |= !q.fits;
+    toks += q.add, pages += q.new_pages;
+    if (blockIdx.x == 0)
+      a.seq_lens[r] = q.ctx + q.add;
+  }
+  long long st = toks, sp = pages;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long t = __shfl_up_sync(~0u, st, d), p = __shfl_up_sync(~0u, sp, d);
+    if (lane >= d)
+      st += t, sp += p;
+  }
+  if (lane == 31)
+    warp_tok[warp] = st, warp_page[warp] = sp;
+  __syncthreads();
+  long long bt = st - toks, bp = sp - pages, all_tok = 0, all_page = 0;
+#pragma unroll
+  for (int w = 0; w < PM_THREADS / 32; ++w) {
+    if (w < warp)
+      bt += warp_tok[w], bp += warp_page[w];
+    all_tok += warp_tok[w], all_page += warp_page[w];
+  }
+  for (int r = r0; r < r1; ++r) {
+    const ReqLens q = req_lens(a, r);
+    if (blockIdx.x == 0)
+      a.query_start[r] = static_cast<int>(min(bt, 1ll * INT_MAX));
+    bt += q.add, bp += q.new_pages;
+    tok_end[r] = static_cast<int>(min(bt, 1ll * INT_MAX));
+    page_end[r] = static_cast<int>(min(bp, 1ll * INT_MAX));
+  }
+  if (blockIdx.x == 0) {
+    if (bad)
+      atomicCAS(a.status, 0, MU_DEV_BAD_LENGTH);
+    if (full || (tid == 0 && (all_tok > a.n_slots || all_page > a.n_free)))
+      atomicCAS(a.status, 0, MU_DEV_NO_PAGE);
+    if (tid == 0) {
+      a.query_start[a.B] = static_cast<int>(min(all_tok, 1ll * INT_MAX));
+      a.pages_taken[0] = static_cast<int>(min(all_page, 1ll * a.n_free));
+    }
+  }
+  __syncthreads();
+
+  const unsigned ps = a.page_size;
+  const int stride = gridDim.x * PM_THREADS, first = blockIdx.x * PM_THREADS + tid;
+  // new pages: entry j of the free list goes to the request whose range of new pages holds j
+  const long long fresh = min(all_page, 1ll * INT_MAX - stride);
+  for (int f = first; f < fresh; f += stride) {
+    const int r = upper_bound(page_end, a.B, f);
+    if (r >= a.B)
+      break;
+    const ReqLens q = req_lens(a, r);
+    const int j = f - (page_end[r] - q.new_pages);
+    int page = f < a.n_free ? a.free_pages[f] : -1;
+    if (f < a.n_free && (page < 0 || page >= a.num_pages)) {
+      atomicCAS(a.status, 0, MU_DEV_BAD_PAGE);
+      page = -1;
+    }
+    a.block_table[1ll * r * a.table_stride + q.old_pages + j] = page;
+  }
+  // tokens: a page the request held before comes from its table, a new one from the free list
+  const int limit = static_cast<int>(min(all_tok, 1ll * a.n_slots));
+  for (long long tl = first; tl < a.n_slots; tl += stride) {
+    const int t = static_cast<int>(tl);
+    int slot = -1, pos = 0;
+    if (t < limit) {
+      const int r = upper_bound(tok_end, a.B, t);
+      const ReqLens q = req_lens(a, r);
+      pos = q.ctx + (t - (tok_end[r] - q.add));
+      const int pi = static_cast<int>(static_cast<unsigned>(pos) / ps);
+      int page = -1;
+      bool known = false;
+      if (pi < q.old_pages) {
+        page = a.block_table[1ll * r * a.table_stride + pi];
+        known = true;
+      } else if (pi < q.old_pages + q.new_pages) {
+        const int f = page_end[r] - q.new_pages + (pi - q.old_pages);
+        if (f < a.n_free)
+          page = a.free_pages[f], known = true;
+      }
+      if (page >= 0 && page < a.num_pages)
+        slot = static_cast<int>(static_cast<unsigned>(page) * ps + static_cast<unsigned>(pos) % ps);
+      else if (known)
+        atomicCAS(a.status, 0, MU_DEV_BAD_PAGE);
+    }
+    a.slots[t] = slot;
+    a.positions[t] = pos;
+  }
+}
+
+// 0 ok, 2 CUDA error
+int launch_page_map(const PageMapArgs &a, int num_sms, cudaStream_t st) {
+  const size_t smem = 2ull * sizeof(int) * a.B;
+  static PerDeviceOnce once;
+  if (once.get() < 0) {
+    if (cudaFuncSetAttribute(page_map_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(2 * sizeof(int) * MU_PAGE_MAP_MAX_REQUESTS)) != cudaSuccess)
+      return 2;
+    once.set(1);
+  }
+  long long blocks = (1ll * a.n_slots + PM_THREADS - 1) / PM_THREADS; // a new page holds a new token at least
+  if (blocks > num_sms)
+    blocks = num_sms;
+  if (blocks < 1)
+    blocks = 1;
+  page_map_kernel<<<static_cast<unsigned>(blocks), PM_THREADS, smem, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? 0 : 2;
+}
+
+// ---- write into the cache -----------------------------------------------------------------------
+// Work unit: the run of consecutive new tokens that fall into one page, for one head of K or V. Its
+// CTA finds the run's largest magnitude, derives the page's scale, requantises what the page held
+// before if the scale grew, and stores the new rows. The rows stay in registers between the two
+// steps (64 elements per thread: a page of 64 x 128), so HBM sees them once.
+//
+// Scale: the smallest power of two s >= 2^-64 with amax <= 448 s. e4m3 keeps its three mantissa bits
+// at every magnitude, so a power of two loses nothing against amax/448 except range at the bottom,
+// and growing it later is exact for everything above the subnormals.
+constexpr int AP_THREADS = 128;
+constexpr int AP_REGS = 8;       // vectors of 8 elements a thread keeps
+constexpr int AP_MAX_BLOCK = 64; // most tokens one CTA looks at for run starts
+
+struct AppendArgs {
+  const void *x[2]; // K, V
+  long long ld;     // elements between tokens
+  const int *slots;
+  int n_tokens;
+  uint8_t *cache[2];
+  float *scale[2];
+  int num_pages, page_size, H, D;
+  int block_tokens; // tokens per CTA
+  unsigned dv, dv_magic; // vectors per row and ceil(2^32 / dv)
+  int *status;
+};
+
+template <typename T, int VE> __device__ __forceinline__ void load_row_vec(const T *p, float (&f)[VE]) {
+  if constexpr (VE == 8 && sizeof(T) == 2) {
+    const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p));
+    f[0] = bf16_lo(u.x), f[1] = bf16_hi(u.x), f[2] = bf16_lo(u.y), f[3] = bf16_hi(u.y);
+    f[4] = bf16_lo(u.z), f[5] = bf16_hi(u.z), f[6] = bf16_lo(u.w), f[7] = bf16_hi(u.w);
+  } else if constexpr (VE == 8) {
+    const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VE; ++i)
+      f[i] = static_cast<float>(p[i]);
+  }
+}
+// largest finite magnitude, as bits (ordered like the values)
+template <int VE> __device__ __forceinline__ uint32_t amax_bits(const float (&f)[VE], uint32_t m) {
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    const uint32_t b = __float_as_uint(f[i]) & 0x7fffffffu;
+    m = max(m, b < 0x7f800000u ? b : 0u);
+  }
+  return m;
+}
+// smallest power of two s >= 2^-64 with amax <= 448 s (448 = 1.75 * 2^8)
+__device__ __forceinline__ float page_scale(uint32_t amax) {
+  int e = static_cast<int>(amax >> 23) - 127; // subnormals end at the floor
+  if ((amax & 0x7fffffu) > 0x600000u)         // mantissa above 1.75
+    ++e;
+  e = max(e - 8, -64);
+  return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+}
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t two) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3);
+  return __half22float2(static_cast<__half2>(h));
+}
+// One rounding, from 64 bits: for scales that are no power of two (a cache that someone else filled).
+__device__ __forceinline__ uint32_t e4m3_of_double(double v) {
+  return __nv_cvt_double_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+}
+// Rows leave as v / s. A power of two's reciprocal is exact, so the product rounds once, in the
+// conversion; any other scale is divided by in 64 bits, or the quotient would be rounded twice.
+struct Divisor {
+  float s, inv;
+  bool pow2;
+  __device__ __forceinline__ explicit Divisor(float scale) : s(scale) {
+    pow2 = (__float_as_uint(scale) & 0x7fffffu) == 0;
+    inv = 1.0f / scale;
+  }
+  __device__ __forceinline__ uint32_t code2(float a, float b) const {
+    if (pow2)
+      return e4m3x2(a * inv, b * inv);
+    return e4m3_of_double(static_cast<double>(a) / s) | (e4m3_of_double(static_cast<double>(b) / s) << 8);
+  }
+};
+template <int VE>
+__device__ __forceinline__ void store_row_vec(uint8_t *dst, const float (&f)[VE], const Divisor &div) {
+  if constexpr (VE == 8) {
+    uint2 u;
+    u.x = div.code2(f[0], f[1]) | (div.code2(f[2], f[3]) << 16);
+    u.y = div.code2(f[4], f[5]) | (div.code2(f[6], f[7]) << 16);
+    *reinterpret_cast<uint2 *>(dst) = u;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VE; ++i)
+      dst[i] = static_cast<uint8_t>(div.code2(f[i], 0.f) & 0xffu);
+  }
+}
+
+// First set bit of `bits` at or after `from`, `n` if none below n.
+__device__ __forceinline__ int next_bit(const uint32_t *bits, int from, int n) {
+  for (int w = from >> 5; w * 32 < n; ++w) {
+    uint32_t v = bits[w];
+    if (w == from >> 5)
+      v &= ~0u << (from & 31);
+    if (v)
+      return min(w * 32 + __ffs(v) - 1, n);
+  }
+  return n;
+}
+
+template <typename T, int VE>
+__global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(AppendArgs a) {
+  // window of slots: the CTA's tokens and as many as one page holds after them
+  extern __shared__ int sm[];
+  const int win = min(a.block_tokens + a.page_size, a.n_tokens - static_cast<int>(blockIdx.x) * a.block_tokens);
+  const int words = (a.block_tokens + a.page_size + 31) / 32;
+  int *slot = sm;                                                             // [win]
+  uint32_t *starts = reinterpret_cast<uint32_t *>(sm + a.block_tokens + a.page_size); // token begins a run (or none)
+  uint32_t *disorder = starts + words;                                        // token continues a run at a lower offset
+  __shared__ uint32_t red[AP_THREADS / 32];
+  const int tid = threadIdx.x, t0 = blockIdx.x * a.block_tokens;
+  const int which = blockIdx.y & 1, h = blockIdx.y >> 1;
+  const unsigned ps = a.page_size;
+  const unsigned n_slots = static_cast<unsigned>(a.num_pages) * ps;
+  for (int i = tid; i < words * 32; i += AP_THREADS) { // whole warps: the ballots need every lane
+    int s = -1, before = -1;
+    if (i < win) {
+      s = a.slots[t0 + i];
+      before = t0 + i > 0 ? a.slots[t0 + i - 1] : -1;
+      if (s >= 0 && static_cast<unsigned>(s) >= n_slots) {
+        if (blockIdx.y == 0)
+          atomicCAS(a.status, 0, MU_DEV_BAD_PAGE);
+        s = -1;
+      }
+      if (before >= 0 && static_cast<unsigned>(before) >= n_slots)
+        before = -1;
+      slot[i] = s;
+    }
+    const bool same = s >= 0 && before >= 0 && static_cast<unsigned>(s) / ps == static_cast<unsigned>(before) / ps;
+    const uint32_t st = __ballot_sync(~0u, !same), di = __ballot_sync(~0u, same && s <= before);
+    if ((tid & 31) == 0)
+      starts[i >> 5] = st, disorder[i >> 5] = di;
+  }
+  __syncthreads();
+
+  const T *x = static_cast<const T *>(a.x[which]) + 1ll * h * a.D;
+  // row of vector v: exact for v < 2^18, dv <= 2^8
+  auto row_of = [&](unsigned v) { return a.dv == 1 ? v : __umulhi(v, a.dv_magic); };
+  for (int i = next_bit(starts, 0, a.block_tokens); i < a.block_tokens && i < win;
+       i = next_bit(starts, i + 1, a.block_tokens)) {
+    if (slot[i] < 0)
+      continue;
+    int n = next_bit(starts, i + 1, win) - i;
+    const unsigned page = static_cast<unsigned>(slot[i]) / ps;
+    // A run in ascending order ends within the window. One that is out of order, or repeats a slot,
+    // takes the slow walk below, token by token, so that the last write of a slot is the one that stays.
+    const bool ordered = next_bit(disorder, i + 1, i + n) >= i + n && n <= a.page_size;
+    int low = static_cast<int>(slot[i] - page * ps);
+    if (!ordered) {
+      int j = i + 1;
+      for (; t0 + j < a.n_tokens; ++j) {
+        const int s = a.slots[t0 + j];
+        if (s < 0 || static_cast<unsigned>(s) >= n_slots || static_cast<unsigned>(s) / ps != page)
+          break;
+        low = min(low, static_cast<int>(s - page * ps));
+      }
+      n = j - i;
+    }
+    uint8_t *tile = a.cache[which] + (1ull * page * a.H + h) * ps * a.D;
+    float *scale = a.scale[which] + 1ull * page * a.H + h;
+    const float held = low > 0 ? *scale : 0.f;
+    const T *rows = x + (1ll * t0 + i) * a.ld;
+    const long long total = 1ll * n * a.dv;
+
+    float keep[AP_REGS][VE];
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < AP_REGS; ++k) {
+      const unsigned v = tid + k * AP_THREADS;
+      if (v < total) {
+        const unsigned row = row_of(v);
+        load_row_vec<T, VE>(rows + row * a.ld + (v - row * a.dv) * VE, keep[k]);
+        m = amax_bits<VE>(keep[k], m);
+      }
+    }
+    for (long long v = tid + AP_REGS * AP_THREADS; v < total; v += AP_THREADS) {
+      float f[VE];
+      load_row_vec<T, VE>(rows + (v / a.dv) * a.ld + (v % a.dv) * VE, f);
+      m = amax_bits<VE>(f, m);
+    }
+    m = __reduce_max_sync(~0u, m);
+    if ((tid & 31) == 0)
+      red[tid >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < AP_THREADS / 32; ++w)
+      m = max(m, red[w]);
+    const float now = fmaxf(held, page_scale(m));
+    if (tid == 0)
+      *scale = now;
+    if (low > 0 && now > held) { // what the page held: low * D bytes from the tile's start
+      // now is a power of two here, so q * (held / now) is exact in float for a held power of two and in
+      // double for any other
+      const double f = held > 0.f ? static_cast<double>(held) / now : 0.0;
+      const bool pow2 = (__float_as_uint(held) & 0x7fffffu) == 0;
+      const float ff = static_cast<float>(f);
+      const int bytes = low * a.D;
+      auto again = [&](uint32_t two) -> uint32_t {
+        const float2 p = e4m3x2_to_float2(two);
+        return pow2 ? e4m3x2(p.x * ff, p.y * ff) : e4m3_of_double(p.x * f) | (e4m3_of_double(p.y * f) << 8);
+      };
+      uint32_t *w = reinterpret_cast<uint32_t *>(tile);
+      for (int k = tid; k < bytes / 4; k += AP_THREADS) {
+        const uint32_t u = w[k];
+        w[k] = again(u & 0xffffu) | (again(u >> 16) << 16);
+      }
+      for (int k = (bytes & ~3) + tid; k < bytes; k += AP_THREADS)
+        tile[k] = static_cast<uint8_t>(again(tile[k]) & 0xffu);
+    }
+    const Divisor div(now);
+    if (ordered) {
+#pragma unroll
+      for (int k = 0; k < AP_REGS; ++k) {
+        const unsigned v = tid + k * AP_THREADS;
+        if (v < total) {
+          const unsigned row = row_of(v);
+          store_row_vec<VE>(tile + (slot[i + row] - page * ps) * a.D + (v - row * a.dv) * VE, keep[k], div);
+        }
+      }
+      for (unsigned v = tid + AP_REGS * AP_THREADS; v < total; v += AP_THREADS) {
+        const unsigned row = row_of(v);
+        float f[VE];
+        load_row_vec<T, VE>(rows + row * a.ld + (v - row * a.dv) * VE, f);
+        store_row_vec<VE>(tile + (slot[i + row] - page * ps) * a.D + (v - row * a.dv) * VE, f, div);
+      }
+    } else {
+      for (int j = 0; j < n; ++j) {
+        __syncthreads(); // the requantised bytes and the token before are in place
+        const unsigned s = a.slots[t0 + i + j];
+        for (unsigned v = tid; v < a.dv; v += AP_THREADS) {
+          float f[VE];
+          load_row_vec<T, VE>(rows + j * a.ld + v * VE, f);
+          store_row_vec<VE>(tile + (s - page * ps) * a.D + v * VE, f, div);
+        }
+      }
+    }
+    __syncthreads(); // red[] is free again
+  }
+}
+
+// 0 ok, 1 dtype not implemented, 2 CUDA error
+int launch_kv_append(AppendArgs a, int dtype, int num_sms, cudaStream_t st) {
+  if (dtype != F32 && dtype != BF16)
+    return 1;
+  const int es = dtype == F32 ? 4 : 2;
+  bool vec = a.D % 8 == 0 && (a.ld * es) % 16 == 0;
+  for (int i = 0; i < 2; ++i)
+    vec = vec && (reinterpret_cast<uintptr_t>(a.x[i]) & 15u) == 0;
+  a.dv = vec ? a.D / 8 : a.D;
+  a.dv_magic = static_cast<unsigned>((0x100000000ull + a.dv - 1) / a.dv); // unused where dv is 1
+  // Tokens per CTA: one where the calls are few (a decode step: every token starts a run), more where
+  // that would only launch CTAs that find no start (prompts: one start per page).
+  const long long ctas = 2ll * a.H * a.n_tokens;
+  long long tb = ctas / (num_sms * 64ll);
+  if (tb > AP_MAX_BLOCK)
+    tb = AP_MAX_BLOCK;
+  if (tb > a.page_size)
+    tb = a.page_size;
+  if (tb < 1)
+    tb = 1;
+  a.block_tokens = static_cast<int>(tb);
+  const int span = a.block_tokens + a.page_size, words = (span + 31) / 32;
+  const size_t smem = sizeof(int) * (span + 2ull * words);
+  const dim3 grid(static_cast<unsigned>((a.n_tokens + tb - 1) / tb), static_cast<unsigned>(2 * a.H));
+  if (dtype == F32) {
+    if (vec)
+      kv_append_kernel<float, 8><<<grid, AP_THREADS, smem, st>>>(a);
+    else
+      kv_append_kernel<float, 1><<<grid, AP_THREADS, smem, st>>>(a);
+  } else {
+    if (vec)
+      kv_append_kernel<__nv_bfloat16, 8><<<grid, AP_THREADS, smem, st>>>(a);
+    else
+      kv_append_kernel<__nv_bfloat16, 1><<<grid, AP_THREADS, smem, st>>>(a);
+  }
+  return cudaGetLastError() == cudaSuccess ? 0 : 2;
+}
+
+} // namespace mu
+
+extern "C" {
+
+int mu_set_error(mu_ctx *ctx, int code, const char *msg);
+int mu_ctx_select_device(mu_ctx *ctx);
+int mu_ctx_num_sms(const mu_ctx *ctx);
+int *mu_ctx_status_ptr(mu_ctx *ctx);
+
+int mu_page_map(mu_ctx *ctx, const int32_t *context_lens, const int32_t *new_lens, const int32_t *free_pages,
+                int n_free, int32_t *block_table, int table_stride, int B, int page_size, int num_pages,
+                int32_t *query_start, int32_t *seq_lens, int32_t *slots, int32_t *positions, int n_slots,
+                int32_t *pages_taken, void *stream) {
+  if (!ctx)
+    return MU_ERR_INVALID;
+  if (B < 0 || n_free < 0 || n_slots < 0 || table_stride < 0 || page_size <= 0 || num_pages < 0)
+    return mu_set_error(ctx, MU_ERR_INVALID, "page_map: negative size");
+  if (B > MU_PAGE_MAP_MAX_REQUESTS)
+    return mu_set_error(ctx, MU_ERR_SIZE, "page_map: more than MU_PAGE_MAP_MAX_REQUESTS requests");
+  if (1ll * num_pages * page_size > INT_MAX)
+    return mu_set_error(ctx, MU_ERR_SIZE, "page_map: num_pages * page_size does not fit a 32-bit slot");
+  if (!query_start || !pages_taken || (B > 0 && (!context_lens || !new_lens || !seq_lens)) ||
+      (B > 0 && table_stride > 0 && !block_table) || (n_free > 0 && !free_pages) ||
+      (n_slots > 0 && (!slots || !positions)))
+    return mu_set_error(ctx, MU_ERR_INVALID, "page_map: null pointer");
+  if (mu_ctx_select_device(ctx) != MU_OK)
+    return mu_set_error(ctx, MU_ERR_CUDA, "page_map: cannot select device");
+  const mu::PageMapArgs a{context_lens, new_lens, free_pages, n_free, block_table, table_stride, B, page_size,
+                          num_pages, query_start, seq_lens, slots, positions, n_slots, pages_taken,
+                          mu_ctx_status_ptr(ctx)};
+  if (mu::launch_page_map(a, mu_ctx_num_sms(ctx), static_cast<cudaStream_t>(stream)))
+    return mu_set_error(ctx, MU_ERR_CUDA, cudaGetErrorString(cudaGetLastError()));
+  return MU_OK;
+}
+
+int mu_kv_cache_append(mu_ctx *ctx, const void *k, const void *v, long long ld, const int32_t *slots,
+                       int n_tokens, void *k_cache, void *v_cache, float *k_scale, float *v_scale,
+                       int num_pages, int page_size, int Hkv, int D, int dtype, void *stream) {
+  if (!ctx)
+    return MU_ERR_INVALID;
+  if (n_tokens < 0 || num_pages < 0 || Hkv <= 0 || D <= 0 || page_size <= 0)
+    return mu_set_error(ctx, MU_ERR_INVALID, "kv_cache_append: bad dimensions");
+  if (page_size % 16 != 0 || page_size > 1024 || D > 256 || Hkv > 16384)
+    return mu_set_error(ctx, MU_ERR_UNSUPPORTED, "kv_cache_append: page size a multiple of 16 up to 1024, head size "
+                        "up to 256, at most 16384 heads");
+  if (dtype != MU_F32 && dtype != MU_BF16)
+    return mu_set_error(ctx, MU_ERR_UNSUPPORTED, "kv_cache_append: dtype not implemented (float32, bfloat16)");
+  if (ld < 1ll * Hkv * D)
+    return mu_set_error(ctx, MU_ERR_INVALID, "kv_cache_append: row stride below Hkv * D");
+  if (1ll * num_pages * page_size > INT_MAX)
+    return mu_set_error(ctx, MU_ERR_SIZE, "kv_cache_append: num_pages * page_size does not fit a 32-bit slot");
+  if (n_tokens == 0)
+    return MU_OK;
+  if (!k || !v || !slots || !k_cache || !v_cache || !k_scale || !v_scale)
+    return mu_set_error(ctx, MU_ERR_INVALID, "kv_cache_append: null pointer");
+  if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15u)
+    return mu_set_error(ctx, MU_ERR_INVALID, "kv_cache_append: the caches must be 16-byte aligned");
+  if (mu_ctx_select_device(ctx) != MU_OK)
+    return mu_set_error(ctx, MU_ERR_CUDA, "kv_cache_append: cannot select device");
+  mu::AppendArgs a{};
+  a.x[0] = k, a.x[1] = v, a.ld = ld, a.slots = slots, a.n_tokens = n_tokens;
+  a.cache[0] = static_cast<uint8_t *>(k_cache), a.cache[1] = static_cast<uint8_t *>(v_cache);
+  a.scale[0] = k_scale, a.scale[1] = v_scale;
+  a.num_pages = num_pages, a.page_size = page_size, a.H = Hkv, a.D = D, a.status = mu_ctx_status_ptr(ctx);
+  if (mu::launch_kv_append(a, dtype, mu_ctx_num_sms(ctx), static_cast<cudaStream_t>(stream)))
+    return mu_set_error(ctx, MU_ERR_CUDA, cudaGetErrorString(cudaGetLastError()));
+  return MU_OK;
+}
+
+} // extern "C"

@@ -19,6 +19,9 @@ enum : int {
   MU_DEV_TIMEOUT_EPILOGUE = 103,
   MU_DEV_TIMEOUT_OTHER = 104,
   MU_DEV_BAD_INDEX = 110,
+  MU_DEV_BAD_PAGE = 111,   // page or slot outside the cache / block table
+  MU_DEV_NO_PAGE = 112,    // free pages, block table or slots too few for the request lengths
+  MU_DEV_BAD_LENGTH = 113, // negative or contradictory request lengths
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {
