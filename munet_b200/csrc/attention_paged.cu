@@ -444,6 +444,386 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_paged_simt_kernel(Page
   }
 }
 
+// ---- tensor-core kernel: bfloat16 queries, head size 64 or 128 -------------------------------------
+// Bound by reading the cache. Sixteen rows (tokens x heads of the group) share every key. Each of the
+// four warps works alone on every fourth tile of 32 keys: it copies the tile's K and V bytes into its
+// own ring in shared memory (cp.async, 16 bytes a lane; MMA_STAGES tiles of 64 D bytes in flight), turns
+// them into fp16 in registers and multiplies with mma.m16n8k16. Nothing but the end of a segment
+// synchronises the CTA.
+//
+// Numbers: e4m3 is exact in fp16. A query row is scaled by a power of two to at most 2^15, which keeps a
+// bfloat16 mantissa exact. A page's K scale multiplies its fp32 scores. Its V scale goes into the weight:
+// with t = s + log2(vs), weights are 2^(t - max t + 12) in fp16 (2^-12 of them lies above the fp16
+// subnormals, so a page of small values that matters keeps its bits), and the softmax sum takes
+// w / vs back out in fp32.
+//
+// Both products may permute what they sum over, so fragments are read straight from the bytes: in q.k lane
+// c of a quad owns dimensions [c D/4, (c+1) D/4); in p.v lane group g owns dimensions [g D/8, (g+1) D/8).
+// 16-byte chunks are XOR-swizzled by the key's row so that those reads meet no bank twice.
+constexpr int MMA_WARPS = 4, MMA_THREADS = 32 * MMA_WARPS, MMA_ROWS = 16, MMA_TILE = 32;
+constexpr int MMA_CTAS_PER_SM = 2;
+template <int D> struct MmaCfg {
+  static constexpr int STAGES = D == 128 ? 3 : 6;
+  static constexpr int TILE_BYTES = MMA_TILE * D;           // of K, and of V
+  static constexpr int WARP_BYTES = STAGES * 2 * TILE_BYTES; // 24 KB
+  static_assert(WARP_BYTES >= MMA_ROWS * D * 4, "a warp's ring also carries its rows at the end");
+};
+
+__device__ __forceinline__ uint32_t f16x2_of_e4m3_lo(uint32_t w) {
+  uint32_t d;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(d) : "r"(w));
+  return d;
+}
+__device__ __forceinline__ uint32_t f16x2_of_e4m3_hi(uint32_t w) {
+  uint32_t d;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(d) : "r"(w));
+  return d;
+}
+__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 16 bytes into shared memory, or 16 zero bytes
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// byte offset of 16-byte chunk `chunk` of row `row` in a tile
+template <int D> __device__ __forceinline__ uint32_t tile_at(int row, int chunk) {
+  if constexpr (D == 128)
+    return row * 128 + ((chunk ^ (row & 7)) << 4);
+  else
+    return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
+}
+__device__ __forceinline__ bool has_nan_e4m3(uint32_t w) {
+  return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+}
+
+// Page of a half tile (16 keys never leave a page) and its scales, one per lane.
+struct HalfPage {
+  int page; // -1: none
+  float ks, lv, iv; // K scale, log2 and reciprocal of the V scale
+};
+__device__ __forceinline__ HalfPage load_half(const PagedArgs &a, const Segment &g, int key, int end) {
+  HalfPage h;
+  h.page = -1, h.ks = 0.f, h.lv = -INFINITY, h.iv = 0.f;
+  if (key < end) {
+    const int page = a.table[1ll * g.b * a.table_stride + static_cast<unsigned>(key) / static_cast<unsigned>(a.page_size)];
+    if (page >= 0 && page < a.num_pages) {
+      const long long t = 1ll * page * a.Hkv + g.head;
+      const float vs = fmaxf(a.vs[t], 0x1p-64f);
+      h.page = page, h.ks = a.ks[t], h.lv = log2f(vs), h.iv = 1.f / vs;
+    } else {
+      atomicCAS(a.status, 0, MU_DEV_BAD_PAGE);
+    }
+  }
+  return h;
+}
+
+template <int D> __global__ void __launch_bounds__(MMA_THREADS, MMA_CTAS_PER_SM) attention_paged_mma_kernel(PagedArgs a) {
+  using Cfg = MmaCfg<D>;
+  constexpr int S = Cfg::STAGES, KW = D / 16, NT = D / 8; // k-steps of q.k = 32-bit words a lane reads per key; n-tiles of p.v
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  __shared__ long long warp_sum[MMA_WARPS];
+  __shared__ float2 ml_s[MMA_WARPS][MMA_ROWS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, grp = lane >> 2, quad = lane & 3;
+  unsigned char *ring = smem_raw + warp * Cfg::WARP_BYTES;
+  long long *upto = reinterpret_cast<long long *>(smem_raw + MMA_WARPS * Cfg::WARP_BYTES);
+  const uint32_t ring_u32 = smem_u32(ring);
+
+  if (tid == 0)
+    a.items[blockIdx.x].used = 0;
+  const long long total = scan_units<MMA_THREADS, MMA_ROWS>(a, upto, warp_sum);
+  if (total == 0)
+    return;
+  Walk walk(total, blockIdx.x, gridDim.x);
+  Segment g;
+  Seq s;
+  const unsigned ps = a.page_size;
+  while (walk.next<MMA_ROWS>(a, upto, g, s)) {
+    // limits: least over the tile's rows, most over them, and this lane's two rows
+    const int least = row_limit(a, s, g.row0), most = row_limit(a, s, g.row0 + g.n_rows - 1);
+    const int lim0 = row_limit(a, s, g.row0 + grp), lim1 = row_limit(a, s, g.row0 + grp + 8);
+    const int first = g.chunk0 * CHUNK + warp * MMA_TILE, end = min(most, (g.chunk0 + g.chunks) * CHUNK);
+    const int tiles = end > first ? (end - first + CHUNK - 1) / CHUNK : 0; // this warp's, CHUNK apart
+    auto half_key = [&](int batch) { return first + (batch * 16 + (lane >> 1)) * CHUNK + (lane & 1) * 16; };
+    HalfPage cur = load_half(a, g, half_key(0), end), nxt = load_half(a, g, half_key(1), end);
+
+    auto issue = [&](int i, const HalfPage &hp) {
+      if (i < tiles) {
+        const uint32_t st = ring_u32 + (i % S) * 2 * Cfg::TILE_BYTES;
+        const int key0 = first + i * CHUNK;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const int page = __shfl_sync(~0u, hp.page, (i & 15) * 2 + hf);
+          const int key = key0 + 16 * hf, live = page >= 0 ? s.seen - key : 0; // rows behind it hold anything
+          const unsigned in_page = static_cast<unsigned>(key) % ps;
+          const long long off = page >= 0 ? ((1ll * page * a.Hkv + g.head) * ps + in_page) * D + lane * 16 : 0;
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j) {
+            const int idx = lane + 32 * j, row = idx / (D / 16), chunk = idx % (D / 16);
+            const uint32_t at = tile_at<D>(hf * 16 + row, chunk);
+            const bool real = row < live;
+            const long long o = real ? off + 512 * j : 0;
+            cp_async16(st + at, a.kc + o, real);
+            cp_async16(st + Cfg::TILE_BYTES + at, a.vc + o, real);
+          }
+        }
+      }
+      cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i)
+      issue(i, cur);
+
+    // queries: fp16 fragments and each row's factor back
+    uint32_t qf[KW][4];
+    float fac[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float v[D / 4];
+      const bool live = grp + 8 * r < g.n_rows;
+      const long long row = g.row0 + grp + 8 * r;
+      const __nv_bfloat16 *qp = static_cast<const __nv_bfloat16 *>(a.q) +
+                                (live ? (s.q0 + row / a.G) * a.q_ld + (1ll * g.head * a.G + row % a.G) * D + quad * (D / 4) : 0);
+      if ((reinterpret_cast<uintptr_t>(qp) & 15u) == 0 && live) {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          const uint4 u = *(reinterpret_cast<const uint4 *>(qp) + i);
+          v[8 * i] = bf16_lo(u.x), v[8 * i + 1] = bf16_hi(u.x), v[8 * i + 2] = bf16_lo(u.y), v[8 * i + 3] = bf16_hi(u.y);
+          v[8 * i + 4] = bf16_lo(u.z), v[8 * i + 5] = bf16_hi(u.z), v[8 * i + 6] = bf16_lo(u.w), v[8 * i + 7] = bf16_hi(u.w);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i)
+          v[i] = live ? __bfloat162float(qp[i]) : 0.f;
+      }
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i)
+        top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+      top = max(top, __shfl_xor_sync(~0u, top, 1));
+      top = max(top, __shfl_xor_sync(~0u, top, 2));
+      const int e = min(max(static_cast<int>(top >> 23) - 127 - 14, -100), 113);
+      const float f = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      fac[r] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * a.scale_log2;
+#pragma unroll
+      for (int i = 0; i < KW; ++i) {
+        qf[i][r] = f16x2(v[4 * i] * f, v[4 * i + 1] * f);
+        qf[i][r + 2] = f16x2(v[4 * i + 2] * f, v[4 * i + 3] * f);
+      }
+    }
+
+    float o[NT][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+      o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+
+    for (int i = 0; i < tiles; ++i) {
+      if ((i & 15) == 0 && i > 0)
+        cur = nxt, nxt = load_half(a, g, half_key((i >> 4) + 1), end);
+      issue(i + S - 1, ((i + S - 1) >> 4) == (i >> 4) ? cur : nxt);
+      cp_async_wait<S - 1>();
+      __syncwarp();
+      const unsigned char *kt = ring + (i % S) * 2 * Cfg::TILE_BYTES, *vt = kt + Cfg::TILE_BYTES;
+      const int key0 = first + i * CHUNK;
+
+      float sc[4][4];
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt) {
+        sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+        uint32_t w[KW];
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          const uint4 u = *reinterpret_cast<const uint4 *>(kt + tile_at<D>(nt * 8 + grp, quad * (D / 64) + c));
+          w[4 * c] = u.x, w[4 * c + 1] = u.y, w[4 * c + 2] = u.z, w[4 * c + 3] = u.w;
+        }
+#pragma unroll
+        for (int k = 0; k < KW; ++k)
+          mma_f16(sc[nt], qf[k], f16x2_of_e4m3_lo(w[k]), f16x2_of_e4m3_hi(w[k]));
+      }
+      float iv[2];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int src = (i & 15) * 2 + hf;
+        const float ks = __shfl_sync(~0u, cur.ks, src), lv = __shfl_sync(~0u, cur.lv, src);
+        iv[hf] = __shfl_sync(~0u, cur.iv, src);
+#pragma unroll
+        for (int nt = 2 * hf; nt < 2 * hf + 2; ++nt) {
+          sc[nt][0] = fmaf(sc[nt][0], ks * fac[0], lv), sc[nt][1] = fmaf(sc[nt][1], ks * fac[0], lv);
+          sc[nt][2] = fmaf(sc[nt][2], ks * fac[1], lv), sc[nt][3] = fmaf(sc[nt][3], ks * fac[1], lv);
+        }
+      }
+      const bool edge = key0 + MMA_TILE > least;
+      if (edge) {
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int key = key0 + nt * 8 + quad * 2 + e;
+            if (key >= lim0)
+              sc[nt][e] = -INFINITY;
+            if (key >= lim1)
+              sc[nt][2 + e] = -INFINITY;
+          }
+      }
+      float t0 = m0, t1 = m1;
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt)
+        t0 = fmaxf(t0, fmaxf(sc[nt][0], sc[nt][1])), t1 = fmaxf(t1, fmaxf(sc[nt][2], sc[nt][3]));
+      t0 = fmaxf(t0, __shfl_xor_sync(~0u, t0, 1)), t1 = fmaxf(t1, __shfl_xor_sync(~0u, t1, 1));
+      t0 = fmaxf(t0, __shfl_xor_sync(~0u, t0, 2)), t1 = fmaxf(t1, __shfl_xor_sync(~0u, t1, 2));
+      const float ref0 = t0 == -INFINITY ? 0.f : t0 - 12.f, ref1 = t1 == -INFINITY ? 0.f : t1 - 12.f;
+      if (__any_sync(~0u, t0 != m0 || t1 != m1)) {
+        const float f0 = m0 == -INFINITY ? 0.f : ex2_approx(m0 - t0), f1 = m1 == -INFINITY ? 0.f : ex2_approx(m1 - t1);
+        l0 *= f0, l1 *= f1;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          o[j][0] *= f0, o[j][1] *= f0, o[j][2] *= f1, o[j][3] *= f1;
+        m0 = t0, m1 = t1;
+      }
+      uint32_t pf[2][4];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          float (&x)[4] = sc[2 * hf + n];
+          x[0] = ex2_approx(x[0] - ref0), x[1] = ex2_approx(x[1] - ref0);
+          x[2] = ex2_approx(x[2] - ref1), x[3] = ex2_approx(x[3] - ref1);
+          sum0 += x[0] + x[1], sum1 += x[2] + x[3];
+          pf[hf][2 * n] = f16x2(x[0], x[1]), pf[hf][2 * n + 1] = f16x2(x[2], x[3]);
+        }
+        l0 = fmaf(sum0, iv[hf], l0), l1 = fmaf(sum1, iv[hf], l1);
+      }
+
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        constexpr int VW = D / 32; // 32-bit words a lane reads per key
+        uint32_t w[4][VW];         // keys 2 quad, 2 quad + 1, and both + 8
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = hf * 16 + 2 * quad + (r & 1) + 8 * (r >> 1);
+          if constexpr (D == 128) {
+            const uint4 u = *reinterpret_cast<const uint4 *>(vt + tile_at<D>(row, grp));
+            w[r][0] = u.x, w[r][1] = u.y, w[r][2] = u.z, w[r][3] = u.w;
+          } else {
+            const uint2 u = *reinterpret_cast<const uint2 *>(vt + tile_at<D>(row, grp >> 1) + (grp & 1) * 8);
+            w[r][0] = u.x, w[r][1] = u.y;
+          }
+        }
+        auto product = [&](float (&c)[4], const uint32_t (&p)[4], const uint32_t (&x)[4][VW], int j) {
+          const uint32_t sel = j & 2 ? 0x7362 : 0x5140; // bytes of two keys side by side, two dimensions
+          const uint32_t b0 = __byte_perm(x[0][j >> 2], x[1][j >> 2], sel), b1 = __byte_perm(x[2][j >> 2], x[3][j >> 2], sel);
+          if (j & 1)
+            mma_f16(c, p, f16x2_of_e4m3_hi(b0), f16x2_of_e4m3_hi(b1));
+          else
+            mma_f16(c, p, f16x2_of_e4m3_lo(b0), f16x2_of_e4m3_lo(b1));
+        };
+        bool nan = false;
+        if (edge) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int q = 0; q < VW; ++q)
+              nan |= has_nan_e4m3(w[r][q]);
+          nan = __any_sync(~0u, nan);
+        }
+        if (!nan) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+            product(o[j], pf[hf], w, j);
+        } else {
+          // A NaN among keys that some rows may not see: zero weights would not keep it out, so the keys go
+          // one at a time and a row takes only those it sees.
+#pragma unroll 1
+          for (int t = 0; t < 16; ++t) {
+            const int key = key0 + hf * 16 + t;
+            uint32_t x[4][VW], p[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const bool mine = t == 2 * quad + (r & 1) + 8 * (r >> 1);
+#pragma unroll
+              for (int q = 0; q < VW; ++q)
+                x[r][q] = mine ? w[r][q] : 0u;
+            }
+            const uint32_t keep = (t & 7) >> 1 == quad ? (t & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              p[r] = (r >> 1) == (t >> 3) ? pf[hf][r] & keep : 0u;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              float c[4] = {0.f, 0.f, 0.f, 0.f};
+              product(c, p, x, j);
+              if (key < lim0)
+                o[j][0] += c[0], o[j][1] += c[1];
+              if (key < lim1)
+                o[j][2] += c[2], o[j][3] += c[3];
+            }
+          }
+        }
+      }
+      __syncwarp(); // the stage may be overwritten
+    }
+    cp_async_wait<0>();
+    __syncwarp();
+
+    // join the warps: every ring now carries its warp's rows
+    l0 += __shfl_xor_sync(~0u, l0, 1), l1 += __shfl_xor_sync(~0u, l1, 1);
+    l0 += __shfl_xor_sync(~0u, l0, 2), l1 += __shfl_xor_sync(~0u, l1, 2);
+    if (quad == 0)
+      ml_s[warp][grp] = make_float2(m0 - 12.f, l0), ml_s[warp][grp + 8] = make_float2(m1 - 12.f, l1);
+    float *mine = reinterpret_cast<float *>(ring);
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+      if (grp + 8 * r < g.n_rows) {
+        float *p = mine + (grp + 8 * r) * D + quad * (D / 4);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int j = 0; j < NT; j += 4)
+            *reinterpret_cast<float4 *>(p + e * NT + j) =
+                make_float4(o[j][2 * r + e], o[j + 1][2 * r + e], o[j + 2][2 * r + e], o[j + 3][2 * r + e]);
+      }
+    __syncthreads();
+    for (int e = tid; e < g.n_rows * D; e += MMA_THREADS) {
+      const int r = e / D, d = e % D;
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < MMA_WARPS; ++w)
+        M = fmaxf(M, ml_s[w][r].x);
+      float sum = 0.f, x = 0.f;
+#pragma unroll
+      for (int w = 0; w < MMA_WARPS; ++w) {
+        const float f = rel_weight(ml_s[w][r].x, M);
+        sum = fmaf(f, ml_s[w][r].y, sum);
+        x = fmaf(f, reinterpret_cast<const float *>(smem_raw + w * Cfg::WARP_BYTES)[e], x);
+      }
+      if (g.slot < 0) {
+        const long long row = g.row0 + r;
+        store_out(static_cast<__nv_bfloat16 *>(a.out) + (s.q0 + row / a.G) * a.out_ld +
+                      (1ll * g.head * a.G + row % a.G) * D + d,
+                  sum == 0.f ? 0.f : x / sum);
+      } else {
+        const long long pr = 1ll * g.slot * a.rows_per_tile + r;
+        a.part_o[pr * D + d] = x;
+        if (d == 0)
+          a.part_ml[pr] = make_float2(M, sum);
+      }
+    }
+    __syncthreads();
+  }
+}
+
 // ---- joining the pieces ---------------------------------------------------------------------------
 // One CTA per (first CTA of a split item, row). Launched so that it may become resident while the main
 // kernel drains; griddepcontrol.wait is what orders its reads after that kernel's writes.
@@ -540,6 +920,23 @@ template <typename T> int launch_simt_dim(const PagedArgs &a, int num_sms, cudaS
   return launch_simt_rows<T, 1, 8>(a, num_sms, st);
 }
 
+template <int D> int launch_mma(PagedArgs a, int num_sms, cudaStream_t st) {
+  const size_t smem = MMA_WARPS * MmaCfg<D>::WARP_BYTES + 8ull * a.B;
+  static PerDeviceOnce once;
+  if (once.get() < 0) {
+    if (cudaFuncSetAttribute(attention_paged_mma_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             MMA_WARPS * MmaCfg<D>::WARP_BYTES + 8 * MU_ATTENTION_PAGED_MAX_REQUESTS) != cudaSuccess)
+      return 2;
+    once.set(1);
+  }
+  const int ctas = num_sms * MMA_CTAS_PER_SM;
+  a.rows_per_tile = MMA_ROWS;
+  attention_paged_mma_kernel<D><<<ctas, MMA_THREADS, smem, st>>>(a);
+  if (cudaGetLastError() != cudaSuccess)
+    return 2;
+  return launch_join<__nv_bfloat16>(a, ctas, st);
+}
+
 // 0 ok, 1 dtype not implemented, 2 CUDA error
 int launch_attention_paged(PagedArgs a, void *workspace, int dtype, int num_sms, cudaStream_t st) {
   const size_t ctas = static_cast<size_t>(num_sms) * MAX_CTAS_PER_SM;
@@ -551,6 +948,10 @@ int launch_attention_paged(PagedArgs a, void *workspace, int dtype, int num_sms,
   a.items = reinterpret_cast<SplitItem *>(w);
   if (dtype == F32)
     return launch_simt_dim<float>(a, num_sms, st);
+  if (dtype == BF16 && a.D == 128)
+    return launch_mma<128>(a, num_sms, st);
+  if (dtype == BF16 && a.D == 64)
+    return launch_mma<64>(a, num_sms, st);
   if (dtype == BF16)
     return launch_simt_dim<__nv_bfloat16>(a, num_sms, st);
   return 1;

@@ -83,11 +83,12 @@ def append(x, slots, cache, scale, page):
 
 
 def attention(q, kc, vc, ks, vs, table, query_start, seq, page, causal):
-    """(out, weight, spread) [n,Hq,D]: the result, sum_j p_j |v_j| and, per row, max_j sum_d |q_d k_jd| / sqrt(D)."""
+    """(out, weight, spread, top): the result and sum_j p_j |v_j|, [n,Hq,D]; per row max_j sum_d |q_d k_jd| / sqrt(D)
+    and max_j p_j vs_j (vs: the scale of key j's page)."""
     n, Hq, D = q.shape
     Hkv = kc.shape[1]
     G = Hq // Hkv
-    out, weight, spread = np.zeros(q.shape), np.zeros(q.shape), np.zeros((n, Hq))
+    out, weight, spread, top = np.zeros(q.shape), np.zeros(q.shape), np.zeros((n, Hq)), np.zeros((n, Hq))
     for b in range(len(seq)):
         L, a, e = seq[b], query_start[b], query_start[b + 1]
         ids = table[b, :-(-L // page)]
@@ -103,8 +104,9 @@ def attention(q, kc, vc, ks, vs, table, query_start, seq, page, causal):
                     w = np.exp(s - s.max())
                     w /= w.sum()
                     out[i, g], weight[i, g] = w @ v[:lim], w @ np.abs(v[:lim])
+                    top[i, g] = (w * np.repeat(vs[ids, h], page)[:lim]).max()
                     spread[i, g] = (np.abs(k[:lim]) @ np.abs(q[i, g])).max() / math.sqrt(D)
-    return out, weight, spread
+    return out, weight, spread, top
 
 
 def sample(x, u, T=1.0, k=0, p=1.0, min_p=0.0):
