@@ -5,12 +5,13 @@
 // Token i of a request with n new tokens and `len` tokens in the cache sits at position len - n + i;
 // causal attention lets it see j <= that position. A row that sees nothing gives zeros.
 //
-// Work split (both kernels): a request's rows (token, head of the group) are cut into row tiles, its
-// keys into chunks of 128 tokens; (request, KV head, row tile, chunk) in this order is one long list of
-// units that the resident CTAs share out evenly, whatever the lengths are. A CTA walks its range as
-// segments, one per (request, head, row tile). A segment that covers all chunks writes its rows; one
-// that does not leaves (running maximum, sum, weighted values) in the workspace, and a second small
-// kernel joins them. No atomics: results do not depend on the order in which CTAs run.
+// Work split: a request's rows (token, head of the group) are cut into row tiles, its keys into chunks;
+// (request, KV head, row tile, chunk) in this order is one long list of units that the resident workers
+// (warps of the tensor-core kernel, CTAs of the CUDA-core one) share out evenly, whatever the lengths
+// are. A worker walks its range as segments, one per (request, head, row tile). A segment that covers
+// all chunks writes its rows; one that does not leaves (running maximum, sum, weighted values) in the
+// workspace, and a second small kernel joins the pieces. No atomics: results do not depend on the order
+// in which workers run.
 #include "../../include/munet_b200.h"
 #include "common.h"
 #include "ptx.cuh"
@@ -40,13 +41,12 @@ struct PagedArgs {
   int *status;
 };
 
-// A (request, head, row tile) whose chunks went to more than one CTA; entry c belongs to the CTA that
-// holds its first chunk. Its later pieces are the first segments of CTAs c+1 .. last_cta.
+// A (request, head, row tile) whose chunks went to more than one worker; entry w belongs to the worker
+// that holds its first chunk. Its later pieces are the first segments of workers w+1 .. last.
+// n_rows 0: no such item.
 struct SplitItem {
-  int used, first_slot, last_cta, row0, n_rows, q0, head;
+  int n_rows, first_slot, last, row0, q0, head;
 };
-
-constexpr int CHUNK = 128; // tokens per unit
 
 struct Seq {
   int q0, nq, len;  // first row of q, new tokens, tokens in the cache (as given)
@@ -70,32 +70,33 @@ __device__ __forceinline__ Seq load_seq(const PagedArgs &a, int b) {
   }
   return s;
 }
-__device__ __forceinline__ int chunks_of(const Seq &s) { return s.seen > 0 ? (s.seen - 1) / CHUNK + 1 : 1; }
-__device__ __forceinline__ long long units_of(const PagedArgs &a, const Seq &s, int R) {
+template <int CHUNK> __device__ __forceinline__ int chunks_of(const Seq &s) {
+  return s.seen > 0 ? (s.seen - 1) / CHUNK + 1 : 1;
+}
+template <int R, int CHUNK> __device__ __forceinline__ long long units_of(const PagedArgs &a, const Seq &s) {
   if (s.nq <= 0)
     return 0;
-  const long long rows = 1ll * s.nq * a.G;
-  return a.Hkv * ((rows + R - 1) / R) * chunks_of(s);
+  const unsigned rows = static_cast<unsigned>(s.nq) * a.G; // n_tokens * Hq fits 31 bits
+  return 1ll * a.Hkv * ((rows + R - 1) / R) * chunks_of<CHUNK>(s);
 }
 // Keys row `row` of a request may see.
-__device__ __forceinline__ int row_limit(const PagedArgs &a, const Seq &s, long long row) {
-  if (row >= 1ll * s.nq * a.G)
+__device__ __forceinline__ int row_limit(const PagedArgs &a, const Seq &s, int row) {
+  if (row >= s.nq * a.G)
     return 0;
   if (!a.causal)
     return s.seen;
-  const int i = static_cast<int>(row / a.G);
-  return max(0, min(s.seen, s.len - s.nq + i + 1));
+  return max(0, min(s.seen, s.len - s.nq + row / a.G + 1));
 }
 
 // Inclusive prefix of units over the requests into shared memory; returns the total.
-template <int THREADS, int R>
+template <int THREADS, int R, int CHUNK>
 __device__ __forceinline__ long long scan_units(const PagedArgs &a, long long *upto, long long *warp_sum) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (a.B + THREADS - 1) / THREADS;
   const int b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
   long long sum = 0;
   for (int b = b0; b < b1; ++b) {
-    sum += units_of(a, load_seq(a, b), R);
+    sum += units_of<R, CHUNK>(a, load_seq(a, b));
     upto[b] = sum;
   }
   long long inc = sum;
@@ -122,40 +123,50 @@ __device__ __forceinline__ long long scan_units(const PagedArgs &a, long long *u
 }
 
 struct Segment {
-  int b, head, n_rows;   // request, KV head, rows of the tile that exist
-  long long row0;        // first row of the tile
-  int chunk0, chunks;    // range of this CTA
-  int slot;              // -1: complete
+  int b, head, n_rows, row0; // request, KV head, rows of the tile that exist, first of them
+  int chunk0, chunks;        // range of this worker
+  int slot;                  // -1: complete
 };
 
-// Walks one CTA's share of the unit list.
-struct Walk {
-  long long u, end, total;
-  int grid, cta, b;
-  bool first;
-  __device__ __forceinline__ Walk(long long total_, int cta_, int grid_) : total(total_), cta(cta_), b(0), first(true) {
-    grid = static_cast<int>(min(static_cast<long long>(grid_), total_)); // every active CTA has a unit
-    if (cta < grid) {
-      u = total / grid * cta + total % grid * cta / grid;
-      end = total / grid * (cta + 1) + total % grid * (cta + 1) / grid;
-    } else {
-      u = end = 0;
-    }
+// Quotient and remainder; units of one request hardly ever need 64 bits.
+__device__ __forceinline__ long long div_rem(long long x, int d, int &rem) {
+  if (x >> 32 == 0) {
+    const unsigned q = static_cast<unsigned>(x) / static_cast<unsigned>(d);
+    rem = static_cast<int>(static_cast<unsigned>(x) - q * static_cast<unsigned>(d));
+    return q;
   }
-  // CTA that holds unit x: the largest c with start(c) <= x. start(c) = floor(total * c / grid).
+  rem = static_cast<int>(x % d);
+  return x / d;
+}
+
+// Walks one worker's share of the unit list.
+template <int R, int CHUNK> struct Walk {
+  long long u, end, total;
+  int workers, me, b;
+  bool first;
+  __device__ __forceinline__ long long start(int w) const { // floor(total * w / workers)
+    return total / workers * w + total % workers * w / workers;
+  }
+  __device__ __forceinline__ Walk(long long total_, int me_, int workers_) : total(total_), me(me_), b(0), first(true) {
+    workers = static_cast<int>(min(static_cast<long long>(workers_), total_)); // every active one has a unit
+    u = end = 0;
+    if (me < workers)
+      u = start(me), end = start(me + 1);
+  }
+  // the worker that holds unit x: the largest w with start(w) <= x
   __device__ __forceinline__ int owner(long long x) const {
-    int lo = 0, hi = grid - 1;
+    int lo = 0, hi = workers - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (total / grid * mid + total % grid * mid / grid <= x)
+      if (start(mid) <= x)
         lo = mid;
       else
         hi = mid - 1;
     }
     return lo;
   }
-  template <int R>
-  __device__ __forceinline__ bool next(const PagedArgs &a, const long long *upto, Segment &g, Seq &s) {
+  // The next segment. `leader`: the thread that notes down a split item.
+  __device__ __forceinline__ bool next(const PagedArgs &a, const long long *upto, Segment &g, Seq &s, bool leader) {
     if (u >= end)
       return false;
     int lo = b, hi = a.B - 1;
@@ -169,24 +180,22 @@ struct Walk {
     b = lo;
     s = load_seq(a, b);
     const long long base = b ? upto[b - 1] : 0;
-    const long long rows = 1ll * s.nq * a.G;
-    const long long tiles = (rows + R - 1) / R;
-    const int nc = chunks_of(s);
-    const long long item = (u - base) / nc;
+    const int rows = s.nq * a.G, tiles = (rows + R - 1) / R, nc = chunks_of<CHUNK>(s);
     g.b = b;
-    g.head = static_cast<int>(item / tiles);
-    g.row0 = item % tiles * R;
-    g.n_rows = static_cast<int>(min(rows - g.row0, static_cast<long long>(R)));
-    g.chunk0 = static_cast<int>((u - base) % nc);
+    const long long item = div_rem(u - base, nc, g.chunk0);
+    int tile;
+    g.head = static_cast<int>(div_rem(item, tiles, tile));
+    g.row0 = tile * R;
+    g.n_rows = min(rows - g.row0, R);
     g.chunks = static_cast<int>(min(static_cast<long long>(nc - g.chunk0), end - u));
     g.slot = -1;
     if (g.chunks < nc) {
-      g.slot = 2 * cta + (first ? 0 : 1);
-      if (g.chunk0 == 0 && threadIdx.x == 0) {
+      g.slot = 2 * me + (first ? 0 : 1);
+      if (g.chunk0 == 0 && leader) {
         SplitItem it;
-        it.used = 1, it.first_slot = g.slot, it.last_cta = owner(u + nc - 1);
-        it.row0 = static_cast<int>(g.row0), it.n_rows = g.n_rows, it.q0 = s.q0, it.head = g.head;
-        a.items[cta] = it;
+        it.first_slot = g.slot, it.last = owner(u + nc - 1);
+        it.row0 = g.row0, it.n_rows = g.n_rows, it.q0 = s.q0, it.head = g.head;
+        a.items[me] = it;
       }
     }
     u += g.chunks;
@@ -202,11 +211,11 @@ __device__ __forceinline__ float load_in(const __nv_bfloat16 *p) { return __bflo
 // weight of a piece whose running maximum is m where the whole's is M
 __device__ __forceinline__ float rel_weight(float m, float M) { return M == -INFINITY ? 1.f : ex2_approx(m - M); }
 
-// ---- CUDA-core kernel: float32, and every head size -----------------------------------------------
-// float32 queries keep float32 products and sums. Per warp a tile of 32 keys: for the scores a lane
-// owns a key (its row is D consecutive bytes), for the weighted values a lane owns four dimensions.
-// VB: bytes per load (16 / 4 / 1 by the head size), RT rows share every key, NA units per lane.
-constexpr int SIMT_WARPS = 4, SIMT_THREADS = 32 * SIMT_WARPS;
+// ---- CUDA-core kernel: head sizes that are no multiple of 16 ---------------------------------------
+// float32 products and sums. Per warp a tile of 32 keys: for the scores a lane owns a key (its row is D
+// consecutive bytes), for the weighted values a lane owns four dimensions (one, where D is odd).
+// VB: bytes per load (4 or 1 by the head size), RT rows share every key, NA units per lane.
+constexpr int SIMT_WARPS = 4, SIMT_THREADS = 32 * SIMT_WARPS, SIMT_CHUNK = 32 * SIMT_WARPS;
 
 __device__ __forceinline__ float2 fp8x2_to_float2(uint32_t two) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3);
@@ -230,20 +239,20 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_paged_simt_kernel(Page
   float *o_s = q_s + RT * Dq;                                        // [warps][groups][RT][D]
 
   if (tid == 0)
-    a.items[blockIdx.x].used = 0;
-  const long long total = scan_units<SIMT_THREADS, RT>(a, upto, warp_sum);
+    a.items[blockIdx.x].n_rows = 0;
+  const long long total = scan_units<SIMT_THREADS, RT, SIMT_CHUNK>(a, upto, warp_sum);
   if (total == 0)
     return;
-  Walk walk(total, blockIdx.x, gridDim.x);
+  Walk<RT, SIMT_CHUNK> walk(total, blockIdx.x, gridDim.x);
   Segment g;
   Seq s;
   const unsigned ps = a.page_size;
-  while (walk.next<RT>(a, upto, g, s)) {
+  while (walk.next(a, upto, g, s, tid == 0)) {
     for (int e = tid; e < RT * Dq; e += SIMT_THREADS) {
       const int r = e / Dq, d = e - r * Dq;
       float v = 0.f;
       if (r < g.n_rows && d < a.D) {
-        const long long row = g.row0 + r;
+        const int row = g.row0 + r;
         v = load_in(static_cast<const T *>(a.q) + (s.q0 + row / a.G) * a.q_ld +
                     (1ll * g.head * a.G + row % a.G) * a.D + d);
       }
@@ -268,7 +277,7 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_paged_simt_kernel(Page
           acc[r][n][w] = 0.f;
     }
     for (int c = g.chunk0; c < g.chunk0 + g.chunks; ++c) {
-      const int base = c * CHUNK + warp * 32;
+      const int base = c * SIMT_CHUNK + warp * 32;
       if (base >= most)
         break;
       const int j = base + lane;
@@ -291,22 +300,7 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_paged_simt_kernel(Page
         sc[r] = 0.f;
       if (row >= 0) {
         const uint8_t *k = a.kc + row * a.D;
-        if constexpr (VB == 16) {
-#pragma unroll 2
-          for (int d = 0; d < a.D; d += 16) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4 *>(k + d));
-            const uint32_t w4[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 x = fp8x2_to_float2(w4[i] & 0xffffu), y = fp8x2_to_float2(w4[i] >> 16);
-#pragma unroll
-              for (int r = 0; r < RT; ++r) {
-                const float4 qv = *reinterpret_cast<const float4 *>(q_s + r * Dq + d + 4 * i);
-                sc[r] = fmaf(qv.x, x.x, fmaf(qv.y, x.y, fmaf(qv.z, y.x, fmaf(qv.w, y.y, sc[r]))));
-              }
-            }
-          }
-        } else if constexpr (VB == 4) {
+        if constexpr (VB == 4) {
           for (int d = 0; d < a.D; d += 4) {
             const uint32_t w4 = __ldg(reinterpret_cast<const uint32_t *>(k + d));
             const float2 x = fp8x2_to_float2(w4 & 0xffffu), y = fp8x2_to_float2(w4 >> 16);
@@ -429,7 +423,7 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_paged_simt_kernel(Page
         sum += f * ml_s[w][r].y, o += f * x;
       }
       if (g.slot < 0) {
-        const long long row = g.row0 + r;
+        const int row = g.row0 + r;
         store_out(static_cast<T *>(a.out) + (s.q0 + row / a.G) * a.out_ld +
                       (1ll * g.head * a.G + row % a.G) * a.D + d,
                   sum == 0.f ? 0.f : o / sum);
@@ -444,29 +438,36 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_paged_simt_kernel(Page
   }
 }
 
-// ---- tensor-core kernel: bfloat16 queries, head size 64 or 128 -------------------------------------
-// Bound by reading the cache. Sixteen rows (tokens x heads of the group) share every key. Each of the
-// four warps works alone on every fourth tile of 32 keys: it copies the tile's K and V bytes into its
-// own ring in shared memory (cp.async, 16 bytes a lane; MMA_STAGES tiles of 64 D bytes in flight), turns
-// them into fp16 in registers and multiplies with mma.m16n8k16. Nothing but the end of a segment
+// ---- tensor-core kernel: head sizes that are multiples of 16 ----------------------------------------
+// Bound by reading the cache. A warp is a worker: it walks its keys in tiles (32 of them, 16 for head
+// sizes above 128), copies a tile's K and V bytes into its own two stages of shared memory (cp.async, 16
+// bytes a lane), turns them into fp16 in registers and multiplies with mma.m16n8k16. Nothing ever
 // synchronises the CTA.
+//
+// The keys are the M side of both products, so that eight rows fill the N side: S' = K q' is 16 keys x 8
+// rows, O' = V' P' is 16 dimensions x 8 rows (with the rows as M, half to 15/16 of every product would be
+// thrown away for single tokens). P leaves the first product's layout for the second's by movmatrix.
+// Both products may permute what they sum over and O' its rows, so operands are read straight from the
+// bytes: lane (g, c) = (lane / 4, lane % 4) reads, of keys g and g + 8, dimensions [c D/4, (c+1) D/4), and,
+// of keys 2c, 2c+1, 2c+8, 2c+9, dimensions [g D/8, (g+1) D/8).
 //
 // Numbers: e4m3 is exact in fp16. A query row is scaled by a power of two to at most 2^15, which keeps a
 // bfloat16 mantissa exact. A page's K scale multiplies its fp32 scores. Its V scale goes into the weight:
-// with t = s + log2(vs), weights are 2^(t - max t + 12) in fp16 (2^-12 of them lies above the fp16
-// subnormals, so a page of small values that matters keeps its bits), and the softmax sum takes
-// w / vs back out in fp32.
-//
-// Both products may permute what they sum over, so fragments are read straight from the bytes: in q.k lane
-// c of a quad owns dimensions [c D/4, (c+1) D/4); in p.v lane group g owns dimensions [g D/8, (g+1) D/8).
-// 16-byte chunks are XOR-swizzled by the key's row so that those reads meet no bank twice.
-constexpr int MMA_WARPS = 4, MMA_THREADS = 32 * MMA_WARPS, MMA_ROWS = 16, MMA_TILE = 32;
-constexpr int MMA_CTAS_PER_SM = 2;
-template <int D> struct MmaCfg {
-  static constexpr int STAGES = D == 128 ? 3 : 6;
-  static constexpr int TILE_BYTES = MMA_TILE * D;           // of K, and of V
-  static constexpr int WARP_BYTES = STAGES * 2 * TILE_BYTES; // 24 KB
-  static_assert(WARP_BYTES >= MMA_ROWS * D * 4, "a warp's ring also carries its rows at the end");
+// with t = s + log2(vs), weights are 2^(t - max t + 15) in fp16 (so that a page of small values that
+// matters keeps its bits above fp16's subnormals), and the softmax sum takes w / vs back out in fp32.
+// SPLIT (float32): queries and weights are the sum of two fp16 numbers, 22 bits, and every product starts
+// from zero and is added in fp32, because the tensor core rounds its running sum towards zero.
+constexpr float W_EXP = 15.f; // the largest weight of a row is 2^15: fp16 ends at 65504
+
+template <int DP, int NR, bool SPLIT> struct MmaCfg {
+  static constexpr int WARPS = 4, THREADS = 32 * WARPS;
+  static constexpr int CTAS_PER_SM = (DP <= 128 && NR == 1) ? 3 : 2; // 12 or 8 warps: by their registers
+  static constexpr int R = 8 * NR;
+  static constexpr int TILE = DP <= 128 ? 32 : 16, CHUNK = 64, MT = TILE / 16;
+  // bytes between keys: whole bank cycles are swizzled, others padded
+  static constexpr int PITCH = DP == 64 || DP == 128 || DP == 256 ? DP : DP + 16;
+  static constexpr int TILE_BYTES = TILE * PITCH, WARP_BYTES = 4 * TILE_BYTES; // K and V, two stages
+  static constexpr int KW = DP / 16, VW = DP / 32, NT = DP / 16; // 32-bit words of K / V a lane reads per key; d-tiles
 };
 
 __device__ __forceinline__ uint32_t f16x2_of_e4m3_lo(uint32_t w) {
@@ -484,10 +485,20 @@ __device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
   return d;
 }
+// what is left of two floats after their rounding to fp16
+__device__ __forceinline__ uint32_t f16x2_rest(float lo, float hi, uint32_t h) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+  return f16x2(lo - f.x, hi - f.y);
+}
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+  return d;
 }
 // 16 bytes into shared memory, or 16 zero bytes
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool real) {
@@ -497,18 +508,44 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N> __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-// byte offset of 16-byte chunk `chunk` of row `row` in a tile
-template <int D> __device__ __forceinline__ uint32_t tile_at(int row, int chunk) {
-  if constexpr (D == 128)
-    return row * 128 + ((chunk ^ (row & 7)) << 4);
+// byte offset of 16-byte chunk `chunk` of key `row` in a tile
+template <int DP, int PITCH> __device__ __forceinline__ uint32_t tile_at(int row, int chunk) {
+  if constexpr (DP == 128 || DP == 256)
+    return row * PITCH + ((chunk ^ (row & 7)) << 4);
+  else if constexpr (DP == 64)
+    return row * PITCH + ((chunk ^ ((row >> 1) & 3)) << 4);
   else
-    return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
+    return row * PITCH + (chunk << 4);
+}
+// N 32-bit words from byte `byte` (a multiple of 4 N, of 4 or of 8) of key `row`
+template <int DP, int PITCH, int N>
+__device__ __forceinline__ void read_words(uint32_t (&w)[N], const unsigned char *tile, int row, int byte) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 u = *reinterpret_cast<const uint4 *>(tile + tile_at<DP, PITCH>(row, byte / 16 + i));
+      w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+    }
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const int at = byte + 8 * i;
+      const uint2 u = *reinterpret_cast<const uint2 *>(tile + tile_at<DP, PITCH>(row, at / 16) + at % 16);
+      w[2 * i] = u.x, w[2 * i + 1] = u.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = byte + 4 * i;
+      w[i] = *reinterpret_cast<const uint32_t *>(tile + tile_at<DP, PITCH>(row, at / 16) + at % 16);
+    }
+  }
 }
 __device__ __forceinline__ bool has_nan_e4m3(uint32_t w) {
   return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
 }
 
-// Page of a half tile (16 keys never leave a page) and its scales, one per lane.
+// Page of 16 keys (they never leave one) and its scales, one per lane.
 struct HalfPage {
   int page; // -1: none
   float ks, lv, iv; // K scale, log2 and reciprocal of the V scale
@@ -529,51 +566,63 @@ __device__ __forceinline__ HalfPage load_half(const PagedArgs &a, const Segment 
   return h;
 }
 
-template <int D> __global__ void __launch_bounds__(MMA_THREADS, MMA_CTAS_PER_SM) attention_paged_mma_kernel(PagedArgs a) {
-  using Cfg = MmaCfg<D>;
-  constexpr int S = Cfg::STAGES, KW = D / 16, NT = D / 8; // k-steps of q.k = 32-bit words a lane reads per key; n-tiles of p.v
+template <typename T, int DP, int NR>
+__global__ void __launch_bounds__(MmaCfg<DP, NR, sizeof(T) == 4>::THREADS, MmaCfg<DP, NR, sizeof(T) == 4>::CTAS_PER_SM)
+    attention_paged_mma_kernel(PagedArgs a) {
+  constexpr bool SPLIT = sizeof(T) == 4;
+  using Cfg = MmaCfg<DP, NR, SPLIT>;
+  constexpr int KW = Cfg::KW, VW = Cfg::VW, NT = Cfg::NT, MT = Cfg::MT, TILE = Cfg::TILE, R = Cfg::R;
+  constexpr int PITCH = Cfg::PITCH, NS = SPLIT ? 2 : 1;
   extern __shared__ __align__(128) unsigned char smem_raw[];
-  __shared__ long long warp_sum[MMA_WARPS];
-  __shared__ float2 ml_s[MMA_WARPS][MMA_ROWS];
+  __shared__ long long warp_sum[Cfg::WARPS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, grp = lane >> 2, quad = lane & 3;
   unsigned char *ring = smem_raw + warp * Cfg::WARP_BYTES;
-  long long *upto = reinterpret_cast<long long *>(smem_raw + MMA_WARPS * Cfg::WARP_BYTES);
+  long long *upto = reinterpret_cast<long long *>(smem_raw + Cfg::WARPS * Cfg::WARP_BYTES);
   const uint32_t ring_u32 = smem_u32(ring);
 
-  if (tid == 0)
-    a.items[blockIdx.x].used = 0;
-  const long long total = scan_units<MMA_THREADS, MMA_ROWS>(a, upto, warp_sum);
+  // neighbouring workers sit on different SMs, so that a short list spreads out
+  const int me = warp * gridDim.x + blockIdx.x;
+  if (lane == 0)
+    a.items[me].n_rows = 0;
+  __syncwarp();
+  const long long total = scan_units<Cfg::THREADS, R, Cfg::CHUNK>(a, upto, warp_sum);
   if (total == 0)
     return;
-  Walk walk(total, blockIdx.x, gridDim.x);
+  Walk<R, Cfg::CHUNK> walk(total, me, gridDim.x * Cfg::WARPS);
   Segment g;
   Seq s;
   const unsigned ps = a.page_size;
-  while (walk.next<MMA_ROWS>(a, upto, g, s)) {
-    // limits: least over the tile's rows, most over them, and this lane's two rows
+  const int D = a.D;
+  while (walk.next(a, upto, g, s, lane == 0)) {
+    // limits: least and most over the row tile, and this lane's rows (rb * 8 + 2 quad + e)
     const int least = row_limit(a, s, g.row0), most = row_limit(a, s, g.row0 + g.n_rows - 1);
-    const int lim0 = row_limit(a, s, g.row0 + grp), lim1 = row_limit(a, s, g.row0 + grp + 8);
-    const int first = g.chunk0 * CHUNK + warp * MMA_TILE, end = min(most, (g.chunk0 + g.chunks) * CHUNK);
-    const int tiles = end > first ? (end - first + CHUNK - 1) / CHUNK : 0; // this warp's, CHUNK apart
-    auto half_key = [&](int batch) { return first + (batch * 16 + (lane >> 1)) * CHUNK + (lane & 1) * 16; };
+    int lim[NR][2];
+#pragma unroll
+    for (int rb = 0; rb < NR; ++rb)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        lim[rb][e] = row_limit(a, s, g.row0 + rb * 8 + quad * 2 + e);
+    const int first = g.chunk0 * Cfg::CHUNK, end = min(most, (g.chunk0 + g.chunks) * Cfg::CHUNK);
+    const int tiles = end > first ? (end - first + TILE - 1) / TILE : 0;
+    constexpr int BATCH = 32 / MT; // tiles whose pages the lanes hold
+    auto half_key = [&](int batch) { return first + (batch * 32 + lane) * 16; };
     HalfPage cur = load_half(a, g, half_key(0), end), nxt = load_half(a, g, half_key(1), end);
 
     auto issue = [&](int i, const HalfPage &hp) {
       if (i < tiles) {
-        const uint32_t st = ring_u32 + (i % S) * 2 * Cfg::TILE_BYTES;
-        const int key0 = first + i * CHUNK;
+        const uint32_t st = ring_u32 + (i & 1) * 2 * Cfg::TILE_BYTES;
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const int page = __shfl_sync(~0u, hp.page, (i & 15) * 2 + hf);
-          const int key = key0 + 16 * hf, live = page >= 0 ? s.seen - key : 0; // rows behind it hold anything
+        for (int hf = 0; hf < MT; ++hf) {
+          const int page = __shfl_sync(~0u, hp.page, (i % BATCH) * MT + hf);
+          const int key = first + i * TILE + 16 * hf, live = page >= 0 ? s.seen - key : 0; // behind it: anything
           const unsigned in_page = static_cast<unsigned>(key) % ps;
-          const long long off = page >= 0 ? ((1ll * page * a.Hkv + g.head) * ps + in_page) * D + lane * 16 : 0;
+          const long long off = page >= 0 ? ((1ll * page * a.Hkv + g.head) * ps + in_page) * D : 0;
 #pragma unroll
-          for (int j = 0; j < D / 32; ++j) {
-            const int idx = lane + 32 * j, row = idx / (D / 16), chunk = idx % (D / 16);
-            const uint32_t at = tile_at<D>(hf * 16 + row, chunk);
-            const bool real = row < live;
-            const long long o = real ? off + 512 * j : 0;
+          for (int j = 0; j < DP / 32; ++j) {
+            const int idx = lane + 32 * j, row = idx / (DP / 16), chunk = idx % (DP / 16);
+            const uint32_t at = tile_at<DP, PITCH>(hf * 16 + row, chunk);
+            const bool real = row < live && chunk * 16 < D;
+            const long long o = real ? off + row * D + chunk * 16 : 0;
             cp_async16(st + at, a.kc + o, real);
             cp_async16(st + Cfg::TILE_BYTES + at, a.vc + o, real);
           }
@@ -581,153 +630,176 @@ template <int D> __global__ void __launch_bounds__(MMA_THREADS, MMA_CTAS_PER_SM)
       }
       cp_async_commit();
     };
-#pragma unroll
-    for (int i = 0; i < S - 1; ++i)
-      issue(i, cur);
+    issue(0, cur);
 
     // queries: fp16 fragments and each row's factor back
-    uint32_t qf[KW][4];
-    float fac[2];
+    uint32_t qf[NS][NR][KW][2];
+    float fac[NR][2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      float v[D / 4];
-      const bool live = grp + 8 * r < g.n_rows;
-      const long long row = g.row0 + grp + 8 * r;
-      const __nv_bfloat16 *qp = static_cast<const __nv_bfloat16 *>(a.q) +
-                                (live ? (s.q0 + row / a.G) * a.q_ld + (1ll * g.head * a.G + row % a.G) * D + quad * (D / 4) : 0);
-      if ((reinterpret_cast<uintptr_t>(qp) & 15u) == 0 && live) {
+    for (int rb = 0; rb < NR; ++rb) {
+      const int r = rb * 8 + grp, row = g.row0 + r;
+      const bool live = r < g.n_rows;
+      const T *qp = static_cast<const T *>(a.q) +
+                    (live ? (s.q0 + row / a.G) * a.q_ld + (1ll * g.head * a.G + row % a.G) * D : 0);
+      const bool vec = (reinterpret_cast<uintptr_t>(qp) & 7u) == 0;
+      float v[DP / 4];
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          const uint4 u = *(reinterpret_cast<const uint4 *>(qp) + i);
-          v[8 * i] = bf16_lo(u.x), v[8 * i + 1] = bf16_hi(u.x), v[8 * i + 2] = bf16_lo(u.y), v[8 * i + 3] = bf16_hi(u.y);
-          v[8 * i + 4] = bf16_lo(u.z), v[8 * i + 5] = bf16_hi(u.z), v[8 * i + 6] = bf16_lo(u.w), v[8 * i + 7] = bf16_hi(u.w);
+      for (int i = 0; i < DP / 16; ++i) {
+        const int d = quad * (DP / 4) + 4 * i;
+        if (live && d < D) {
+          if (vec && sizeof(T) == 2) {
+            const uint2 u = *reinterpret_cast<const uint2 *>(qp + d);
+            v[4 * i] = bf16_lo(u.x), v[4 * i + 1] = bf16_hi(u.x), v[4 * i + 2] = bf16_lo(u.y), v[4 * i + 3] = bf16_hi(u.y);
+          } else if (vec) {
+            const float2 x = *reinterpret_cast<const float2 *>(qp + d), y = *reinterpret_cast<const float2 *>(qp + d + 2);
+            v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = y.x, v[4 * i + 3] = y.y;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              v[4 * i + j] = load_in(qp + d + j);
+          }
+        } else {
+          v[4 * i] = v[4 * i + 1] = v[4 * i + 2] = v[4 * i + 3] = 0.f;
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < D / 4; ++i)
-          v[i] = live ? __bfloat162float(qp[i]) : 0.f;
       }
       uint32_t top = 0;
 #pragma unroll
-      for (int i = 0; i < D / 4; ++i)
+      for (int i = 0; i < DP / 4; ++i)
         top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
       top = max(top, __shfl_xor_sync(~0u, top, 1));
       top = max(top, __shfl_xor_sync(~0u, top, 2));
       const int e = min(max(static_cast<int>(top >> 23) - 127 - 14, -100), 113);
       const float f = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-      fac[r] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * a.scale_log2;
+      const float back = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+      fac[rb][0] = __shfl_sync(~0u, back, quad * 8) * a.scale_log2; // row 2 quad: lanes 8 quad ..
+      fac[rb][1] = __shfl_sync(~0u, back, quad * 8 + 4) * a.scale_log2;
 #pragma unroll
-      for (int i = 0; i < KW; ++i) {
-        qf[i][r] = f16x2(v[4 * i] * f, v[4 * i + 1] * f);
-        qf[i][r + 2] = f16x2(v[4 * i + 2] * f, v[4 * i + 3] * f);
-      }
+      for (int i = 0; i < KW; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float x = v[4 * i + 2 * h] * f, y = v[4 * i + 2 * h + 1] * f;
+          qf[0][rb][i][h] = f16x2(x, y);
+          if constexpr (SPLIT)
+            qf[NS - 1][rb][i][h] = f16x2_rest(x, y, qf[0][rb][i][h]);
+        }
     }
 
-    float o[NT][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    float o[NR][NT][4], m[NR][2], l[NR][2];
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
-      o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    for (int rb = 0; rb < NR; ++rb) {
+      m[rb][0] = m[rb][1] = -INFINITY, l[rb][0] = l[rb][1] = 0.f;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+        o[rb][j][0] = o[rb][j][1] = o[rb][j][2] = o[rb][j][3] = 0.f;
+    }
 
     for (int i = 0; i < tiles; ++i) {
-      if ((i & 15) == 0 && i > 0)
-        cur = nxt, nxt = load_half(a, g, half_key((i >> 4) + 1), end);
-      issue(i + S - 1, ((i + S - 1) >> 4) == (i >> 4) ? cur : nxt);
-      cp_async_wait<S - 1>();
+      if (i % BATCH == 0 && i > 0)
+        cur = nxt, nxt = load_half(a, g, half_key(i / BATCH + 1), end);
+      issue(i + 1, (i + 1) % BATCH != 0 ? cur : nxt);
+      cp_async_wait<1>();
       __syncwarp();
-      const unsigned char *kt = ring + (i % S) * 2 * Cfg::TILE_BYTES, *vt = kt + Cfg::TILE_BYTES;
-      const int key0 = first + i * CHUNK;
+      const unsigned char *kt = ring + (i & 1) * 2 * Cfg::TILE_BYTES, *vt = kt + Cfg::TILE_BYTES;
+      const int key0 = first + i * TILE;
+      const bool edge = key0 + TILE > least;
 
-      float sc[4][4];
+      // scores, in units of log2, with log2 of the V scale
+      float sc[NR][MT][4], iv[MT];
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt) {
-        sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
-        uint32_t w[KW];
+      for (int mt = 0; mt < MT; ++mt) {
+        uint32_t w0[KW], w1[KW];
+        read_words<DP, PITCH, KW>(w0, kt, mt * 16 + grp, quad * (DP / 4));
+        read_words<DP, PITCH, KW>(w1, kt, mt * 16 + grp + 8, quad * (DP / 4));
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          const uint4 u = *reinterpret_cast<const uint4 *>(kt + tile_at<D>(nt * 8 + grp, quad * (D / 64) + c));
-          w[4 * c] = u.x, w[4 * c + 1] = u.y, w[4 * c + 2] = u.z, w[4 * c + 3] = u.w;
+        for (int rb = 0; rb < NR; ++rb)
+          sc[rb][mt][0] = sc[rb][mt][1] = sc[rb][mt][2] = sc[rb][mt][3] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KW; ++k) {
+          const uint32_t ka[4] = {f16x2_of_e4m3_lo(w0[k]), f16x2_of_e4m3_lo(w1[k]), f16x2_of_e4m3_hi(w0[k]),
+                                  f16x2_of_e4m3_hi(w1[k])};
+#pragma unroll
+          for (int rb = 0; rb < NR; ++rb) {
+            if constexpr (SPLIT) {
+              float c[4] = {0.f, 0.f, 0.f, 0.f};
+              mma_f16(c, ka, qf[NS - 1][rb][k][0], qf[NS - 1][rb][k][1]);
+              mma_f16(c, ka, qf[0][rb][k][0], qf[0][rb][k][1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                sc[rb][mt][e] += c[e];
+            } else {
+              mma_f16(sc[rb][mt], ka, qf[0][rb][k][0], qf[0][rb][k][1]);
+            }
+          }
         }
-#pragma unroll
-        for (int k = 0; k < KW; ++k)
-          mma_f16(sc[nt], qf[k], f16x2_of_e4m3_lo(w[k]), f16x2_of_e4m3_hi(w[k]));
-      }
-      float iv[2];
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int src = (i & 15) * 2 + hf;
+        const int src = (i % BATCH) * MT + mt;
         const float ks = __shfl_sync(~0u, cur.ks, src), lv = __shfl_sync(~0u, cur.lv, src);
-        iv[hf] = __shfl_sync(~0u, cur.iv, src);
+        iv[mt] = __shfl_sync(~0u, cur.iv, src);
 #pragma unroll
-        for (int nt = 2 * hf; nt < 2 * hf + 2; ++nt) {
-          sc[nt][0] = fmaf(sc[nt][0], ks * fac[0], lv), sc[nt][1] = fmaf(sc[nt][1], ks * fac[0], lv);
-          sc[nt][2] = fmaf(sc[nt][2], ks * fac[1], lv), sc[nt][3] = fmaf(sc[nt][3], ks * fac[1], lv);
-        }
+        for (int rb = 0; rb < NR; ++rb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            sc[rb][mt][e] = fmaf(sc[rb][mt][e], ks * fac[rb][e & 1], lv);
+            if (edge && key0 + mt * 16 + grp + 8 * (e >> 1) >= lim[rb][e & 1])
+              sc[rb][mt][e] = -INFINITY;
+          }
       }
-      const bool edge = key0 + MMA_TILE > least;
-      if (edge) {
+
+      uint32_t pf[NS][NR][MT][2];
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt)
+      for (int rb = 0; rb < NR; ++rb) {
+        float t[2], ref[2];
+        bool grew = false;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          t[e] = m[rb][e];
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+            t[e] = fmaxf(t[e], fmaxf(sc[rb][mt][e], sc[rb][mt][e + 2]));
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1)
+            t[e] = fmaxf(t[e], __shfl_xor_sync(~0u, t[e], d));
+          ref[e] = t[e] == -INFINITY ? 0.f : t[e] - W_EXP;
+          grew |= t[e] != m[rb][e];
+        }
+        if (__any_sync(~0u, grew)) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const int key = key0 + nt * 8 + quad * 2 + e;
-            if (key >= lim0)
-              sc[nt][e] = -INFINITY;
-            if (key >= lim1)
-              sc[nt][2 + e] = -INFINITY;
+            const float f = m[rb][e] == -INFINITY ? 0.f : ex2_approx(m[rb][e] - t[e]);
+            l[rb][e] *= f, m[rb][e] = t[e];
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+              o[rb][j][e] *= f, o[rb][j][e + 2] *= f;
           }
-      }
-      float t0 = m0, t1 = m1;
-#pragma unroll
-      for (int nt = 0; nt < 4; ++nt)
-        t0 = fmaxf(t0, fmaxf(sc[nt][0], sc[nt][1])), t1 = fmaxf(t1, fmaxf(sc[nt][2], sc[nt][3]));
-      t0 = fmaxf(t0, __shfl_xor_sync(~0u, t0, 1)), t1 = fmaxf(t1, __shfl_xor_sync(~0u, t1, 1));
-      t0 = fmaxf(t0, __shfl_xor_sync(~0u, t0, 2)), t1 = fmaxf(t1, __shfl_xor_sync(~0u, t1, 2));
-      const float ref0 = t0 == -INFINITY ? 0.f : t0 - 12.f, ref1 = t1 == -INFINITY ? 0.f : t1 - 12.f;
-      if (__any_sync(~0u, t0 != m0 || t1 != m1)) {
-        const float f0 = m0 == -INFINITY ? 0.f : ex2_approx(m0 - t0), f1 = m1 == -INFINITY ? 0.f : ex2_approx(m1 - t1);
-        l0 *= f0, l1 *= f1;
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-          o[j][0] *= f0, o[j][1] *= f0, o[j][2] *= f1, o[j][3] *= f1;
-        m0 = t0, m1 = t1;
-      }
-      uint32_t pf[2][4];
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          float (&x)[4] = sc[2 * hf + n];
-          x[0] = ex2_approx(x[0] - ref0), x[1] = ex2_approx(x[1] - ref0);
-          x[2] = ex2_approx(x[2] - ref1), x[3] = ex2_approx(x[3] - ref1);
-          sum0 += x[0] + x[1], sum1 += x[2] + x[3];
-          pf[hf][2 * n] = f16x2(x[0], x[1]), pf[hf][2 * n + 1] = f16x2(x[2], x[3]);
         }
-        l0 = fmaf(sum0, iv[hf], l0), l1 = fmaf(sum1, iv[hf], l1);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          float (&x)[4] = sc[rb][mt];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            x[e] = ex2_approx(x[e] - ref[e & 1]);
+          l[rb][0] = fmaf(x[0] + x[2], iv[mt], l[rb][0]), l[rb][1] = fmaf(x[1] + x[3], iv[mt], l[rb][1]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t hi = f16x2(x[2 * h], x[2 * h + 1]);
+            pf[0][rb][mt][h] = transpose8x8(hi);
+            if constexpr (SPLIT)
+              pf[NS - 1][rb][mt][h] = transpose8x8(f16x2_rest(x[2 * h], x[2 * h + 1], hi));
+          }
+        }
       }
 
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        constexpr int VW = D / 32; // 32-bit words a lane reads per key
-        uint32_t w[4][VW];         // keys 2 quad, 2 quad + 1, and both + 8
+      for (int mt = 0; mt < MT; ++mt) {
+        uint32_t w[4][VW]; // keys 2 quad, 2 quad + 1, and both + 8
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = hf * 16 + 2 * quad + (r & 1) + 8 * (r >> 1);
-          if constexpr (D == 128) {
-            const uint4 u = *reinterpret_cast<const uint4 *>(vt + tile_at<D>(row, grp));
-            w[r][0] = u.x, w[r][1] = u.y, w[r][2] = u.z, w[r][3] = u.w;
-          } else {
-            const uint2 u = *reinterpret_cast<const uint2 *>(vt + tile_at<D>(row, grp >> 1) + (grp & 1) * 8);
-            w[r][0] = u.x, w[r][1] = u.y;
-          }
-        }
-        auto product = [&](float (&c)[4], const uint32_t (&p)[4], const uint32_t (&x)[4][VW], int j) {
-          const uint32_t sel = j & 2 ? 0x7362 : 0x5140; // bytes of two keys side by side, two dimensions
-          const uint32_t b0 = __byte_perm(x[0][j >> 2], x[1][j >> 2], sel), b1 = __byte_perm(x[2][j >> 2], x[3][j >> 2], sel);
-          if (j & 1)
-            mma_f16(c, p, f16x2_of_e4m3_hi(b0), f16x2_of_e4m3_hi(b1));
-          else
-            mma_f16(c, p, f16x2_of_e4m3_lo(b0), f16x2_of_e4m3_lo(b1));
+        for (int r = 0; r < 4; ++r)
+          read_words<DP, PITCH, VW>(w[r], vt, mt * 16 + 2 * quad + (r & 1) + 8 * (r >> 1), grp * (DP / 8));
+        // dimensions 2j and 2j + 1 of this lane's for two keys side by side
+        auto values = [&](const uint32_t (&x)[4][VW], int j, uint32_t (&va)[4]) {
+          const uint32_t sel = j & 1 ? 0x7362 : 0x5140;
+          const uint32_t b0 = __byte_perm(x[0][j >> 1], x[1][j >> 1], sel), b1 = __byte_perm(x[2][j >> 1], x[3][j >> 1], sel);
+          va[0] = f16x2_of_e4m3_lo(b0), va[1] = f16x2_of_e4m3_hi(b0);
+          va[2] = f16x2_of_e4m3_lo(b1), va[3] = f16x2_of_e4m3_hi(b1);
         };
         bool nan = false;
         if (edge) {
@@ -740,34 +812,52 @@ template <int D> __global__ void __launch_bounds__(MMA_THREADS, MMA_CTAS_PER_SM)
         }
         if (!nan) {
 #pragma unroll
-          for (int j = 0; j < NT; ++j)
-            product(o[j], pf[hf], w, j);
+          for (int j = 0; j < NT; ++j) {
+            uint32_t va[4];
+            values(w, j, va);
+#pragma unroll
+            for (int rb = 0; rb < NR; ++rb) {
+              if constexpr (SPLIT) {
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
+                mma_f16(c, va, pf[NS - 1][rb][mt][0], pf[NS - 1][rb][mt][1]);
+                mma_f16(c, va, pf[0][rb][mt][0], pf[0][rb][mt][1]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  o[rb][j][e] += c[e];
+              } else {
+                mma_f16(o[rb][j], va, pf[0][rb][mt][0], pf[0][rb][mt][1]);
+              }
+            }
+          }
         } else {
           // A NaN among keys that some rows may not see: zero weights would not keep it out, so the keys go
           // one at a time and a row takes only those it sees.
 #pragma unroll 1
           for (int t = 0; t < 16; ++t) {
-            const int key = key0 + hf * 16 + t;
-            uint32_t x[4][VW], p[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const bool mine = t == 2 * quad + (r & 1) + 8 * (r >> 1);
-#pragma unroll
-              for (int q = 0; q < VW; ++q)
-                x[r][q] = mine ? w[r][q] : 0u;
-            }
-            const uint32_t keep = (t & 7) >> 1 == quad ? (t & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
+            const int key = key0 + mt * 16 + t;
+            uint32_t x[4][VW];
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              p[r] = (r >> 1) == (t >> 3) ? pf[hf][r] & keep : 0u;
+#pragma unroll
+              for (int q = 0; q < VW; ++q)
+                x[r][q] = t == 2 * quad + (r & 1) + 8 * (r >> 1) ? w[r][q] : 0u;
+            const uint32_t keep = (t & 7) >> 1 == quad ? (t & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
+            const uint32_t k0 = t < 8 ? keep : 0u, k1 = t < 8 ? 0u : keep;
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-              float c[4] = {0.f, 0.f, 0.f, 0.f};
-              product(c, p, x, j);
-              if (key < lim0)
-                o[j][0] += c[0], o[j][1] += c[1];
-              if (key < lim1)
-                o[j][2] += c[2], o[j][3] += c[3];
+              uint32_t va[4];
+              values(x, j, va);
+#pragma unroll
+              for (int rb = 0; rb < NR; ++rb) {
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int n = NS - 1; n >= 0; --n)
+                  mma_f16(c, va, pf[n][rb][mt][0] & k0, pf[n][rb][mt][1] & k1);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (key < lim[rb][e & 1])
+                    o[rb][j][e] += c[e];
+              }
             }
           }
         }
@@ -775,114 +865,170 @@ template <int D> __global__ void __launch_bounds__(MMA_THREADS, MMA_CTAS_PER_SM)
       __syncwarp(); // the stage may be overwritten
     }
     cp_async_wait<0>();
-    __syncwarp();
 
-    // join the warps: every ring now carries its warp's rows
-    l0 += __shfl_xor_sync(~0u, l0, 1), l1 += __shfl_xor_sync(~0u, l1, 1);
-    l0 += __shfl_xor_sync(~0u, l0, 2), l1 += __shfl_xor_sync(~0u, l1, 2);
-    if (quad == 0)
-      ml_s[warp][grp] = make_float2(m0 - 12.f, l0), ml_s[warp][grp + 8] = make_float2(m1 - 12.f, l1);
-    float *mine = reinterpret_cast<float *>(ring);
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
-      if (grp + 8 * r < g.n_rows) {
-        float *p = mine + (grp + 8 * r) * D + quad * (D / 4);
+    for (int rb = 0; rb < NR; ++rb)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+      for (int e = 0; e < 2; ++e) {
+        float sum = l[rb][e];
 #pragma unroll
-          for (int j = 0; j < NT; j += 4)
-            *reinterpret_cast<float4 *>(p + e * NT + j) =
-                make_float4(o[j][2 * r + e], o[j + 1][2 * r + e], o[j + 2][2 * r + e], o[j + 3][2 * r + e]);
+        for (int d = 4; d < 32; d <<= 1)
+          sum += __shfl_xor_sync(~0u, sum, d);
+        const int r = rb * 8 + quad * 2 + e;
+        if (r >= g.n_rows)
+          continue;
+        if (g.slot < 0) {
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          const int row = g.row0 + r;
+          T *p = static_cast<T *>(a.out) + (s.q0 + row / a.G) * a.out_ld + (1ll * g.head * a.G + row % a.G) * D;
+          const bool vec = (reinterpret_cast<uintptr_t>(p) & (2 * sizeof(T) - 1)) == 0;
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const int d = grp * (DP / 8) + 2 * j;
+            // the reciprocal is off by half a unit; float32 takes the quotient
+            const float x = SPLIT ? (sum == 0.f ? 0.f : o[rb][j][e] / sum) : o[rb][j][e] * inv;
+            const float y = SPLIT ? (sum == 0.f ? 0.f : o[rb][j][e + 2] / sum) : o[rb][j][e + 2] * inv;
+            if (d >= D)
+              continue;
+            if (vec && sizeof(T) == 2) {
+              *reinterpret_cast<uint32_t *>(p + d) = pack_bf16x2(x, y);
+            } else if (vec) {
+              *reinterpret_cast<float2 *>(p + d) = make_float2(x, y);
+            } else {
+              store_out(p + d, x), store_out(p + d + 1, y);
+            }
+          }
+        } else {
+          const long long pr = 1ll * g.slot * R + r;
+          if (grp == 0)
+            a.part_ml[pr] = make_float2(m[rb][e] - W_EXP, sum);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const int d = grp * (DP / 8) + 2 * j;
+            if (d < D)
+              *reinterpret_cast<float2 *>(a.part_o + pr * D + d) = make_float2(o[rb][j][e], o[rb][j][e + 2]);
+          }
+        }
       }
-    __syncthreads();
-    for (int e = tid; e < g.n_rows * D; e += MMA_THREADS) {
-      const int r = e / D, d = e % D;
-      float M = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < MMA_WARPS; ++w)
-        M = fmaxf(M, ml_s[w][r].x);
-      float sum = 0.f, x = 0.f;
-#pragma unroll
-      for (int w = 0; w < MMA_WARPS; ++w) {
-        const float f = rel_weight(ml_s[w][r].x, M);
-        sum = fmaf(f, ml_s[w][r].y, sum);
-        x = fmaf(f, reinterpret_cast<const float *>(smem_raw + w * Cfg::WARP_BYTES)[e], x);
-      }
-      if (g.slot < 0) {
-        const long long row = g.row0 + r;
-        store_out(static_cast<__nv_bfloat16 *>(a.out) + (s.q0 + row / a.G) * a.out_ld +
-                      (1ll * g.head * a.G + row % a.G) * D + d,
-                  sum == 0.f ? 0.f : x / sum);
-      } else {
-        const long long pr = 1ll * g.slot * a.rows_per_tile + r;
-        a.part_o[pr * D + d] = x;
-        if (d == 0)
-          a.part_ml[pr] = make_float2(M, sum);
-      }
-    }
-    __syncthreads();
+    __syncwarp();
   }
 }
 
 // ---- joining the pieces ---------------------------------------------------------------------------
-// One CTA per (first CTA of a split item, row). Launched so that it may become resident while the main
-// kernel drains; griddepcontrol.wait is what orders its reads after that kernel's writes.
-constexpr int JOIN_THREADS = 128;
-template <typename T> __global__ void __launch_bounds__(JOIN_THREADS) attention_paged_join_kernel(PagedArgs a) {
+// A fixed grid; every CTA lists the split items (their flags fit a few loads) and takes every gridDim-th
+// (item, row). Its warps share the row's pieces. Launched so that it may become resident while the main
+// kernel drains; griddepcontrol.wait orders its reads after that kernel's writes.
+constexpr int JOIN_THREADS = 128, JOIN_WARPS = JOIN_THREADS / 32;
+template <typename T> __global__ void __launch_bounds__(JOIN_THREADS) attention_paged_join_kernel(PagedArgs a, int workers) {
+  extern __shared__ int list[]; // (item, first of its rows in the list of rows) pairs
+  __shared__ int warp_sum[2][JOIN_WARPS];
+  __shared__ float red_o[JOIN_WARPS][256];
+  __shared__ float2 red_ml[JOIN_WARPS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const SplitItem it = a.items[blockIdx.x];
-  const int r = blockIdx.y;
-  if (!it.used || r >= it.n_rows)
-    return;
-  __shared__ float red[JOIN_THREADS / 32];
-  const int tid = threadIdx.x, pieces = it.last_cta - static_cast<int>(blockIdx.x) + 1;
-  auto slot_row = [&](int i) {
-    return 1ll * (i == 0 ? it.first_slot : 2 * (static_cast<int>(blockIdx.x) + i)) * a.rows_per_tile + r;
-  };
-  float M = -INFINITY;
-  for (int i = tid; i < pieces; i += JOIN_THREADS)
-    M = fmaxf(M, a.part_ml[slot_row(i)].x);
+  int items = 0, rows = 0;
+  for (int w0 = 0; w0 < workers; w0 += JOIN_THREADS) {
+    const int n = w0 + tid < workers ? a.items[w0 + tid].n_rows : 0;
+    const unsigned used = __ballot_sync(~0u, n > 0);
+    int inc = n;
 #pragma unroll
-  for (int d = 16; d; d >>= 1)
-    M = fmaxf(M, __shfl_xor_sync(~0u, M, d));
-  if ((tid & 31) == 0)
-    red[tid >> 5] = M;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < JOIN_THREADS / 32; ++w)
-    M = fmaxf(M, red[w]);
-  const long long row = 1ll * it.row0 + r;
-  T *out = static_cast<T *>(a.out) + (it.q0 + row / a.G) * a.out_ld + (1ll * it.head * a.G + row % a.G) * a.D;
-  for (int d = tid; d < a.D; d += JOIN_THREADS) {
-    float sum = 0.f, o = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < pieces; ++i) {
-      const long long pr = slot_row(i);
-      const float2 ml = a.part_ml[pr];
-      const float f = rel_weight(ml.x, M);
-      sum += f * ml.y, o += f * a.part_o[pr * a.D + d];
+    for (int d = 1; d < 32; d <<= 1) {
+      const int t = __shfl_up_sync(~0u, inc, d);
+      if (lane >= d)
+        inc += t;
     }
-    store_out(out + d, sum == 0.f ? 0.f : o / sum);
+    __syncthreads();
+    if (lane == 31)
+      warp_sum[0][warp] = __popc(used), warp_sum[1][warp] = inc;
+    __syncthreads();
+    int at = items + __popc(used & ((1u << lane) - 1)), row = rows + inc - n;
+#pragma unroll
+    for (int w = 0; w < JOIN_WARPS; ++w) {
+      if (w < warp)
+        at += warp_sum[0][w], row += warp_sum[1][w];
+      items += warp_sum[0][w], rows += warp_sum[1][w];
+    }
+    if (n > 0)
+      list[2 * at] = w0 + tid, list[2 * at + 1] = row;
+  }
+  __syncthreads();
+  constexpr int V = 8; // dimensions a lane may hold
+  for (int k = blockIdx.x; k < rows; k += gridDim.x) {
+    int lo = 0, hi = items - 1; // the last item whose first row is <= k
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (list[2 * mid + 1] <= k)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    const int owner = list[2 * lo], r = k - list[2 * lo + 1];
+    const SplitItem it = a.items[owner];
+    const int pieces = it.last - owner + 1;
+    float M = -INFINITY, sum = 0.f, o[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      o[v] = 0.f;
+#pragma unroll 4
+    for (int i = warp; i < pieces; i += JOIN_WARPS) {
+      const long long pr = 1ll * (i == 0 ? it.first_slot : 2 * (owner + i)) * a.rows_per_tile + r;
+      const float2 ml = a.part_ml[pr];
+      float x[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        x[v] = lane + 32 * v < a.D ? a.part_o[pr * a.D + lane + 32 * v] : 0.f;
+      const float top = fmaxf(M, ml.x), f = rel_weight(M, top), h = rel_weight(ml.x, top);
+      sum = sum * f + ml.y * h, M = top;
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        o[v] = o[v] * f + x[v] * h;
+    }
+    if (lane == 0)
+      red_ml[warp] = make_float2(M, sum);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      red_o[warp][lane + 32 * v] = o[v];
+    __syncthreads();
+    M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < JOIN_WARPS; ++w)
+      M = fmaxf(M, red_ml[w].x);
+    const int row = it.row0 + r;
+    T *out = static_cast<T *>(a.out) + (it.q0 + row / a.G) * a.out_ld + (1ll * it.head * a.G + row % a.G) * a.D;
+    for (int d = tid; d < a.D; d += JOIN_THREADS) {
+      float all = 0.f, x = 0.f;
+#pragma unroll
+      for (int w = 0; w < JOIN_WARPS; ++w) {
+        const float f = rel_weight(red_ml[w].x, M);
+        all += f * red_ml[w].y, x += f * red_o[w][d];
+      }
+      store_out(out + d, all == 0.f ? 0.f : x / all);
+    }
+    __syncthreads();
   }
 }
 
 // ---- host -----------------------------------------------------------------------------------------
-constexpr int SIMT_CTAS_PER_SM = 4;
-constexpr int MAX_ROWS = 16, MAX_CTAS_PER_SM = 4;
+constexpr int SIMT_CTAS_PER_SM = 4, JOIN_CTAS_PER_SM = 4;
+constexpr int MAX_WORKERS_PER_SM = 12;
+
+// Rows of partial results over all workers: 12 workers of 8 rows, 8 of 16, or 4 CTAs of 8 per SM, two each.
+constexpr size_t MAX_PART_ROWS_PER_SM = 2 * 128;
 
 size_t paged_workspace_bytes(int num_sms, int D) {
-  const size_t ctas = static_cast<size_t>(num_sms) * MAX_CTAS_PER_SM;
-  return ctas * sizeof(SplitItem) + 64 + 2 * ctas * MAX_ROWS * (sizeof(float2) + sizeof(float) * D);
+  const size_t rows = static_cast<size_t>(num_sms) * MAX_PART_ROWS_PER_SM;
+  return rows * (sizeof(float) * D + sizeof(float2)) + sizeof(SplitItem) * num_sms * MAX_WORKERS_PER_SM;
 }
 
-template <typename T> int launch_join(const PagedArgs &a, int ctas, cudaStream_t st) {
+template <typename T> int launch_join(const PagedArgs &a, int workers, int num_sms, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas, a.rows_per_tile), cfg.blockDim = dim3(JOIN_THREADS), cfg.stream = st;
+  cfg.gridDim = dim3(num_sms * JOIN_CTAS_PER_SM), cfg.blockDim = dim3(JOIN_THREADS), cfg.stream = st;
+  cfg.dynamicSmemBytes = 2 * sizeof(int) * workers;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at, cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attention_paged_join_kernel<T>, a) == cudaSuccess ? 0 : 2;
+  return cudaLaunchKernelEx(&cfg, attention_paged_join_kernel<T>, a, workers) == cudaSuccess ? 0 : 2;
 }
 
 template <typename T, int RT, int VB, int NA> int launch_simt(PagedArgs a, int num_sms, cudaStream_t st) {
@@ -901,7 +1047,7 @@ template <typename T, int RT, int VB, int NA> int launch_simt(PagedArgs a, int n
   attention_paged_simt_kernel<T, RT, VB, NA><<<ctas, SIMT_THREADS, smem, st>>>(a);
   if (cudaGetLastError() != cudaSuccess)
     return 2;
-  return launch_join<T>(a, ctas, st);
+  return launch_join<T>(a, ctas, num_sms, st);
 }
 template <typename T, int VB, int NA> int launch_simt_rows(const PagedArgs &a, int num_sms, cudaStream_t st) {
   // rows that share a key: the group's heads for single tokens, up to 8 otherwise
@@ -912,48 +1058,60 @@ template <typename T, int VB, int NA> int launch_simt_rows(const PagedArgs &a, i
     return launch_simt<T, 4, VB, NA>(a, num_sms, st);
   return launch_simt<T, 8, VB, NA>(a, num_sms, st);
 }
-template <typename T> int launch_simt_dim(const PagedArgs &a, int num_sms, cudaStream_t st) {
-  if (a.D % 16 == 0)
-    return a.D <= 128 ? launch_simt_rows<T, 16, 1>(a, num_sms, st) : launch_simt_rows<T, 16, 2>(a, num_sms, st);
-  if (a.D % 4 == 0)
-    return a.D <= 128 ? launch_simt_rows<T, 4, 1>(a, num_sms, st) : launch_simt_rows<T, 4, 2>(a, num_sms, st);
-  return launch_simt_rows<T, 1, 8>(a, num_sms, st);
-}
 
-template <int D> int launch_mma(PagedArgs a, int num_sms, cudaStream_t st) {
-  const size_t smem = MMA_WARPS * MmaCfg<D>::WARP_BYTES + 8ull * a.B;
+template <typename T, int DP, int NR> int launch_mma(PagedArgs a, int num_sms, cudaStream_t st) {
+  using Cfg = MmaCfg<DP, NR, sizeof(T) == 4>;
+  constexpr size_t ring = Cfg::WARPS * Cfg::WARP_BYTES;
+  static_assert(ring + 8 * MU_ATTENTION_PAGED_MAX_REQUESTS <= 227 * 1024, "shared memory");
+  static_assert(Cfg::CTAS_PER_SM * Cfg::WARPS <= MAX_WORKERS_PER_SM, "workspace");
+  static_assert(2 * Cfg::CTAS_PER_SM * Cfg::WARPS * Cfg::R <= MAX_PART_ROWS_PER_SM, "workspace");
   static PerDeviceOnce once;
   if (once.get() < 0) {
-    if (cudaFuncSetAttribute(attention_paged_mma_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             MMA_WARPS * MmaCfg<D>::WARP_BYTES + 8 * MU_ATTENTION_PAGED_MAX_REQUESTS) != cudaSuccess)
+    if (cudaFuncSetAttribute(attention_paged_mma_kernel<T, DP, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             ring + 8 * MU_ATTENTION_PAGED_MAX_REQUESTS) != cudaSuccess)
       return 2;
     once.set(1);
   }
-  const int ctas = num_sms * MMA_CTAS_PER_SM;
-  a.rows_per_tile = MMA_ROWS;
-  attention_paged_mma_kernel<D><<<ctas, MMA_THREADS, smem, st>>>(a);
+  const int ctas = num_sms * Cfg::CTAS_PER_SM;
+  a.rows_per_tile = Cfg::R;
+  attention_paged_mma_kernel<T, DP, NR><<<ctas, Cfg::THREADS, ring + 8ull * a.B, st>>>(a);
   if (cudaGetLastError() != cudaSuccess)
     return 2;
-  return launch_join<__nv_bfloat16>(a, ctas, st);
+  return launch_join<T>(a, ctas * Cfg::WARPS, num_sms, st);
+}
+
+template <typename T> int launch_by_dim(const PagedArgs &a, int num_sms, cudaStream_t st) {
+  if (a.D % 16 != 0) {
+    if (a.D % 4 != 0)
+      return launch_simt_rows<T, 1, 8>(a, num_sms, st);
+    return a.D <= 128 ? launch_simt_rows<T, 4, 1>(a, num_sms, st) : launch_simt_rows<T, 4, 2>(a, num_sms, st);
+  }
+  // 8 rows share every key read for single tokens (the group's heads), 16 where there are more
+  const bool more = a.n_tokens > a.B || a.G > 8;
+  if (a.D > 128)
+    return launch_mma<T, 256, 1>(a, num_sms, st);
+  if (a.D > 96)
+    return more ? launch_mma<T, 128, 2>(a, num_sms, st) : launch_mma<T, 128, 1>(a, num_sms, st);
+  if (a.D > 64)
+    return more ? launch_mma<T, 96, 2>(a, num_sms, st) : launch_mma<T, 96, 1>(a, num_sms, st);
+  if (a.D > 32)
+    return more ? launch_mma<T, 64, 2>(a, num_sms, st) : launch_mma<T, 64, 1>(a, num_sms, st);
+  return more ? launch_mma<T, 32, 2>(a, num_sms, st) : launch_mma<T, 32, 1>(a, num_sms, st);
 }
 
 // 0 ok, 1 dtype not implemented, 2 CUDA error
 int launch_attention_paged(PagedArgs a, void *workspace, int dtype, int num_sms, cudaStream_t st) {
-  const size_t ctas = static_cast<size_t>(num_sms) * MAX_CTAS_PER_SM;
+  const size_t rows = static_cast<size_t>(num_sms) * MAX_PART_ROWS_PER_SM;
   unsigned char *w = static_cast<unsigned char *>(workspace);
   a.part_o = reinterpret_cast<float *>(w);
-  w += sizeof(float) * 2 * ctas * MAX_ROWS * a.D;
+  w += sizeof(float) * rows * a.D;
   a.part_ml = reinterpret_cast<float2 *>(w);
-  w += sizeof(float2) * 2 * ctas * MAX_ROWS;
+  w += sizeof(float2) * rows;
   a.items = reinterpret_cast<SplitItem *>(w);
   if (dtype == F32)
-    return launch_simt_dim<float>(a, num_sms, st);
-  if (dtype == BF16 && a.D == 128)
-    return launch_mma<128>(a, num_sms, st);
-  if (dtype == BF16 && a.D == 64)
-    return launch_mma<64>(a, num_sms, st);
+    return launch_by_dim<float>(a, num_sms, st);
   if (dtype == BF16)
-    return launch_simt_dim<__nv_bfloat16>(a, num_sms, st);
+    return launch_by_dim<__nv_bfloat16>(a, num_sms, st);
   return 1;
 }
 
