@@ -11,7 +11,8 @@
 // are. A worker walks its range as segments, one per (request, head, row tile). A segment that covers
 // all chunks writes its rows; one that does not leaves (running maximum, sum, weighted values) in the
 // workspace, and a second small kernel joins the pieces. No atomics: results do not depend on the order
-// in which workers run.
+// in which workers run. Every item counts one unit more than its chunks, for what starting a segment
+// costs: without it the workers that got many short requests finished last.
 #include "../../include/munet_b200.h"
 #include "common.h"
 #include "ptx.cuh"
@@ -34,7 +35,9 @@ struct PagedArgs {
   const int *query_start, *seq_lens;
   int B, n_tokens, Hq, Hkv, G, D, num_pages, page_size, causal;
   float scale_log2; // log2(e) / sqrt(D)
-  struct SplitItem *items;
+  struct SplitItem *items; // by the worker that holds the first chunk
+  int2 *notes;             // per worker: rows of the split item it begins (0: none), worker that began the
+                           // item its first segment continues (-1: none)
   float2 *part_ml;
   float *part_o;
   int rows_per_tile; // stride of the partial results
@@ -43,10 +46,11 @@ struct PagedArgs {
 
 // A (request, head, row tile) whose chunks went to more than one worker; entry w belongs to the worker
 // that holds its first chunk. Its later pieces are the first segments of workers w+1 .. last.
-// n_rows 0: no such item.
 struct SplitItem {
-  int n_rows, first_slot, last, row0, q0, head;
+  int first_slot, last, row0, n_rows, q0, head;
 };
+
+constexpr int START_UNITS = 1; // what beginning an item counts for
 
 struct Seq {
   int q0, nq, len;  // first row of q, new tokens, tokens in the cache (as given)
@@ -77,7 +81,7 @@ template <int R, int CHUNK> __device__ __forceinline__ long long units_of(const 
   if (s.nq <= 0)
     return 0;
   const unsigned rows = static_cast<unsigned>(s.nq) * a.G; // n_tokens * Hq fits 31 bits
-  return 1ll * a.Hkv * ((rows + R - 1) / R) * chunks_of<CHUNK>(s);
+  return 1ll * a.Hkv * ((rows + R - 1) / R) * (chunks_of<CHUNK>(s) + START_UNITS);
 }
 // Keys row `row` of a request may see.
 __device__ __forceinline__ int row_limit(const PagedArgs &a, const Seq &s, int row) {
@@ -167,38 +171,45 @@ template <int R, int CHUNK> struct Walk {
   }
   // The next segment. `leader`: the thread that notes down a split item.
   __device__ __forceinline__ bool next(const PagedArgs &a, const long long *upto, Segment &g, Seq &s, bool leader) {
-    if (u >= end)
-      return false;
-    int lo = b, hi = a.B - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (upto[mid] > u)
-        hi = mid;
-      else
-        lo = mid + 1;
-    }
-    b = lo;
-    s = load_seq(a, b);
-    const long long base = b ? upto[b - 1] : 0;
-    const int rows = s.nq * a.G, tiles = (rows + R - 1) / R, nc = chunks_of<CHUNK>(s);
+    int rows, tiles, nc, at, to;
+    do { // more than once only where this worker's share ends inside an item's starting units
+      if (u >= end)
+        return false;
+      int lo = b, hi = a.B - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (upto[mid] > u)
+          hi = mid;
+        else
+          lo = mid + 1;
+      }
+      b = lo;
+      s = load_seq(a, b);
+      rows = s.nq * a.G, tiles = (rows + R - 1) / R, nc = chunks_of<CHUNK>(s);
+      const long long item = div_rem(u - (b ? upto[b - 1] : 0), nc + START_UNITS, at);
+      int tile;
+      g.head = static_cast<int>(div_rem(item, tiles, tile));
+      g.row0 = tile * R;
+      to = static_cast<int>(min(static_cast<long long>(nc + START_UNITS), at + (end - u)));
+      u += to - at;
+    } while (to <= START_UNITS);
     g.b = b;
-    const long long item = div_rem(u - base, nc, g.chunk0);
-    int tile;
-    g.head = static_cast<int>(div_rem(item, tiles, tile));
-    g.row0 = tile * R;
     g.n_rows = min(rows - g.row0, R);
-    g.chunks = static_cast<int>(min(static_cast<long long>(nc - g.chunk0), end - u));
+    g.chunk0 = max(at - START_UNITS, 0);
+    g.chunks = to - START_UNITS - g.chunk0;
     g.slot = -1;
     if (g.chunks < nc) {
       g.slot = 2 * me + (first ? 0 : 1);
-      if (g.chunk0 == 0 && leader) {
+      const long long item0 = u - to; // of the item's units
+      if (leader && g.chunk0 == 0) {
         SplitItem it;
-        it.first_slot = g.slot, it.last = owner(u + nc - 1);
+        it.first_slot = g.slot, it.last = owner(item0 + nc + START_UNITS - 1);
         it.row0 = g.row0, it.n_rows = g.n_rows, it.q0 = s.q0, it.head = g.head;
-        a.items[me] = it;
+        a.items[me] = it, a.notes[me].x = g.n_rows;
+      } else if (leader) {
+        a.notes[me].y = owner(item0 + START_UNITS);
       }
     }
-    u += g.chunks;
     first = false;
     return true;
   }
@@ -239,7 +250,7 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_paged_simt_kernel(Page
   float *o_s = q_s + RT * Dq;                                        // [warps][groups][RT][D]
 
   if (tid == 0)
-    a.items[blockIdx.x].n_rows = 0;
+    a.notes[blockIdx.x] = make_int2(0, -1);
   const long long total = scan_units<SIMT_THREADS, RT, SIMT_CHUNK>(a, upto, warp_sum);
   if (total == 0)
     return;
@@ -439,10 +450,13 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_paged_simt_kernel(Page
 }
 
 // ---- tensor-core kernel: head sizes that are multiples of 16 ----------------------------------------
-// Bound by reading the cache. A warp is a worker: it walks its keys in tiles (32 of them, 16 for head
-// sizes above 128), copies a tile's K and V bytes into its own two stages of shared memory (cp.async, 16
-// bytes a lane), turns them into fp16 in registers and multiplies with mma.m16n8k16. Nothing ever
-// synchronises the CTA.
+// Bound by reading the cache. A warp walks its keys in tiles (32 of them, 16 for head sizes above 128),
+// copies a tile's K and V bytes into its own two stages of shared memory (cp.async, 16 bytes a lane),
+// turns them into fp16 in registers and multiplies with mma.m16n8k16. Where requests x KV heads are many,
+// a warp is a worker of its own and nothing ever synchronises the CTA (TEAM 1). Where they are few, every
+// item is cut into many pieces whose join would cost as much as the rest (3 requests x 2 heads: 296 pieces
+// each); there the four warps of a CTA are one worker, take every fourth tile and join in shared memory
+// (TEAM 4).
 //
 // The keys are the M side of both products, so that eight rows fill the N side: S' = K q' is 16 keys x 8
 // rows, O' = V' P' is 16 dimensions x 8 rows (with the rows as M, half to 15/16 of every product would be
@@ -459,14 +473,15 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_paged_simt_kernel(Page
 // from zero and is added in fp32, because the tensor core rounds its running sum towards zero.
 constexpr float W_EXP = 15.f; // the largest weight of a row is 2^15: fp16 ends at 65504
 
-template <int DP, int NR, bool SPLIT> struct MmaCfg {
+template <int DP, int NR, int TEAM, bool SPLIT> struct MmaCfg {
   static constexpr int WARPS = 4, THREADS = 32 * WARPS;
   static constexpr int CTAS_PER_SM = (DP <= 128 && NR == 1) ? 3 : 2; // 12 or 8 warps: by their registers
   static constexpr int R = 8 * NR;
-  static constexpr int TILE = DP <= 128 ? 32 : 16, CHUNK = 64, MT = TILE / 16;
+  static constexpr int TILE = DP <= 128 ? 32 : 16, CHUNK = TEAM * TILE, MT = TILE / 16;
   // bytes between keys: whole bank cycles are swizzled, others padded
   static constexpr int PITCH = DP == 64 || DP == 128 || DP == 256 ? DP : DP + 16;
   static constexpr int TILE_BYTES = TILE * PITCH, WARP_BYTES = 4 * TILE_BYTES; // K and V, two stages
+  static_assert(TEAM == 1 || (TEAM == WARPS && WARP_BYTES >= R * DP * 4), "a warp's ring carries its rows to the join");
   static constexpr int KW = DP / 16, VW = DP / 32, NT = DP / 16; // 32-bit words of K / V a lane reads per key; d-tiles
 };
 
@@ -501,6 +516,9 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return d;
 }
 // 16 bytes into shared memory, or 16 zero bytes
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool real) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
@@ -545,162 +563,229 @@ __device__ __forceinline__ bool has_nan_e4m3(uint32_t w) {
   return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
 }
 
-// Page of 16 keys (they never leave one) and its scales, one per lane.
-struct HalfPage {
-  int page; // -1: none
-  float ks, lv, iv; // K scale, log2 and reciprocal of the V scale
-};
-__device__ __forceinline__ HalfPage load_half(const PagedArgs &a, const Segment &g, int key, int end) {
-  HalfPage h;
-  h.page = -1, h.ks = 0.f, h.lv = -INFINITY, h.iv = 0.f;
-  if (key < end) {
-    const int page = a.table[1ll * g.b * a.table_stride + static_cast<unsigned>(key) / static_cast<unsigned>(a.page_size)];
-    if (page >= 0 && page < a.num_pages) {
-      const long long t = 1ll * page * a.Hkv + g.head;
-      const float vs = fmaxf(a.vs[t], 0x1p-64f);
-      h.page = page, h.ks = a.ks[t], h.lv = log2f(vs), h.iv = 1.f / vs;
-    } else {
-      atomicCAS(a.status, 0, MU_DEV_BAD_PAGE);
-    }
-  }
-  return h;
-}
-
-template <typename T, int DP, int NR>
-__global__ void __launch_bounds__(MmaCfg<DP, NR, sizeof(T) == 4>::THREADS, MmaCfg<DP, NR, sizeof(T) == 4>::CTAS_PER_SM)
+template <typename T, int DP, int NR, int TEAM>
+__global__ void __launch_bounds__(MmaCfg<DP, NR, TEAM, sizeof(T) == 4>::THREADS,
+                                  MmaCfg<DP, NR, TEAM, sizeof(T) == 4>::CTAS_PER_SM)
     attention_paged_mma_kernel(PagedArgs a) {
   constexpr bool SPLIT = sizeof(T) == 4;
-  using Cfg = MmaCfg<DP, NR, SPLIT>;
+  using Cfg = MmaCfg<DP, NR, TEAM, SPLIT>;
   constexpr int KW = Cfg::KW, VW = Cfg::VW, NT = Cfg::NT, MT = Cfg::MT, TILE = Cfg::TILE, R = Cfg::R;
   constexpr int PITCH = Cfg::PITCH, NS = SPLIT ? 2 : 1;
-  extern __shared__ __align__(128) unsigned char smem_raw[];
+  extern __shared__ __align__(16) unsigned char smem_raw[];
   __shared__ long long warp_sum[Cfg::WARPS];
+  __shared__ float2 team_ml[TEAM][R];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, grp = lane >> 2, quad = lane & 3;
   unsigned char *ring = smem_raw + warp * Cfg::WARP_BYTES;
   long long *upto = reinterpret_cast<long long *>(smem_raw + Cfg::WARPS * Cfg::WARP_BYTES);
   const uint32_t ring_u32 = smem_u32(ring);
 
   // neighbouring workers sit on different SMs, so that a short list spreads out
-  const int me = warp * gridDim.x + blockIdx.x;
-  if (lane == 0)
-    a.items[me].n_rows = 0;
+  const int me = TEAM == 1 ? warp * gridDim.x + blockIdx.x : blockIdx.x;
+  const bool leader = TEAM == 1 ? lane == 0 : tid == 0;
+  if (leader)
+    a.notes[me] = make_int2(0, -1);
   __syncwarp();
   const long long total = scan_units<Cfg::THREADS, R, Cfg::CHUNK>(a, upto, warp_sum);
   if (total == 0)
     return;
-  Walk<R, Cfg::CHUNK> walk(total, me, gridDim.x * Cfg::WARPS);
-  Segment g;
-  Seq s;
+  Walk<R, Cfg::CHUNK> walk(total, me, gridDim.x * (Cfg::WARPS / TEAM));
   const unsigned ps = a.page_size;
   const int D = a.D;
-  while (walk.next(a, upto, g, s, lane == 0)) {
-    // limits: least and most over the row tile, and this lane's rows (rb * 8 + 2 quad + e)
-    const int least = row_limit(a, s, g.row0), most = row_limit(a, s, g.row0 + g.n_rows - 1);
-    int lim[NR][2];
+  // The walk as a stream of batches: up to 32 half tiles of one segment, whose pages and scales the lanes
+  // hold. The batch after the current one is looked up while that runs, in steps that do not wait for one
+  // another's loads (table, then scales), and its first tile is on its way before the current one is done:
+  // a segment begun cold cost 5.6 us of dependent loads.
+  constexpr int BATCH = 32 / MT, STEP = TEAM * TILE; // tiles of a batch; keys between a warp's tiles
+  struct Batch {
+    int head, row0, n_rows, slot, q0, nq, len, seen;
+    int key0, tiles;
+    int page;     // of half tile `lane`; -1: none
+    float ks, vs; // its scales; vs 0: no page
+    bool first, last;
+  };
+  Segment g;
+  Seq s;
+  int seg_key = 0, seg_end = 0; // this warp's keys of segment (g, s) that have not been handed out
+  bool open = false;            // some batch of it is still to come
+  auto half_key = [&](const Batch &n) { return n.key0 + (lane / MT) * STEP + (lane % MT) * 16; };
+  auto fetch = [&](Batch &n) -> bool {
+    n.first = !open;
+    if (!open) {
+      if (!walk.next(a, upto, g, s, leader))
+        return false;
+      seg_key = g.chunk0 * Cfg::CHUNK + (TEAM == 1 ? 0 : warp * TILE);
+      seg_end = min(row_limit(a, s, g.row0 + g.n_rows - 1), (g.chunk0 + g.chunks) * Cfg::CHUNK);
+      const int r = g.row0 + grp; // its queries: into L1
+      if (grp < g.n_rows)
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const T *>(a.q) + (s.q0 + r / a.G) * a.q_ld +
+                                                    (1ll * g.head * a.G + r % a.G) * D + quad * D / 4));
+    }
+    n.head = g.head, n.row0 = g.row0, n.n_rows = g.n_rows, n.slot = g.slot;
+    n.q0 = s.q0, n.nq = s.nq, n.len = s.len, n.seen = s.seen;
+    n.key0 = seg_key;
+    n.tiles = seg_end > seg_key ? min(BATCH, (seg_end - seg_key + STEP - 1) / STEP) : 0;
+    const int key = half_key(n);
+    n.page = -2; // not looked for
+    if (lane / MT < n.tiles && key < seg_end)
+      n.page = a.table[1ll * g.b * a.table_stride + static_cast<unsigned>(key) / ps];
+    seg_key += BATCH * STEP;
+    open = seg_key < seg_end;
+    n.last = !open;
+    return true;
+  };
+  auto scales = [&](Batch &n) { // the pages have arrived
+    n.ks = n.vs = 0.f;
+    if (n.page >= 0 && n.page < a.num_pages) {
+      const long long t = 1ll * n.page * a.Hkv + n.head;
+      n.ks = a.ks[t], n.vs = a.vs[t];
+    } else {
+      if (n.page != -2)
+        atomicCAS(a.status, 0, MU_DEV_BAD_PAGE);
+      n.page = -1;
+    }
+  };
+  auto issue = [&](const Batch &n, int i, int stage) {
+    if (i < n.tiles) {
+      const uint32_t st = ring_u32 + stage * 2 * Cfg::TILE_BYTES;
 #pragma unroll
-    for (int rb = 0; rb < NR; ++rb)
+      for (int hf = 0; hf < MT; ++hf) {
+        const int page = __shfl_sync(~0u, n.page, i * MT + hf);
+        const int key = n.key0 + i * STEP + 16 * hf, live = page >= 0 ? n.seen - key : 0; // behind it: anything
+        const unsigned in_page = static_cast<unsigned>(key) % ps;
+        const long long off = page >= 0 ? ((1ll * page * a.Hkv + n.head) * ps + in_page) * D : 0;
+        if (D == DP && live >= 16) { // sixteen whole rows: one run of bytes
+          const uint8_t *kp = a.kc + off + lane * 16, *vp = a.vc + off + lane * 16;
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        lim[rb][e] = row_limit(a, s, g.row0 + rb * 8 + quad * 2 + e);
-    const int first = g.chunk0 * Cfg::CHUNK, end = min(most, (g.chunk0 + g.chunks) * Cfg::CHUNK);
-    const int tiles = end > first ? (end - first + TILE - 1) / TILE : 0;
-    constexpr int BATCH = 32 / MT; // tiles whose pages the lanes hold
-    auto half_key = [&](int batch) { return first + (batch * 32 + lane) * 16; };
-    HalfPage cur = load_half(a, g, half_key(0), end), nxt = load_half(a, g, half_key(1), end);
-
-    auto issue = [&](int i, const HalfPage &hp) {
-      if (i < tiles) {
-        const uint32_t st = ring_u32 + (i & 1) * 2 * Cfg::TILE_BYTES;
-#pragma unroll
-        for (int hf = 0; hf < MT; ++hf) {
-          const int page = __shfl_sync(~0u, hp.page, (i % BATCH) * MT + hf);
-          const int key = first + i * TILE + 16 * hf, live = page >= 0 ? s.seen - key : 0; // behind it: anything
-          const unsigned in_page = static_cast<unsigned>(key) % ps;
-          const long long off = page >= 0 ? ((1ll * page * a.Hkv + g.head) * ps + in_page) * D : 0;
+          for (int j = 0; j < DP / 32; ++j) {
+            const int idx = lane + 32 * j;
+            const uint32_t at = st + tile_at<DP, PITCH>(hf * 16 + idx / (DP / 16), idx % (DP / 16));
+            cp_async16(at, kp + 512 * j);
+            cp_async16(at + Cfg::TILE_BYTES, vp + 512 * j);
+          }
+        } else {
 #pragma unroll
           for (int j = 0; j < DP / 32; ++j) {
             const int idx = lane + 32 * j, row = idx / (DP / 16), chunk = idx % (DP / 16);
-            const uint32_t at = tile_at<DP, PITCH>(hf * 16 + row, chunk);
+            const uint32_t at = st + tile_at<DP, PITCH>(hf * 16 + row, chunk);
             const bool real = row < live && chunk * 16 < D;
             const long long o = real ? off + row * D + chunk * 16 : 0;
-            cp_async16(st + at, a.kc + o, real);
-            cp_async16(st + Cfg::TILE_BYTES + at, a.vc + o, real);
+            cp_async16(at, a.kc + o, real);
+            cp_async16(at + Cfg::TILE_BYTES, a.vc + o, real);
           }
         }
       }
-      cp_async_commit();
-    };
-    issue(0, cur);
+    }
+    cp_async_commit();
+  };
 
-    // queries: fp16 fragments and each row's factor back
-    uint32_t qf[NS][NR][KW][2];
-    float fac[NR][2];
+  uint32_t qf[NS][NR][KW][2]; // queries: fp16 fragments, and each row's factor back
+  float fac[NR][2];
+  float o[NR][NT][4], m[NR][2], l[NR][2];
+  int lim[NR][2], least = 0; // keys that this lane's rows (rb * 8 + 2 quad + e) see, and the least over all rows
+  int stage = 0;
+  Batch cur, nxt;
+  bool more = fetch(cur);
+  if (more) {
+    scales(cur);
+    issue(cur, 0, stage);
+  }
+  bool ahead = true; // the first tile of `cur` is on its way, its scales are too
+  while (more) {
+    const bool more_after = fetch(nxt);
+    if (!more_after)
+      nxt.tiles = 0, nxt.page = -2;
+    if (!ahead) {
+      scales(cur);
+      issue(cur, 0, stage);
+    }
+    if (cur.first) {
+      const Seq cs{cur.q0, cur.nq, cur.len, cur.seen};
+      least = row_limit(a, cs, cur.row0);
 #pragma unroll
-    for (int rb = 0; rb < NR; ++rb) {
-      const int r = rb * 8 + grp, row = g.row0 + r;
-      const bool live = r < g.n_rows;
-      const T *qp = static_cast<const T *>(a.q) +
-                    (live ? (s.q0 + row / a.G) * a.q_ld + (1ll * g.head * a.G + row % a.G) * D : 0);
-      const bool vec = (reinterpret_cast<uintptr_t>(qp) & 7u) == 0;
-      float v[DP / 4];
+      for (int rb = 0; rb < NR; ++rb) {
+        m[rb][0] = m[rb][1] = -INFINITY, l[rb][0] = l[rb][1] = 0.f;
 #pragma unroll
-      for (int i = 0; i < DP / 16; ++i) {
-        const int d = quad * (DP / 4) + 4 * i;
-        if (live && d < D) {
-          if (vec && sizeof(T) == 2) {
-            const uint2 u = *reinterpret_cast<const uint2 *>(qp + d);
-            v[4 * i] = bf16_lo(u.x), v[4 * i + 1] = bf16_hi(u.x), v[4 * i + 2] = bf16_lo(u.y), v[4 * i + 3] = bf16_hi(u.y);
-          } else if (vec) {
-            const float2 x = *reinterpret_cast<const float2 *>(qp + d), y = *reinterpret_cast<const float2 *>(qp + d + 2);
-            v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = y.x, v[4 * i + 3] = y.y;
+        for (int e = 0; e < 2; ++e)
+          lim[rb][e] = row_limit(a, cs, cur.row0 + rb * 8 + quad * 2 + e);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          o[rb][j][0] = o[rb][j][1] = o[rb][j][2] = o[rb][j][3] = 0.f;
+      }
+      float qv[NR][DP / 4];
+#pragma unroll
+      for (int rb = 0; rb < NR; ++rb) {
+        const int r = rb * 8 + grp, row = cur.row0 + r;
+        const bool live = r < cur.n_rows;
+        const T *qp = static_cast<const T *>(a.q) +
+                      (live ? (cur.q0 + row / a.G) * a.q_ld + (1ll * cur.head * a.G + row % a.G) * D : 0);
+        const bool vec = (reinterpret_cast<uintptr_t>(qp) & 7u) == 0;
+        float (&v)[DP / 4] = qv[rb];
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+          const int d = quad * (DP / 4) + 4 * i;
+          if (live && d < D) {
+            if (vec && sizeof(T) == 2) {
+              const uint2 u = *reinterpret_cast<const uint2 *>(qp + d);
+              v[4 * i] = bf16_lo(u.x), v[4 * i + 1] = bf16_hi(u.x), v[4 * i + 2] = bf16_lo(u.y), v[4 * i + 3] = bf16_hi(u.y);
+            } else if (vec) {
+              const float2 x = *reinterpret_cast<const float2 *>(qp + d), y = *reinterpret_cast<const float2 *>(qp + d + 2);
+              v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = y.x, v[4 * i + 3] = y.y;
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                v[4 * i + j] = load_in(qp + d + j);
+            }
           } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              v[4 * i + j] = load_in(qp + d + j);
+            v[4 * i] = v[4 * i + 1] = v[4 * i + 2] = v[4 * i + 3] = 0.f;
           }
-        } else {
-          v[4 * i] = v[4 * i + 1] = v[4 * i + 2] = v[4 * i + 3] = 0.f;
         }
       }
-      uint32_t top = 0;
+
 #pragma unroll
-      for (int i = 0; i < DP / 4; ++i)
-        top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-      top = max(top, __shfl_xor_sync(~0u, top, 1));
-      top = max(top, __shfl_xor_sync(~0u, top, 2));
-      const int e = min(max(static_cast<int>(top >> 23) - 127 - 14, -100), 113);
-      const float f = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-      const float back = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-      fac[rb][0] = __shfl_sync(~0u, back, quad * 8) * a.scale_log2; // row 2 quad: lanes 8 quad ..
-      fac[rb][1] = __shfl_sync(~0u, back, quad * 8 + 4) * a.scale_log2;
+      for (int rb = 0; rb < NR; ++rb) {
+        const float (&v)[DP / 4] = qv[rb];
+        uint32_t top = 0;
 #pragma unroll
-      for (int i = 0; i < KW; ++i)
+        for (int i = 0; i < DP / 4; ++i)
+          top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+        top = max(top, __shfl_xor_sync(~0u, top, 1));
+        top = max(top, __shfl_xor_sync(~0u, top, 2));
+        const int e = min(max(static_cast<int>(top >> 23) - 127 - 14, -100), 113);
+        const float f = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        const float back = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        fac[rb][0] = __shfl_sync(~0u, back, quad * 8) * a.scale_log2; // row 2 quad: lanes 8 quad ..
+        fac[rb][1] = __shfl_sync(~0u, back, quad * 8 + 4) * a.scale_log2;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float x = v[4 * i + 2 * h] * f, y = v[4 * i + 2 * h + 1] * f;
-          qf[0][rb][i][h] = f16x2(x, y);
-          if constexpr (SPLIT)
-            qf[NS - 1][rb][i][h] = f16x2_rest(x, y, qf[0][rb][i][h]);
-        }
+        for (int i = 0; i < KW; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float x = v[4 * i + 2 * h] * f, y = v[4 * i + 2 * h + 1] * f;
+            qf[0][rb][i][h] = f16x2(x, y);
+            if constexpr (SPLIT)
+              qf[NS - 1][rb][i][h] = f16x2_rest(x, y, qf[0][rb][i][h]);
+          }
+      }
     }
 
-    float o[NR][NT][4], m[NR][2], l[NR][2];
-#pragma unroll
-    for (int rb = 0; rb < NR; ++rb) {
-      m[rb][0] = m[rb][1] = -INFINITY, l[rb][0] = l[rb][1] = 0.f;
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-        o[rb][j][0] = o[rb][j][1] = o[rb][j][2] = o[rb][j][3] = 0.f;
-    }
+    // log2 and reciprocal of the V scales; no page: no weight
+    const float my_vs = fmaxf(cur.vs, 0x1p-64f);
+    const float my_lv = cur.page >= 0 ? log2f(my_vs) : -INFINITY, my_iv = cur.page >= 0 ? 1.f / my_vs : 0.f;
 
-    for (int i = 0; i < tiles; ++i) {
-      if (i % BATCH == 0 && i > 0)
-        cur = nxt, nxt = load_half(a, g, half_key(i / BATCH + 1), end);
-      issue(i + 1, (i + 1) % BATCH != 0 ? cur : nxt);
+    ahead = false;
+    for (int i = 0; i < cur.tiles; ++i) {
+      if (i + 1 < cur.tiles) {
+        issue(cur, i + 1, stage ^ 1);
+      } else if (TEAM == 1 || !cur.last) {
+        scales(nxt);
+        issue(nxt, 0, stage ^ 1);
+        ahead = true;
+      } else {
+        cp_async_commit(); // the ring is needed for the join
+      }
       cp_async_wait<1>();
       __syncwarp();
-      const unsigned char *kt = ring + (i & 1) * 2 * Cfg::TILE_BYTES, *vt = kt + Cfg::TILE_BYTES;
-      const int key0 = first + i * TILE;
+      const unsigned char *kt = ring + stage * 2 * Cfg::TILE_BYTES, *vt = kt + Cfg::TILE_BYTES;
+      const int key0 = cur.key0 + i * STEP;
       const bool edge = key0 + TILE > least;
 
       // scores, in units of log2, with log2 of the V scale
@@ -731,9 +816,9 @@ __global__ void __launch_bounds__(MmaCfg<DP, NR, sizeof(T) == 4>::THREADS, MmaCf
             }
           }
         }
-        const int src = (i % BATCH) * MT + mt;
-        const float ks = __shfl_sync(~0u, cur.ks, src), lv = __shfl_sync(~0u, cur.lv, src);
-        iv[mt] = __shfl_sync(~0u, cur.iv, src);
+        const int src = i * MT + mt;
+        const float ks = __shfl_sync(~0u, cur.ks, src), lv = __shfl_sync(~0u, my_lv, src);
+        iv[mt] = __shfl_sync(~0u, my_iv, src);
 #pragma unroll
         for (int rb = 0; rb < NR; ++rb)
 #pragma unroll
@@ -863,153 +948,252 @@ __global__ void __launch_bounds__(MmaCfg<DP, NR, sizeof(T) == 4>::THREADS, MmaCf
         }
       }
       __syncwarp(); // the stage may be overwritten
+      stage ^= 1;
     }
-    cp_async_wait<0>();
 
+    if constexpr (TEAM > 1) {
+      if (cur.last) { // every warp's rows through its ring, then the CTA joins them
+        cp_async_wait<0>();
+        __syncwarp();
+        float *mine = reinterpret_cast<float *>(ring);
 #pragma unroll
-    for (int rb = 0; rb < NR; ++rb)
+        for (int rb = 0; rb < NR; ++rb)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float sum = l[rb][e];
+          for (int e = 0; e < 2; ++e) {
+            float sum = l[rb][e];
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1)
-          sum += __shfl_xor_sync(~0u, sum, d);
-        const int r = rb * 8 + quad * 2 + e;
-        if (r >= g.n_rows)
-          continue;
-        if (g.slot < 0) {
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          const int row = g.row0 + r;
-          T *p = static_cast<T *>(a.out) + (s.q0 + row / a.G) * a.out_ld + (1ll * g.head * a.G + row % a.G) * D;
-          const bool vec = (reinterpret_cast<uintptr_t>(p) & (2 * sizeof(T) - 1)) == 0;
+            for (int d = 4; d < 32; d <<= 1)
+              sum += __shfl_xor_sync(~0u, sum, d);
+            const int r = rb * 8 + quad * 2 + e;
+            if (grp == 0)
+              team_ml[warp][r] = make_float2(m[rb][e] - W_EXP, sum);
+            if (r < cur.n_rows)
 #pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            const int d = grp * (DP / 8) + 2 * j;
-            // the reciprocal is off by half a unit; float32 takes the quotient
-            const float x = SPLIT ? (sum == 0.f ? 0.f : o[rb][j][e] / sum) : o[rb][j][e] * inv;
-            const float y = SPLIT ? (sum == 0.f ? 0.f : o[rb][j][e + 2] / sum) : o[rb][j][e + 2] * inv;
-            if (d >= D)
-              continue;
-            if (vec && sizeof(T) == 2) {
-              *reinterpret_cast<uint32_t *>(p + d) = pack_bf16x2(x, y);
-            } else if (vec) {
-              *reinterpret_cast<float2 *>(p + d) = make_float2(x, y);
-            } else {
-              store_out(p + d, x), store_out(p + d + 1, y);
+              for (int j = 0; j < NT; ++j)
+                *reinterpret_cast<float2 *>(mine + r * DP + grp * (DP / 8) + 2 * j) = make_float2(o[rb][j][e], o[rb][j][e + 2]);
+          }
+        __syncthreads();
+        for (int r = warp; r < cur.n_rows; r += Cfg::WARPS) {
+          float M = -INFINITY, sum = 0.f, w[Cfg::WARPS];
+#pragma unroll
+          for (int t = 0; t < Cfg::WARPS; ++t)
+            M = fmaxf(M, team_ml[t][r].x);
+#pragma unroll
+          for (int t = 0; t < Cfg::WARPS; ++t) {
+            w[t] = rel_weight(team_ml[t][r].x, M);
+            sum = fmaf(w[t], team_ml[t][r].y, sum);
+          }
+          const int row = cur.row0 + r;
+          const long long pr = 1ll * cur.slot * R + r;
+          T *p = static_cast<T *>(a.out) + (cur.q0 + row / a.G) * a.out_ld + (1ll * cur.head * a.G + row % a.G) * D;
+          for (int d = lane; d < D; d += 32) {
+            float x = 0.f;
+#pragma unroll
+            for (int t = 0; t < Cfg::WARPS; ++t)
+              x = fmaf(w[t], reinterpret_cast<const float *>(smem_raw + t * Cfg::WARP_BYTES)[r * DP + d], x);
+            if (cur.slot < 0)
+              store_out(p + d, sum == 0.f ? 0.f : x / sum);
+            else
+              a.part_o[pr * D + d] = x;
+          }
+          if (cur.slot >= 0 && lane == 0)
+            a.part_ml[pr] = make_float2(M, sum);
+        }
+        __syncthreads(); // the rings are free again
+      }
+    } else if (cur.last) {
+#pragma unroll
+      for (int rb = 0; rb < NR; ++rb)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float sum = l[rb][e];
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1)
+            sum += __shfl_xor_sync(~0u, sum, d);
+          const int r = rb * 8 + quad * 2 + e;
+          if (r >= cur.n_rows)
+            continue;
+          if (cur.slot < 0) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const int row = cur.row0 + r;
+            T *p = static_cast<T *>(a.out) + (cur.q0 + row / a.G) * a.out_ld + (1ll * cur.head * a.G + row % a.G) * D;
+            const bool vec = (reinterpret_cast<uintptr_t>(p) & (2 * sizeof(T) - 1)) == 0;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              const int d = grp * (DP / 8) + 2 * j;
+              // the reciprocal is off by half a unit; float32 takes the quotient
+              const float x = SPLIT ? (sum == 0.f ? 0.f : o[rb][j][e] / sum) : o[rb][j][e] * inv;
+              const float y = SPLIT ? (sum == 0.f ? 0.f : o[rb][j][e + 2] / sum) : o[rb][j][e + 2] * inv;
+              if (d >= D)
+                continue;
+              if (vec && sizeof(T) == 2) {
+                *reinterpret_cast<uint32_t *>(p + d) = pack_bf16x2(x, y);
+              } else if (vec) {
+                *reinterpret_cast<float2 *>(p + d) = make_float2(x, y);
+              } else {
+                store_out(p + d, x), store_out(p + d + 1, y);
+              }
+            }
+          } else {
+            const long long pr = 1ll * cur.slot * R + r;
+            if (grp == 0)
+              a.part_ml[pr] = make_float2(m[rb][e] - W_EXP, sum);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              const int d = grp * (DP / 8) + 2 * j;
+              if (d < D)
+                *reinterpret_cast<float2 *>(a.part_o + pr * D + d) = make_float2(o[rb][j][e], o[rb][j][e + 2]);
             }
           }
-        } else {
-          const long long pr = 1ll * g.slot * R + r;
-          if (grp == 0)
-            a.part_ml[pr] = make_float2(m[rb][e] - W_EXP, sum);
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            const int d = grp * (DP / 8) + 2 * j;
-            if (d < D)
-              *reinterpret_cast<float2 *>(a.part_o + pr * D + d) = make_float2(o[rb][j][e], o[rb][j][e + 2]);
-          }
         }
-      }
-    __syncwarp();
+      __syncwarp();
+    }
+    cur = nxt, more = more_after;
   }
+  cp_async_wait<0>();
 }
 
 // ---- joining the pieces ---------------------------------------------------------------------------
-// A fixed grid; every CTA lists the split items (their flags fit a few loads) and takes every gridDim-th
-// (item, row). Its warps share the row's pieces. Launched so that it may become resident while the main
+// One CTA per worker of the main kernel. The rows of an item with P pieces are dealt out to the CTAs of
+// the first P workers that have a piece of it, so that one long request is not joined by one CTA; a warp
+// joins a row, or all warps where the pieces are many. Time here is latency (note -> item -> maxima ->
+// rows), so every step loads all it needs at once. Launched so that it may become resident while the main
 // kernel drains; griddepcontrol.wait orders its reads after that kernel's writes.
-constexpr int JOIN_THREADS = 128, JOIN_WARPS = JOIN_THREADS / 32;
-template <typename T> __global__ void __launch_bounds__(JOIN_THREADS) attention_paged_join_kernel(PagedArgs a, int workers) {
-  extern __shared__ int list[]; // (item, first of its rows in the list of rows) pairs
-  __shared__ int warp_sum[2][JOIN_WARPS];
-  __shared__ float red_o[JOIN_WARPS][256];
-  __shared__ float2 red_ml[JOIN_WARPS];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  int items = 0, rows = 0;
-  for (int w0 = 0; w0 < workers; w0 += JOIN_THREADS) {
-    const int n = w0 + tid < workers ? a.items[w0 + tid].n_rows : 0;
-    const unsigned used = __ballot_sync(~0u, n > 0);
-    int inc = n;
+constexpr int JOIN_THREADS = 128, JOIN_WARPS = JOIN_THREADS / 32, JOIN_DIMS = 8; // dimensions per lane: D <= 256
+
+// Where lane `lane` keeps dimension v of its JOIN_DIMS: four in a row where rows are whole 16-byte words.
+__device__ __forceinline__ int join_dim(int D, int lane, int v) {
+  return D % 4 == 0 ? (v >> 2) * 128 + lane * 4 + (v & 3) : lane + 32 * v;
+}
+struct Joined {
+  float M, sum, o[JOIN_DIMS];
+};
+// Pieces first, first + step, ... of one row, by one warp.
+__device__ __forceinline__ Joined join_pieces(const PagedArgs &a, const SplitItem &it, int owner, int r, int first, int step,
+                                              int pieces) {
+  const int lane = threadIdx.x & 31;
+  Joined j;
+  j.M = -INFINITY, j.sum = 0.f;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int t = __shfl_up_sync(~0u, inc, d);
-      if (lane >= d)
-        inc += t;
-    }
-    __syncthreads();
-    if (lane == 31)
-      warp_sum[0][warp] = __popc(used), warp_sum[1][warp] = inc;
-    __syncthreads();
-    int at = items + __popc(used & ((1u << lane) - 1)), row = rows + inc - n;
+  for (int v = 0; v < JOIN_DIMS; ++v)
+    j.o[v] = 0.f;
+  auto row_of = [&](int i) { return 1ll * (i == 0 ? it.first_slot : 2 * (owner + i)) * a.rows_per_tile + r; };
+  for (int p0 = first; p0 < pieces; p0 += 32 * step) {
+    const int mine = p0 + lane * step;
+    const float2 ml = mine < pieces ? a.part_ml[row_of(mine)] : make_float2(-INFINITY, 0.f);
+    float top = fmaxf(ml.x, j.M);
 #pragma unroll
-    for (int w = 0; w < JOIN_WARPS; ++w) {
-      if (w < warp)
-        at += warp_sum[0][w], row += warp_sum[1][w];
-      items += warp_sum[0][w], rows += warp_sum[1][w];
-    }
-    if (n > 0)
-      list[2 * at] = w0 + tid, list[2 * at + 1] = row;
-  }
-  __syncthreads();
-  constexpr int V = 8; // dimensions a lane may hold
-  for (int k = blockIdx.x; k < rows; k += gridDim.x) {
-    int lo = 0, hi = items - 1; // the last item whose first row is <= k
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (list[2 * mid + 1] <= k)
-        lo = mid;
-      else
-        hi = mid - 1;
-    }
-    const int owner = list[2 * lo], r = k - list[2 * lo + 1];
-    const SplitItem it = a.items[owner];
-    const int pieces = it.last - owner + 1;
-    float M = -INFINITY, sum = 0.f, o[V];
+    for (int d = 16; d; d >>= 1)
+      top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+    const float old = rel_weight(j.M, top), h = mine < pieces ? rel_weight(ml.x, top) : 0.f;
+    float sum = mine < pieces ? h * ml.y : 0.f;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      o[v] = 0.f;
-#pragma unroll 4
-    for (int i = warp; i < pieces; i += JOIN_WARPS) {
-      const long long pr = 1ll * (i == 0 ? it.first_slot : 2 * (owner + i)) * a.rows_per_tile + r;
-      const float2 ml = a.part_ml[pr];
-      float x[V];
+    for (int d = 16; d; d >>= 1)
+      sum += __shfl_xor_sync(~0u, sum, d);
+    j.sum = j.sum * old + sum, j.M = top;
 #pragma unroll
-      for (int v = 0; v < V; ++v)
-        x[v] = lane + 32 * v < a.D ? a.part_o[pr * a.D + lane + 32 * v] : 0.f;
-      const float top = fmaxf(M, ml.x), f = rel_weight(M, top), h = rel_weight(ml.x, top);
-      sum = sum * f + ml.y * h, M = top;
+    for (int v = 0; v < JOIN_DIMS; ++v)
+      j.o[v] *= old;
+    const int n = min(32, (pieces - p0 + step - 1) / step);
+    auto add = [&](auto dims, auto count, int i0) { // some pieces, their loads first
+      constexpr int V = decltype(dims)::value, E = decltype(count)::value;
+      float x[E][V];
 #pragma unroll
-      for (int v = 0; v < V; ++v)
-        o[v] = o[v] * f + x[v] * h;
-    }
-    if (lane == 0)
-      red_ml[warp] = make_float2(M, sum);
+      for (int e = 0; e < E; ++e) {
+        const float *src = a.part_o + row_of(p0 + min(i0 + e, n - 1) * step) * a.D;
+        if (a.D % 4 == 0) {
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      red_o[warp][lane + 32 * v] = o[v];
-    __syncthreads();
-    M = -INFINITY;
+          for (int v = 0; v < V; v += 4) {
+            const int d = join_dim(a.D, lane, v);
+            const float4 q = d < a.D ? *reinterpret_cast<const float4 *>(src + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[e][v] = q.x, x[e][v + 1] = q.y, x[e][v + 2] = q.z, x[e][v + 3] = q.w;
+          }
+        } else {
 #pragma unroll
-    for (int w = 0; w < JOIN_WARPS; ++w)
-      M = fmaxf(M, red_ml[w].x);
-    const int row = it.row0 + r;
-    T *out = static_cast<T *>(a.out) + (it.q0 + row / a.G) * a.out_ld + (1ll * it.head * a.G + row % a.G) * a.D;
-    for (int d = tid; d < a.D; d += JOIN_THREADS) {
-      float all = 0.f, x = 0.f;
-#pragma unroll
-      for (int w = 0; w < JOIN_WARPS; ++w) {
-        const float f = rel_weight(red_ml[w].x, M);
-        all += f * red_ml[w].y, x += f * red_o[w][d];
+          for (int v = 0; v < V; ++v)
+            x[e][v] = lane + 32 * v < a.D ? src[lane + 32 * v] : 0.f;
+        }
       }
-      store_out(out + d, all == 0.f ? 0.f : x / all);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float w = __shfl_sync(~0u, h, min(i0 + e, 31));
+        if (i0 + e < n)
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+            j.o[v] = fmaf(w, x[e][v], j.o[v]);
+      }
+    };
+    using Four = std::integral_constant<int, 4>;
+    using Eight = std::integral_constant<int, JOIN_DIMS>;
+    if (a.D > 128) {
+      for (int i0 = 0; i0 < n; i0 += 8)
+        add(Eight{}, Eight{}, i0);
+    } else if (n <= 4) {
+      add(Four{}, Four{}, 0);
+    } else {
+      for (int i0 = 0; i0 < n; i0 += 16)
+        add(Four{}, std::integral_constant<int, 16>{}, i0);
     }
-    __syncthreads();
+  }
+  return j;
+}
+
+template <typename T> __global__ void __launch_bounds__(JOIN_THREADS) attention_paged_join_kernel(PagedArgs a) {
+  __shared__ float red_o[JOIN_WARPS][32 * JOIN_DIMS];
+  __shared__ float2 red_ml[JOIN_WARPS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, me = blockIdx.x;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int2 note = a.notes[me];
+#pragma unroll 1
+  for (int job = 0; job < 2; ++job) { // the item this worker began, the one its first segment continued
+    const int owner = job == 0 ? me : note.y;
+    if (job == 0 ? note.x == 0 : note.y < 0)
+      continue;
+    const SplitItem it = a.items[owner];
+    const int pieces = it.last - owner + 1, share = min(pieces, it.n_rows);
+    auto out_row = [&](int r) {
+      const int row = it.row0 + r;
+      return static_cast<T *>(a.out) + (it.q0 + row / a.G) * a.out_ld + (1ll * it.head * a.G + row % a.G) * a.D;
+    };
+    if (pieces <= 16) {
+      for (int r = me - owner + warp * share; r < it.n_rows; r += JOIN_WARPS * share) {
+        const Joined j = join_pieces(a, it, owner, r, 0, 1, pieces);
+        T *out = out_row(r);
+#pragma unroll
+        for (int v = 0; v < JOIN_DIMS; ++v)
+          if (const int d = join_dim(a.D, lane, v); d < a.D)
+            store_out(out + d, j.sum == 0.f ? 0.f : j.o[v] / j.sum);
+      }
+    } else {
+      for (int r = me - owner; r < it.n_rows; r += share) {
+        const Joined j = join_pieces(a, it, owner, r, warp, JOIN_WARPS, pieces);
+        if (lane == 0)
+          red_ml[warp] = make_float2(j.M, j.sum);
+#pragma unroll
+        for (int v = 0; v < JOIN_DIMS; ++v)
+          red_o[warp][join_dim(a.D, lane, v)] = j.o[v];
+        __syncthreads();
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < JOIN_WARPS; ++w)
+          M = fmaxf(M, red_ml[w].x);
+        for (int d = tid; d < a.D; d += JOIN_THREADS) {
+          float all = 0.f, x = 0.f;
+#pragma unroll
+          for (int w = 0; w < JOIN_WARPS; ++w) {
+            const float f = rel_weight(red_ml[w].x, M);
+            all += f * red_ml[w].y, x += f * red_o[w][d];
+          }
+          store_out(out_row(r) + d, all == 0.f ? 0.f : x / all);
+        }
+        __syncthreads();
+      }
+    }
   }
 }
 
 // ---- host -----------------------------------------------------------------------------------------
-constexpr int SIMT_CTAS_PER_SM = 4, JOIN_CTAS_PER_SM = 4;
+constexpr int SIMT_CTAS_PER_SM = 4;
 constexpr int MAX_WORKERS_PER_SM = 12;
 
 // Rows of partial results over all workers: 12 workers of 8 rows, 8 of 16, or 4 CTAs of 8 per SM, two each.
@@ -1017,18 +1201,17 @@ constexpr size_t MAX_PART_ROWS_PER_SM = 2 * 128;
 
 size_t paged_workspace_bytes(int num_sms, int D) {
   const size_t rows = static_cast<size_t>(num_sms) * MAX_PART_ROWS_PER_SM;
-  return rows * (sizeof(float) * D + sizeof(float2)) + sizeof(SplitItem) * num_sms * MAX_WORKERS_PER_SM;
+  return rows * (sizeof(float) * D + sizeof(float2)) + (sizeof(SplitItem) + sizeof(int2)) * num_sms * MAX_WORKERS_PER_SM;
 }
 
-template <typename T> int launch_join(const PagedArgs &a, int workers, int num_sms, cudaStream_t st) {
+template <typename T> int launch_join(const PagedArgs &a, int workers, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(num_sms * JOIN_CTAS_PER_SM), cfg.blockDim = dim3(JOIN_THREADS), cfg.stream = st;
-  cfg.dynamicSmemBytes = 2 * sizeof(int) * workers;
+  cfg.gridDim = dim3(workers), cfg.blockDim = dim3(JOIN_THREADS), cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at, cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attention_paged_join_kernel<T>, a, workers) == cudaSuccess ? 0 : 2;
+  return cudaLaunchKernelEx(&cfg, attention_paged_join_kernel<T>, a) == cudaSuccess ? 0 : 2;
 }
 
 template <typename T, int RT, int VB, int NA> int launch_simt(PagedArgs a, int num_sms, cudaStream_t st) {
@@ -1047,7 +1230,7 @@ template <typename T, int RT, int VB, int NA> int launch_simt(PagedArgs a, int n
   attention_paged_simt_kernel<T, RT, VB, NA><<<ctas, SIMT_THREADS, smem, st>>>(a);
   if (cudaGetLastError() != cudaSuccess)
     return 2;
-  return launch_join<T>(a, ctas, num_sms, st);
+  return launch_join<T>(a, ctas, st);
 }
 template <typename T, int VB, int NA> int launch_simt_rows(const PagedArgs &a, int num_sms, cudaStream_t st) {
   // rows that share a key: the group's heads for single tokens, up to 8 otherwise
@@ -1059,25 +1242,34 @@ template <typename T, int VB, int NA> int launch_simt_rows(const PagedArgs &a, i
   return launch_simt<T, 8, VB, NA>(a, num_sms, st);
 }
 
-template <typename T, int DP, int NR> int launch_mma(PagedArgs a, int num_sms, cudaStream_t st) {
-  using Cfg = MmaCfg<DP, NR, sizeof(T) == 4>;
+template <typename T, int DP, int NR, int TEAM> int launch_mma_team(PagedArgs a, int num_sms, cudaStream_t st) {
+  using Cfg = MmaCfg<DP, NR, TEAM, sizeof(T) == 4>;
   constexpr size_t ring = Cfg::WARPS * Cfg::WARP_BYTES;
   static_assert(ring + 8 * MU_ATTENTION_PAGED_MAX_REQUESTS <= 227 * 1024, "shared memory");
   static_assert(Cfg::CTAS_PER_SM * Cfg::WARPS <= MAX_WORKERS_PER_SM, "workspace");
   static_assert(2 * Cfg::CTAS_PER_SM * Cfg::WARPS * Cfg::R <= MAX_PART_ROWS_PER_SM, "workspace");
   static PerDeviceOnce once;
   if (once.get() < 0) {
-    if (cudaFuncSetAttribute(attention_paged_mma_kernel<T, DP, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (cudaFuncSetAttribute(attention_paged_mma_kernel<T, DP, NR, TEAM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              ring + 8 * MU_ATTENTION_PAGED_MAX_REQUESTS) != cudaSuccess)
       return 2;
     once.set(1);
   }
   const int ctas = num_sms * Cfg::CTAS_PER_SM;
   a.rows_per_tile = Cfg::R;
-  attention_paged_mma_kernel<T, DP, NR><<<ctas, Cfg::THREADS, ring + 8ull * a.B, st>>>(a);
+  attention_paged_mma_kernel<T, DP, NR, TEAM><<<ctas, Cfg::THREADS, ring + 8ull * a.B, st>>>(a);
   if (cudaGetLastError() != cudaSuccess)
     return 2;
-  return launch_join<T>(a, ctas * Cfg::WARPS, num_sms, st);
+  return launch_join<T>(a, ctas * Cfg::WARPS / TEAM, st);
+}
+template <typename T, int DP, int NR> int launch_mma(const PagedArgs &a, int num_sms, cudaStream_t st) {
+  // Items (an upper bound) against warps: below an eighth every item would be cut into more than eight
+  // pieces, and CTAs become the workers.
+  const long long tiles = (1ll * a.n_tokens * a.G + 8 * NR - 1) / (8 * NR);
+  const long long items = a.Hkv * (tiles > a.B ? tiles : a.B);
+  if (items * 8 <= 1ll * num_sms * MmaCfg<DP, NR, 1, sizeof(T) == 4>::CTAS_PER_SM * MmaCfg<DP, NR, 1, sizeof(T) == 4>::WARPS)
+    return launch_mma_team<T, DP, NR, 4>(a, num_sms, st);
+  return launch_mma_team<T, DP, NR, 1>(a, num_sms, st);
 }
 
 template <typename T> int launch_by_dim(const PagedArgs &a, int num_sms, cudaStream_t st) {
@@ -1107,6 +1299,8 @@ int launch_attention_paged(PagedArgs a, void *workspace, int dtype, int num_sms,
   w += sizeof(float) * rows * a.D;
   a.part_ml = reinterpret_cast<float2 *>(w);
   w += sizeof(float2) * rows;
+  a.notes = reinterpret_cast<int2 *>(w);
+  w += sizeof(int2) * num_sms * MAX_WORKERS_PER_SM;
   a.items = reinterpret_cast<SplitItem *>(w);
   if (dtype == F32)
     return launch_by_dim<float>(a, num_sms, st);
