@@ -11,7 +11,7 @@
 // are. A worker walks its range as segments, one per (request, head, row tile). A segment that covers
 // all chunks writes its rows; one that does not leaves (running maximum, sum, weighted values) in the
 // workspace, and a second small kernel joins the pieces. No atomics: results do not depend on the order
-// in which workers run. Every item counts one unit more than its chunks, for what starting a segment
+// in which workers run. Every item counts a few units more than its chunks, for what starting a segment
 // costs: without it the workers that got many short requests finished last.
 #include "../../include/munet_b200.h"
 #include "common.h"
@@ -24,6 +24,21 @@
 
 namespace mu {
 
+// Division by a number known at launch: n / d for n < 2^31 (mul = ceil(2^(31 + shift) / d), 2^shift >= d).
+struct FastDiv {
+  unsigned d, mul, shift;
+  FastDiv() = default;
+  explicit FastDiv(int by) : d(by), shift(0) {
+    while ((1ull << shift) < d)
+      ++shift;
+    mul = static_cast<unsigned>(((1ull << (31 + shift)) + d - 1) / d);
+  }
+  __device__ __forceinline__ int div(int n) const { // mul has 32 bits: 2^31 <= mul <= 2^32 - 1 for d > 1
+    return d == 1 ? n : static_cast<int>(__umulhi(static_cast<unsigned>(n) << 1, mul) >> shift);
+  }
+  __device__ __forceinline__ int mod(int n) const { return n - div(n) * static_cast<int>(d); }
+};
+
 struct PagedArgs {
   const void *q;
   void *out;
@@ -34,6 +49,7 @@ struct PagedArgs {
   int table_stride;
   const int *query_start, *seq_lens;
   int B, n_tokens, Hq, Hkv, G, D, num_pages, page_size, causal;
+  FastDiv by_group, by_page;
   float scale_log2; // log2(e) / sqrt(D)
   struct SplitItem *items; // by the worker that holds the first chunk
   int2 *notes;             // per worker: rows of the split item it begins (0: none), worker that began the
@@ -50,7 +66,7 @@ struct SplitItem {
   int first_slot, last, row0, n_rows, q0, head;
 };
 
-constexpr int START_UNITS = 1; // what beginning an item counts for
+constexpr int START_UNITS = 3; // what beginning an item counts for, in chunks (1: 69.3 us, 2: 67.3, 3: 66.3 for 64 requests)
 
 struct Seq {
   int q0, nq, len;  // first row of q, new tokens, tokens in the cache (as given)
@@ -89,7 +105,7 @@ __device__ __forceinline__ int row_limit(const PagedArgs &a, const Seq &s, int r
     return 0;
   if (!a.causal)
     return s.seen;
-  return max(0, min(s.seen, s.len - s.nq + row / a.G + 1));
+  return max(0, min(s.seen, s.len - s.nq + a.by_group.div(row) + 1));
 }
 
 // Inclusive prefix of units over the requests into shared memory; returns the total.
@@ -132,15 +148,16 @@ struct Segment {
   int slot;                  // -1: complete
 };
 
-// Quotient and remainder; units of one request hardly ever need 64 bits.
-__device__ __forceinline__ long long div_rem(long long x, int d, int &rem) {
-  if (x >> 32 == 0) {
-    const unsigned q = static_cast<unsigned>(x) / static_cast<unsigned>(d);
-    rem = static_cast<int>(static_cast<unsigned>(x) - q * static_cast<unsigned>(d));
-    return q;
-  }
-  rem = static_cast<int>(x % d);
+// Unit counts hardly ever need 64 bits, and a 64-bit division costs a hundred instructions.
+__device__ __forceinline__ long long div64(long long x, long long d) {
+  if (((x | d) >> 32) == 0)
+    return static_cast<unsigned>(x) / static_cast<unsigned>(d);
   return x / d;
+}
+__device__ __forceinline__ long long div_rem(long long x, int d, int &rem) {
+  const long long q = div64(x, d);
+  rem = static_cast<int>(x - q * d);
+  return q;
 }
 
 // Walks one worker's share of the unit list.
@@ -148,26 +165,19 @@ template <int R, int CHUNK> struct Walk {
   long long u, end, total;
   int workers, me, b;
   bool first;
-  __device__ __forceinline__ long long start(int w) const { // floor(total * w / workers)
-    return total / workers * w + total % workers * w / workers;
-  }
   __device__ __forceinline__ Walk(long long total_, int me_, int workers_) : total(total_), me(me_), b(0), first(true) {
     workers = static_cast<int>(min(static_cast<long long>(workers_), total_)); // every active one has a unit
     u = end = 0;
-    if (me < workers)
-      u = start(me), end = start(me + 1);
-  }
-  // the worker that holds unit x: the largest w with start(w) <= x
-  __device__ __forceinline__ int owner(long long x) const {
-    int lo = 0, hi = workers - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (start(mid) <= x)
-        lo = mid;
-      else
-        hi = mid - 1;
+    if (me < workers) { // start(w) = floor(total * w / workers)
+      int rest;
+      const long long each = div_rem(total, workers, rest);
+      u = each * me + static_cast<unsigned>(rest * me) / static_cast<unsigned>(workers);
+      end = each * (me + 1) + static_cast<unsigned>(rest * (me + 1)) / static_cast<unsigned>(workers);
     }
-    return lo;
+  }
+  // the worker that holds unit x: the largest w with total * w < (x + 1) * workers
+  __device__ __forceinline__ int owner(long long x) const {
+    return static_cast<int>(div64((x + 1) * workers - 1, total));
   }
   // The next segment. `leader`: the thread that notes down a split item.
   __device__ __forceinline__ bool next(const PagedArgs &a, const long long *upto, Segment &g, Seq &s, bool leader) {
@@ -257,15 +267,14 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_paged_simt_kernel(Page
   Walk<RT, SIMT_CHUNK> walk(total, blockIdx.x, gridDim.x);
   Segment g;
   Seq s;
-  const unsigned ps = a.page_size;
   while (walk.next(a, upto, g, s, tid == 0)) {
     for (int e = tid; e < RT * Dq; e += SIMT_THREADS) {
       const int r = e / Dq, d = e - r * Dq;
       float v = 0.f;
       if (r < g.n_rows && d < a.D) {
         const int row = g.row0 + r;
-        v = load_in(static_cast<const T *>(a.q) + (s.q0 + row / a.G) * a.q_ld +
-                    (1ll * g.head * a.G + row % a.G) * a.D + d);
+        v = load_in(static_cast<const T *>(a.q) + (s.q0 + a.by_group.div(row)) * a.q_ld +
+                    (1ll * g.head * a.G + a.by_group.mod(row)) * a.D + d);
       }
       q_s[e] = v * a.scale_log2;
     }
@@ -295,10 +304,10 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_paged_simt_kernel(Page
       long long row = -1;
       float kscale = 0.f, vscale = 0.f;
       if (j < most) {
-        const int page = a.table[1ll * g.b * a.table_stride + j / ps];
+        const int page = a.table[1ll * g.b * a.table_stride + a.by_page.div(j)];
         if (page >= 0 && page < a.num_pages) {
           const long long tile = 1ll * page * a.Hkv + g.head;
-          row = tile * ps + j % ps;
+          row = tile * a.page_size + a.by_page.mod(j);
           kscale = a.ks[tile], vscale = a.vs[tile];
         } else {
           atomicCAS(a.status, 0, MU_DEV_BAD_PAGE);
@@ -435,8 +444,8 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_paged_simt_kernel(Page
       }
       if (g.slot < 0) {
         const int row = g.row0 + r;
-        store_out(static_cast<T *>(a.out) + (s.q0 + row / a.G) * a.out_ld +
-                      (1ll * g.head * a.G + row % a.G) * a.D + d,
+        store_out(static_cast<T *>(a.out) + (s.q0 + a.by_group.div(row)) * a.out_ld +
+                      (1ll * g.head * a.G + a.by_group.mod(row)) * a.D + d,
                   sum == 0.f ? 0.f : o / sum);
       } else {
         const long long pr = 1ll * g.slot * a.rows_per_tile + r;
@@ -582,6 +591,7 @@ __global__ void __launch_bounds__(MmaCfg<DP, NR, TEAM, sizeof(T) == 4>::THREADS,
   // neighbouring workers sit on different SMs, so that a short list spreads out
   const int me = TEAM == 1 ? warp * gridDim.x + blockIdx.x : blockIdx.x;
   const bool leader = TEAM == 1 ? lane == 0 : tid == 0;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); // the join waits for the whole grid anyway
   if (leader)
     a.notes[me] = make_int2(0, -1);
   __syncwarp();
@@ -589,7 +599,6 @@ __global__ void __launch_bounds__(MmaCfg<DP, NR, TEAM, sizeof(T) == 4>::THREADS,
   if (total == 0)
     return;
   Walk<R, Cfg::CHUNK> walk(total, me, gridDim.x * (Cfg::WARPS / TEAM));
-  const unsigned ps = a.page_size;
   const int D = a.D;
   // The walk as a stream of batches: up to 32 half tiles of one segment, whose pages and scales the lanes
   // hold. The batch after the current one is looked up while that runs, in steps that do not wait for one
@@ -617,8 +626,8 @@ __global__ void __launch_bounds__(MmaCfg<DP, NR, TEAM, sizeof(T) == 4>::THREADS,
       seg_end = min(row_limit(a, s, g.row0 + g.n_rows - 1), (g.chunk0 + g.chunks) * Cfg::CHUNK);
       const int r = g.row0 + grp; // its queries: into L1
       if (grp < g.n_rows)
-        asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const T *>(a.q) + (s.q0 + r / a.G) * a.q_ld +
-                                                    (1ll * g.head * a.G + r % a.G) * D + quad * D / 4));
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const T *>(a.q) + (s.q0 + a.by_group.div(r)) * a.q_ld +
+                                                    (1ll * g.head * a.G + a.by_group.mod(r)) * D + quad * D / 4));
     }
     n.head = g.head, n.row0 = g.row0, n.n_rows = g.n_rows, n.slot = g.slot;
     n.q0 = s.q0, n.nq = s.nq, n.len = s.len, n.seen = s.seen;
@@ -627,7 +636,7 @@ __global__ void __launch_bounds__(MmaCfg<DP, NR, TEAM, sizeof(T) == 4>::THREADS,
     const int key = half_key(n);
     n.page = -2; // not looked for
     if (lane / MT < n.tiles && key < seg_end)
-      n.page = a.table[1ll * g.b * a.table_stride + static_cast<unsigned>(key) / ps];
+      n.page = a.table[1ll * g.b * a.table_stride + a.by_page.div(key)];
     seg_key += BATCH * STEP;
     open = seg_key < seg_end;
     n.last = !open;
@@ -651,8 +660,8 @@ __global__ void __launch_bounds__(MmaCfg<DP, NR, TEAM, sizeof(T) == 4>::THREADS,
       for (int hf = 0; hf < MT; ++hf) {
         const int page = __shfl_sync(~0u, n.page, i * MT + hf);
         const int key = n.key0 + i * STEP + 16 * hf, live = page >= 0 ? n.seen - key : 0; // behind it: anything
-        const unsigned in_page = static_cast<unsigned>(key) % ps;
-        const long long off = page >= 0 ? ((1ll * page * a.Hkv + n.head) * ps + in_page) * D : 0;
+        const int in_page = a.by_page.mod(key);
+        const long long off = page >= 0 ? ((1ll * page * a.Hkv + n.head) * a.page_size + in_page) * D : 0;
         if (D == DP && live >= 16) { // sixteen whole rows: one run of bytes
           const uint8_t *kp = a.kc + off + lane * 16, *vp = a.vc + off + lane * 16;
 #pragma unroll
@@ -717,7 +726,7 @@ __global__ void __launch_bounds__(MmaCfg<DP, NR, TEAM, sizeof(T) == 4>::THREADS,
         const int r = rb * 8 + grp, row = cur.row0 + r;
         const bool live = r < cur.n_rows;
         const T *qp = static_cast<const T *>(a.q) +
-                      (live ? (cur.q0 + row / a.G) * a.q_ld + (1ll * cur.head * a.G + row % a.G) * D : 0);
+                      (live ? (cur.q0 + a.by_group.div(row)) * a.q_ld + (1ll * cur.head * a.G + a.by_group.mod(row)) * D : 0);
         const bool vec = (reinterpret_cast<uintptr_t>(qp) & 7u) == 0;
         float (&v)[DP / 4] = qv[rb];
 #pragma unroll
@@ -985,7 +994,7 @@ __global__ void __launch_bounds__(MmaCfg<DP, NR, TEAM, sizeof(T) == 4>::THREADS,
           }
           const int row = cur.row0 + r;
           const long long pr = 1ll * cur.slot * R + r;
-          T *p = static_cast<T *>(a.out) + (cur.q0 + row / a.G) * a.out_ld + (1ll * cur.head * a.G + row % a.G) * D;
+          T *p = static_cast<T *>(a.out) + (cur.q0 + a.by_group.div(row)) * a.out_ld + (1ll * cur.head * a.G + a.by_group.mod(row)) * D;
           for (int d = lane; d < D; d += 32) {
             float x = 0.f;
 #pragma unroll
@@ -1016,7 +1025,7 @@ __global__ void __launch_bounds__(MmaCfg<DP, NR, TEAM, sizeof(T) == 4>::THREADS,
           if (cur.slot < 0) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             const int row = cur.row0 + r;
-            T *p = static_cast<T *>(a.out) + (cur.q0 + row / a.G) * a.out_ld + (1ll * cur.head * a.G + row % a.G) * D;
+            T *p = static_cast<T *>(a.out) + (cur.q0 + a.by_group.div(row)) * a.out_ld + (1ll * cur.head * a.G + a.by_group.mod(row)) * D;
             const bool vec = (reinterpret_cast<uintptr_t>(p) & (2 * sizeof(T) - 1)) == 0;
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
@@ -1054,9 +1063,9 @@ __global__ void __launch_bounds__(MmaCfg<DP, NR, TEAM, sizeof(T) == 4>::THREADS,
 }
 
 // ---- joining the pieces ---------------------------------------------------------------------------
-// One CTA per worker of the main kernel. The rows of an item with P pieces are dealt out to the CTAs of
-// the first P workers that have a piece of it, so that one long request is not joined by one CTA; a warp
-// joins a row, or all warps where the pieces are many. Time here is latency (note -> item -> maxima ->
+// The rows of an item with P pieces are dealt out to the first P workers that have a piece of it, so that
+// one long request is not joined in one place; a CTA stands for one worker of the main kernel or for four.
+// Time here is latency (note -> item -> maxima ->
 // rows), so every step loads all it needs at once. Launched so that it may become resident while the main
 // kernel drains; griddepcontrol.wait orders its reads after that kernel's writes.
 constexpr int JOIN_THREADS = 128, JOIN_WARPS = JOIN_THREADS / 32, JOIN_DIMS = 8; // dimensions per lane: D <= 256
@@ -1138,33 +1147,60 @@ __device__ __forceinline__ Joined join_pieces(const PagedArgs &a, const SplitIte
   return j;
 }
 
-template <typename T> __global__ void __launch_bounds__(JOIN_THREADS) attention_paged_join_kernel(PagedArgs a) {
+template <typename T>
+__global__ void __launch_bounds__(JOIN_THREADS) attention_paged_join_kernel(PagedArgs a, int workers, int per_cta) {
   __shared__ float red_o[JOIN_WARPS][32 * JOIN_DIMS];
   __shared__ float2 red_ml[JOIN_WARPS];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, me = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int2 note = a.notes[me];
+  auto out_row = [&](const SplitItem &it, int r) {
+    const int row = it.row0 + r;
+    return static_cast<T *>(a.out) + (it.q0 + a.by_group.div(row)) * a.out_ld + (1ll * it.head * a.G + a.by_group.mod(row)) * a.D;
+  };
+  constexpr int FEW = 16;
+  // Few pieces: a warp joins a row. With one worker to the CTA its warps share the rows, with four each has
+  // a worker of its own.
+  {
+    const int me = blockIdx.x * per_cta + (per_cta > 1 ? warp : 0), part = per_cta > 1 ? 0 : warp;
+    const int parts = per_cta > 1 ? 1 : JOIN_WARPS;
+    const int2 note = me < workers ? a.notes[me] : make_int2(0, -1);
+    bool many = false;
 #pragma unroll 1
-  for (int job = 0; job < 2; ++job) { // the item this worker began, the one its first segment continued
-    const int owner = job == 0 ? me : note.y;
-    if (job == 0 ? note.x == 0 : note.y < 0)
-      continue;
-    const SplitItem it = a.items[owner];
-    const int pieces = it.last - owner + 1, share = min(pieces, it.n_rows);
-    auto out_row = [&](int r) {
-      const int row = it.row0 + r;
-      return static_cast<T *>(a.out) + (it.q0 + row / a.G) * a.out_ld + (1ll * it.head * a.G + row % a.G) * a.D;
-    };
-    if (pieces <= 16) {
-      for (int r = me - owner + warp * share; r < it.n_rows; r += JOIN_WARPS * share) {
+    for (int job = 0; job < 2; ++job) { // the item this worker began, the one its first segment continued
+      const int owner = job == 0 ? me : note.y;
+      if (job == 0 ? note.x == 0 : note.y < 0)
+        continue;
+      const SplitItem it = a.items[owner];
+      const int pieces = it.last - owner + 1, share = min(pieces, it.n_rows);
+      if (pieces > FEW) {
+        many = true;
+        continue;
+      }
+      for (int r = me - owner + part * share; r < it.n_rows; r += parts * share) {
         const Joined j = join_pieces(a, it, owner, r, 0, 1, pieces);
-        T *out = out_row(r);
+        T *out = out_row(it, r);
 #pragma unroll
         for (int v = 0; v < JOIN_DIMS; ++v)
           if (const int d = join_dim(a.D, lane, v); d < a.D)
             store_out(out + d, j.sum == 0.f ? 0.f : j.o[v] / j.sum);
       }
-    } else {
+    }
+    if (!__syncthreads_or(many))
+      return;
+  }
+  // Many pieces: all warps join a row.
+#pragma unroll 1
+  for (int me = blockIdx.x * per_cta; me < min((static_cast<int>(blockIdx.x) + 1) * per_cta, workers); ++me) {
+    const int2 note = a.notes[me];
+#pragma unroll 1
+    for (int job = 0; job < 2; ++job) {
+      const int owner = job == 0 ? me : note.y;
+      if (job == 0 ? note.x == 0 : note.y < 0)
+        continue;
+      const SplitItem it = a.items[owner];
+      const int pieces = it.last - owner + 1, share = min(pieces, it.n_rows);
+      if (pieces <= FEW)
+        continue;
       for (int r = me - owner; r < it.n_rows; r += share) {
         const Joined j = join_pieces(a, it, owner, r, warp, JOIN_WARPS, pieces);
         if (lane == 0)
@@ -1184,7 +1220,7 @@ template <typename T> __global__ void __launch_bounds__(JOIN_THREADS) attention_
             const float f = rel_weight(red_ml[w].x, M);
             all += f * red_ml[w].y, x += f * red_o[w][d];
           }
-          store_out(out_row(r) + d, all == 0.f ? 0.f : x / all);
+          store_out(out_row(it, r) + d, all == 0.f ? 0.f : x / all);
         }
         __syncthreads();
       }
@@ -1204,14 +1240,15 @@ size_t paged_workspace_bytes(int num_sms, int D) {
   return rows * (sizeof(float) * D + sizeof(float2)) + (sizeof(SplitItem) + sizeof(int2)) * num_sms * MAX_WORKERS_PER_SM;
 }
 
-template <typename T> int launch_join(const PagedArgs &a, int workers, cudaStream_t st) {
+// per_cta: workers that a CTA of the join stands for, 1 or JOIN_WARPS
+template <typename T> int launch_join(const PagedArgs &a, int workers, int per_cta, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(workers), cfg.blockDim = dim3(JOIN_THREADS), cfg.stream = st;
+  cfg.gridDim = dim3((workers + per_cta - 1) / per_cta), cfg.blockDim = dim3(JOIN_THREADS), cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at, cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attention_paged_join_kernel<T>, a) == cudaSuccess ? 0 : 2;
+  return cudaLaunchKernelEx(&cfg, attention_paged_join_kernel<T>, a, workers, per_cta) == cudaSuccess ? 0 : 2;
 }
 
 template <typename T, int RT, int VB, int NA> int launch_simt(PagedArgs a, int num_sms, cudaStream_t st) {
@@ -1230,7 +1267,7 @@ template <typename T, int RT, int VB, int NA> int launch_simt(PagedArgs a, int n
   attention_paged_simt_kernel<T, RT, VB, NA><<<ctas, SIMT_THREADS, smem, st>>>(a);
   if (cudaGetLastError() != cudaSuccess)
     return 2;
-  return launch_join<T>(a, ctas, st);
+  return launch_join<T>(a, ctas, 1, st);
 }
 template <typename T, int VB, int NA> int launch_simt_rows(const PagedArgs &a, int num_sms, cudaStream_t st) {
   // rows that share a key: the group's heads for single tokens, up to 8 otherwise
@@ -1260,7 +1297,7 @@ template <typename T, int DP, int NR, int TEAM> int launch_mma_team(PagedArgs a,
   attention_paged_mma_kernel<T, DP, NR, TEAM><<<ctas, Cfg::THREADS, ring + 8ull * a.B, st>>>(a);
   if (cudaGetLastError() != cudaSuccess)
     return 2;
-  return launch_join<T>(a, ctas * Cfg::WARPS / TEAM, st);
+  return launch_join<T>(a, ctas * Cfg::WARPS / TEAM, TEAM == 1 ? JOIN_WARPS : 1, st);
 }
 template <typename T, int DP, int NR> int launch_mma(const PagedArgs &a, int num_sms, cudaStream_t st) {
   // Items (an upper bound) against warps: below an eighth every item would be cut into more than eight
@@ -1366,6 +1403,7 @@ int mu_attention_paged(mu_ctx *ctx, const void *q, long long q_ld, void *out, lo
   a.ks = k_scale, a.vs = v_scale, a.table = block_table, a.table_stride = table_stride;
   a.query_start = query_start, a.seq_lens = seq_lens, a.B = B, a.n_tokens = n_tokens;
   a.Hq = Hq, a.Hkv = Hkv, a.G = Hq / Hkv, a.D = D, a.num_pages = num_pages, a.page_size = page_size;
+  a.by_group = mu::FastDiv(a.G), a.by_page = mu::FastDiv(page_size);
   a.causal = causal != 0, a.status = mu_ctx_status_ptr(ctx);
   a.scale_log2 = static_cast<float>(1.4426950408889634 / sqrt(static_cast<double>(D)));
   if (mu::launch_attention_paged(a, workspace, dtype, mu_ctx_num_sms(ctx), static_cast<cudaStream_t>(stream)))
