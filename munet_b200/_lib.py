@@ -149,18 +149,35 @@ def lib() -> C.CDLL:
 
 
 def _ptr(t):
-    if t is None:
-        return None
+    if t is None or type(t) is int:
+        return t
     if isinstance(t, int):
         return t
     return t.data_ptr()
 
 
+def _current_stream_of():
+    """The current stream's handle, by torch's direct lookup where it has one: making a Stream object costs more
+    than the rest of a small call."""
+    import torch
+    try:
+        raw, device = torch._C._cuda_getCurrentRawStream, torch.cuda.current_device
+        raw(device())
+        return lambda: raw(device())
+    except AttributeError:
+        return lambda: torch.cuda.current_stream().cuda_stream
+
+
+_current = None
+
+
 def _stream(stream):
+    global _current
     if stream is None:
         try:
-            import torch
-            return torch.cuda.current_stream().cuda_stream
+            if _current is None:
+                _current = _current_stream_of()
+            return _current()
         except Exception:
             return None
     if isinstance(stream, int):

@@ -109,4 +109,21 @@ struct PerDeviceOnce {
   }
 };
 
+// Division by a number known at launch: n / d for n < 2^31 (mul = ceil(2^(31 + shift) / d), 2^shift >= d).
+struct FastDiv {
+  unsigned d, mul, shift;
+  FastDiv() = default;
+  explicit FastDiv(int by) : d(by), shift(0) {
+    while ((1ull << shift) < d)
+      ++shift;
+    mul = static_cast<unsigned>(((1ull << (31 + shift)) + d - 1) / d);
+  }
+#ifdef __CUDACC__
+  __device__ __forceinline__ int div(int n) const { // mul has 32 bits: 2^31 <= mul <= 2^32 - 1 for d > 1
+    return d == 1 ? n : static_cast<int>(__umulhi(static_cast<unsigned>(n) << 1, mul) >> shift);
+  }
+  __device__ __forceinline__ int mod(int n) const { return n - div(n) * static_cast<int>(d); }
+#endif
+};
+
 } // namespace mu

@@ -188,15 +188,17 @@ int launch_page_map(const PageMapArgs &a, int num_sms, cudaStream_t st) {
 }
 
 // ---- write into the cache -----------------------------------------------------------------------
-// Work unit: the run of consecutive new tokens that fall into one page, for one head of K or V. Its
-// CTA finds the run's largest magnitude, derives the page's scale, requantises what the page held
-// before if the scale grew, and stores the new rows. The rows stay in registers between the two
-// steps (64 elements per thread: a page of 64 x 128), so HBM sees them once.
+// Work unit: the run of consecutive new tokens that fall into one page, for one head of K or V. A team of
+// threads finds the run's largest magnitude, derives the page's scale, requantises what the page held
+// before if the scale grew, and stores the new rows. The rows stay in registers, as they came, between
+// the two steps (64 elements per thread: a page of 64 x 128 for a team of 128), so HBM sees them once.
+// Teams: a CTA where the tokens are many (prompts: one run per page); a warp, four heads to the CTA, where
+// they are few (a decode step: every token is a run of its own, and a CTA would idle over 128 elements).
 //
 // Scale: the smallest power of two s >= 2^-64 with amax <= 448 s. e4m3 keeps its three mantissa bits
 // at every magnitude, so a power of two loses nothing against amax/448 except range at the bottom,
 // and growing it later is exact for everything above the subnormals.
-constexpr int AP_THREADS = 128;
+constexpr int AP_THREADS = 128, AP_WARPS = AP_THREADS / 32;
 constexpr int AP_REGS = 8;       // vectors of 8 elements a thread keeps
 constexpr int AP_MAX_BLOCK = 64; // most tokens one CTA looks at for run starts
 
@@ -208,25 +210,39 @@ struct AppendArgs {
   uint8_t *cache[2];
   float *scale[2];
   int num_pages, page_size, H, D;
+  FastDiv by_page;
   int block_tokens; // tokens per CTA
   unsigned dv, dv_magic; // vectors per row and ceil(2^32 / dv)
   int *status;
 };
 
-template <typename T, int VE> __device__ __forceinline__ void load_row_vec(const T *p, float (&f)[VE]) {
-  if constexpr (VE == 8 && sizeof(T) == 2) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p));
-    f[0] = bf16_lo(u.x), f[1] = bf16_hi(u.x), f[2] = bf16_lo(u.y), f[3] = bf16_hi(u.y);
-    f[4] = bf16_lo(u.z), f[5] = bf16_hi(u.z), f[6] = bf16_lo(u.w), f[7] = bf16_hi(u.w);
-  } else if constexpr (VE == 8) {
-    const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-  } else {
+// VE elements of a row as they are in memory: 8 (one or two 16-byte loads) or 1
+template <typename T, int VE> struct RowVec {
+  static constexpr int WORDS = VE == 8 ? 8 * sizeof(T) / 4 : 1;
+  uint32_t w[WORDS];
+  __device__ __forceinline__ void load(const T *p) {
+    if constexpr (VE == 8) {
 #pragma unroll
-    for (int i = 0; i < VE; ++i)
-      f[i] = static_cast<float>(p[i]);
+      for (int i = 0; i < WORDS / 4; ++i) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+        w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+      }
+    } else {
+      w[0] = __float_as_uint(static_cast<float>(*p));
+    }
   }
-}
+  __device__ __forceinline__ void floats(float (&f)[VE]) const {
+    if constexpr (VE == 8 && sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        f[2 * i] = bf16_lo(w[i]), f[2 * i + 1] = bf16_hi(w[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VE; ++i)
+        f[i] = __uint_as_float(w[i]);
+    }
+  }
+};
 // largest finite magnitude, as bits (ordered like the values)
 template <int VE> __device__ __forceinline__ uint32_t amax_bits(const float (&f)[VE], uint32_t m) {
 #pragma unroll
@@ -251,9 +267,14 @@ __device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t two) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3);
   return __half22float2(static_cast<__half2>(h));
 }
-// One rounding, from 64 bits: for scales that are no power of two (a cache that someone else filled).
-__device__ __forceinline__ uint32_t e4m3_of_double(double v) {
-  return __nv_cvt_double_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+// One rounding, from 64 bits: for scales that are no power of two (a cache that someone else filled). The
+// value is rounded to e4m3's grid (three bits below its leading one, 2^-9 at least) in double; what comes out
+// is exact in float and in the conversion.
+__device__ __forceinline__ float on_e4m3_grid(double v) {
+  if (!(fabs(v) < 1e6))
+    return static_cast<float>(v); // saturates, or is NaN
+  const int e = max(((__double2hiint(v) >> 20) & 0x7ff) - 1023, -6) - 3;
+  return static_cast<float>(rint(v * __hiloint2double((1023 - e) << 20, 0)) * __hiloint2double((1023 + e) << 20, 0));
 }
 // Rows leave as v / s. A power of two's reciprocal is exact, so the product rounds once, in the
 // conversion; any other scale is divided by in 64 bits, or the quotient would be rounded twice.
@@ -267,7 +288,7 @@ struct Divisor {
   __device__ __forceinline__ uint32_t code2(float a, float b) const {
     if (pow2)
       return e4m3x2(a * inv, b * inv);
-    return e4m3_of_double(static_cast<double>(a) / s) | (e4m3_of_double(static_cast<double>(b) / s) << 8);
+    return e4m3x2(on_e4m3_grid(static_cast<double>(a) / s), on_e4m3_grid(static_cast<double>(b) / s));
   }
 };
 template <int VE>
@@ -296,8 +317,8 @@ __device__ __forceinline__ int next_bit(const uint32_t *bits, int from, int n) {
   return n;
 }
 
-template <typename T, int VE>
-__global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(AppendArgs a) {
+template <typename T, int VE, int TEAM>
+__global__ void __launch_bounds__(AP_THREADS, VE == 8 ? (sizeof(T) == 2 ? 8 : 5) : 4) kv_append_kernel(AppendArgs a) {
   // window of slots: the CTA's tokens and as many as one page holds after them
   extern __shared__ int sm[];
   const int win = min(a.block_tokens + a.page_size, a.n_tokens - static_cast<int>(blockIdx.x) * a.block_tokens);
@@ -305,32 +326,44 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(AppendArgs a) {
   int *slot = sm;                                                             // [win]
   uint32_t *starts = reinterpret_cast<uint32_t *>(sm + a.block_tokens + a.page_size); // token begins a run (or none)
   uint32_t *disorder = starts + words;                                        // token continues a run at a lower offset
-  __shared__ uint32_t red[AP_THREADS / 32];
-  const int tid = threadIdx.x, t0 = blockIdx.x * a.block_tokens;
-  const int which = blockIdx.y & 1, h = blockIdx.y >> 1;
-  const unsigned ps = a.page_size;
-  const unsigned n_slots = static_cast<unsigned>(a.num_pages) * ps;
-  for (int i = tid; i < words * 32; i += AP_THREADS) { // whole warps: the ballots need every lane
+  __shared__ uint32_t red[AP_WARPS];
+  const int t0 = blockIdx.x * a.block_tokens;
+  const int ps = a.page_size, n_slots = a.num_pages * ps; // a slot fits 31 bits
+  for (int i = threadIdx.x; i < words * 32; i += AP_THREADS) { // whole warps: the ballots need every lane
     int s = -1, before = -1;
     if (i < win) {
       s = a.slots[t0 + i];
       before = t0 + i > 0 ? a.slots[t0 + i - 1] : -1;
-      if (s >= 0 && static_cast<unsigned>(s) >= n_slots) {
+      if (s >= n_slots) {
         if (blockIdx.y == 0)
           atomicCAS(a.status, 0, MU_DEV_BAD_PAGE);
         s = -1;
       }
-      if (before >= 0 && static_cast<unsigned>(before) >= n_slots)
+      if (s < -1 && blockIdx.y == 0)
+        atomicCAS(a.status, 0, MU_DEV_BAD_PAGE);
+      if (before >= n_slots)
         before = -1;
       slot[i] = s;
     }
-    const bool same = s >= 0 && before >= 0 && static_cast<unsigned>(s) / ps == static_cast<unsigned>(before) / ps;
+    const bool same = s >= 0 && before >= 0 && a.by_page.div(s) == a.by_page.div(before);
     const uint32_t st = __ballot_sync(~0u, !same), di = __ballot_sync(~0u, same && s <= before);
-    if ((tid & 31) == 0)
+    if ((threadIdx.x & 31) == 0)
       starts[i >> 5] = st, disorder[i >> 5] = di;
   }
   __syncthreads();
 
+  // this team's head of K or V
+  const int tid = TEAM == AP_THREADS ? threadIdx.x : threadIdx.x & 31;
+  const int unit = TEAM == AP_THREADS ? blockIdx.y : blockIdx.y * AP_WARPS + (threadIdx.x >> 5);
+  if (unit >= 2 * a.H)
+    return; // only whole warps of a CTA that meets no more at a barrier
+  const int which = unit & 1, h = unit >> 1;
+  auto team_sync = [] {
+    if constexpr (TEAM == AP_THREADS)
+      __syncthreads();
+    else
+      __syncwarp();
+  };
   const T *x = static_cast<const T *>(a.x[which]) + 1ll * h * a.D;
   // row of vector v: exact for v < 2^18, dv <= 2^8
   auto row_of = [&](unsigned v) { return a.dv == 1 ? v : __umulhi(v, a.dv_magic); };
@@ -339,18 +372,18 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(AppendArgs a) {
     if (slot[i] < 0)
       continue;
     int n = next_bit(starts, i + 1, win) - i;
-    const unsigned page = static_cast<unsigned>(slot[i]) / ps;
+    const int page = a.by_page.div(slot[i]), page0 = page * ps;
     // A run in ascending order ends within the window. One that is out of order, or repeats a slot,
     // takes the slow walk below, token by token, so that the last write of a slot is the one that stays.
-    const bool ordered = next_bit(disorder, i + 1, i + n) >= i + n && n <= a.page_size;
-    int low = static_cast<int>(slot[i] - page * ps);
+    const bool ordered = next_bit(disorder, i + 1, i + n) >= i + n && n <= ps;
+    int low = slot[i] - page0;
     if (!ordered) {
       int j = i + 1;
       for (; t0 + j < a.n_tokens; ++j) {
         const int s = a.slots[t0 + j];
-        if (s < 0 || static_cast<unsigned>(s) >= n_slots || static_cast<unsigned>(s) / ps != page)
+        if (s < 0 || s >= n_slots || a.by_page.div(s) != page)
           break;
-        low = min(low, static_cast<int>(s - page * ps));
+        low = min(low, s - page0);
       }
       n = j - i;
     }
@@ -360,29 +393,39 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(AppendArgs a) {
     const T *rows = x + (1ll * t0 + i) * a.ld;
     const long long total = 1ll * n * a.dv;
 
-    float keep[AP_REGS][VE];
+    RowVec<T, VE> keep[AP_REGS];
     uint32_t m = 0;
 #pragma unroll
     for (int k = 0; k < AP_REGS; ++k) {
-      const unsigned v = tid + k * AP_THREADS;
+      const unsigned v = tid + k * TEAM;
       if (v < total) {
         const unsigned row = row_of(v);
-        load_row_vec<T, VE>(rows + row * a.ld + (v - row * a.dv) * VE, keep[k]);
-        m = amax_bits<VE>(keep[k], m);
+        keep[k].load(rows + row * a.ld + (v - row * a.dv) * VE);
       }
     }
-    for (long long v = tid + AP_REGS * AP_THREADS; v < total; v += AP_THREADS) {
+#pragma unroll
+    for (int k = 0; k < AP_REGS; ++k)
+      if (tid + k * TEAM < total) {
+        float f[VE];
+        keep[k].floats(f);
+        m = amax_bits<VE>(f, m);
+      }
+    for (long long v = tid + AP_REGS * TEAM; v < total; v += TEAM) {
+      RowVec<T, VE> r;
       float f[VE];
-      load_row_vec<T, VE>(rows + (v / a.dv) * a.ld + (v % a.dv) * VE, f);
+      r.load(rows + (v / a.dv) * a.ld + (v % a.dv) * VE);
+      r.floats(f);
       m = amax_bits<VE>(f, m);
     }
     m = __reduce_max_sync(~0u, m);
-    if ((tid & 31) == 0)
-      red[tid >> 5] = m;
-    __syncthreads();
+    if constexpr (TEAM == AP_THREADS) {
+      if ((tid & 31) == 0)
+        red[tid >> 5] = m;
+      __syncthreads();
 #pragma unroll
-    for (int w = 0; w < AP_THREADS / 32; ++w)
-      m = max(m, red[w]);
+      for (int w = 0; w < AP_WARPS; ++w)
+        m = max(m, red[w]);
+    }
     const float now = fmaxf(held, page_scale(m));
     if (tid == 0)
       *scale = now;
@@ -395,44 +438,64 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(AppendArgs a) {
       const int bytes = low * a.D;
       auto again = [&](uint32_t two) -> uint32_t {
         const float2 p = e4m3x2_to_float2(two);
-        return pow2 ? e4m3x2(p.x * ff, p.y * ff) : e4m3_of_double(p.x * f) | (e4m3_of_double(p.y * f) << 8);
+        return pow2 ? e4m3x2(p.x * ff, p.y * ff) : e4m3x2(on_e4m3_grid(p.x * f), on_e4m3_grid(p.y * f));
       };
       uint32_t *w = reinterpret_cast<uint32_t *>(tile);
-      for (int k = tid; k < bytes / 4; k += AP_THREADS) {
+      for (int k = tid; k < bytes / 4; k += TEAM) {
         const uint32_t u = w[k];
         w[k] = again(u & 0xffffu) | (again(u >> 16) << 16);
       }
-      for (int k = (bytes & ~3) + tid; k < bytes; k += AP_THREADS)
+      for (int k = (bytes & ~3) + tid; k < bytes; k += TEAM)
         tile[k] = static_cast<uint8_t>(again(tile[k]) & 0xffu);
     }
     const Divisor div(now);
     if (ordered) {
 #pragma unroll
       for (int k = 0; k < AP_REGS; ++k) {
-        const unsigned v = tid + k * AP_THREADS;
+        const unsigned v = tid + k * TEAM;
         if (v < total) {
           const unsigned row = row_of(v);
-          store_row_vec<VE>(tile + (slot[i + row] - page * ps) * a.D + (v - row * a.dv) * VE, keep[k], div);
+          float f[VE];
+          keep[k].floats(f);
+          store_row_vec<VE>(tile + (slot[i + row] - page0) * a.D + (v - row * a.dv) * VE, f, div);
         }
       }
-      for (unsigned v = tid + AP_REGS * AP_THREADS; v < total; v += AP_THREADS) {
+      for (unsigned v = tid + AP_REGS * TEAM; v < total; v += TEAM) {
         const unsigned row = row_of(v);
+        RowVec<T, VE> r;
         float f[VE];
-        load_row_vec<T, VE>(rows + row * a.ld + (v - row * a.dv) * VE, f);
-        store_row_vec<VE>(tile + (slot[i + row] - page * ps) * a.D + (v - row * a.dv) * VE, f, div);
+        r.load(rows + row * a.ld + (v - row * a.dv) * VE);
+        r.floats(f);
+        store_row_vec<VE>(tile + (slot[i + row] - page0) * a.D + (v - row * a.dv) * VE, f, div);
       }
     } else {
       for (int j = 0; j < n; ++j) {
-        __syncthreads(); // the requantised bytes and the token before are in place
-        const unsigned s = a.slots[t0 + i + j];
-        for (unsigned v = tid; v < a.dv; v += AP_THREADS) {
+        team_sync(); // the requantised bytes and the token before are in place
+        const int s = a.slots[t0 + i + j];
+        for (unsigned v = tid; v < a.dv; v += TEAM) {
+          RowVec<T, VE> r;
           float f[VE];
-          load_row_vec<T, VE>(rows + j * a.ld + v * VE, f);
-          store_row_vec<VE>(tile + (s - page * ps) * a.D + v * VE, f, div);
+          r.load(rows + j * a.ld + v * VE);
+          r.floats(f);
+          store_row_vec<VE>(tile + (s - page0) * a.D + v * VE, f, div);
         }
       }
     }
-    __syncthreads(); // red[] is free again
+    team_sync(); // red[] is free again
+  }
+}
+
+template <typename T> void launch_append_t(const AppendArgs &a, bool vec, int team, dim3 grid, size_t smem, cudaStream_t st) {
+  if (team == 32) {
+    if (vec)
+      kv_append_kernel<T, 8, 32><<<grid, AP_THREADS, smem, st>>>(a);
+    else
+      kv_append_kernel<T, 1, 32><<<grid, AP_THREADS, smem, st>>>(a);
+  } else {
+    if (vec)
+      kv_append_kernel<T, 8, AP_THREADS><<<grid, AP_THREADS, smem, st>>>(a);
+    else
+      kv_append_kernel<T, 1, AP_THREADS><<<grid, AP_THREADS, smem, st>>>(a);
   }
 }
 
@@ -446,10 +509,11 @@ int launch_kv_append(AppendArgs a, int dtype, int num_sms, cudaStream_t st) {
     vec = vec && (reinterpret_cast<uintptr_t>(a.x[i]) & 15u) == 0;
   a.dv = vec ? a.D / 8 : a.D;
   a.dv_magic = static_cast<unsigned>((0x100000000ull + a.dv - 1) / a.dv); // unused where dv is 1
-  // Tokens per CTA: one where the calls are few (a decode step: every token starts a run), more where
-  // that would only launch CTAs that find no start (prompts: one start per page).
-  const long long ctas = 2ll * a.H * a.n_tokens;
-  long long tb = ctas / (num_sms * 64ll);
+  // Few tokens: one per CTA and a warp for each of four heads. Many: up to a page of tokens per CTA, whose
+  // threads all work on one head; with one token per CTA most would find that no run begins there.
+  const long long units = 2ll * a.H * a.n_tokens;
+  const int team = units <= num_sms * 64ll ? 32 : AP_THREADS;
+  long long tb = team == 32 ? 1 : units / (num_sms * 64ll);
   if (tb > AP_MAX_BLOCK)
     tb = AP_MAX_BLOCK;
   if (tb > a.page_size)
@@ -459,18 +523,12 @@ int launch_kv_append(AppendArgs a, int dtype, int num_sms, cudaStream_t st) {
   a.block_tokens = static_cast<int>(tb);
   const int span = a.block_tokens + a.page_size, words = (span + 31) / 32;
   const size_t smem = sizeof(int) * (span + 2ull * words);
-  const dim3 grid(static_cast<unsigned>((a.n_tokens + tb - 1) / tb), static_cast<unsigned>(2 * a.H));
-  if (dtype == F32) {
-    if (vec)
-      kv_append_kernel<float, 8><<<grid, AP_THREADS, smem, st>>>(a);
-    else
-      kv_append_kernel<float, 1><<<grid, AP_THREADS, smem, st>>>(a);
-  } else {
-    if (vec)
-      kv_append_kernel<__nv_bfloat16, 8><<<grid, AP_THREADS, smem, st>>>(a);
-    else
-      kv_append_kernel<__nv_bfloat16, 1><<<grid, AP_THREADS, smem, st>>>(a);
-  }
+  const int heads = team == 32 ? (2 * a.H + AP_WARPS - 1) / AP_WARPS : 2 * a.H;
+  const dim3 grid(static_cast<unsigned>((a.n_tokens + tb - 1) / tb), static_cast<unsigned>(heads));
+  if (dtype == F32)
+    launch_append_t<float>(a, vec, team, grid, smem, st);
+  else
+    launch_append_t<__nv_bfloat16>(a, vec, team, grid, smem, st);
   return cudaGetLastError() == cudaSuccess ? 0 : 2;
 }
 
@@ -538,6 +596,7 @@ int mu_kv_cache_append(mu_ctx *ctx, const void *k, const void *v, long long ld, 
   a.cache[0] = static_cast<uint8_t *>(k_cache), a.cache[1] = static_cast<uint8_t *>(v_cache);
   a.scale[0] = k_scale, a.scale[1] = v_scale;
   a.num_pages = num_pages, a.page_size = page_size, a.H = Hkv, a.D = D, a.status = mu_ctx_status_ptr(ctx);
+  a.by_page = mu::FastDiv(page_size);
   if (mu::launch_kv_append(a, dtype, mu_ctx_num_sms(ctx), static_cast<cudaStream_t>(stream)))
     return mu_set_error(ctx, MU_ERR_CUDA, cudaGetErrorString(cudaGetLastError()));
   return MU_OK;

@@ -11,6 +11,12 @@
 //
 // One cluster of 1, 2, 4 or 8 CTAs per row; each CTA keeps its slab of the row in shared memory as
 // order-preserving 32-bit keys, so HBM sees a row once and every later pass runs on chip.
+//
+// Where a cut falls is found in two steps: a histogram over 4096 buckets of the logits (1/64 of a factor
+// of two wide, from the maximum down: a monotone function, so buckets are ranges of the order) says in
+// which bucket, and that bucket's few elements are sorted. With top-k everything down to the cut goes into
+// the list, which then settles top-p, min-p and the draw as well. Rows whose bucket holds more than a list
+// (ties, logits of another scale) are cut eight bits of the key at a time.
 #include "../../include/munet_b200.h"
 #include "common.h"
 #include "ptx.cuh"
@@ -22,7 +28,9 @@ namespace cg = cooperative_groups;
 namespace mu {
 
 constexpr int SP_THREADS = 1024, SP_WARPS = SP_THREADS / 32, SP_MAX_CLUSTER = 8;
-constexpr int SP_SMEM_KEYS = 49152; // keys of one CTA that fit its shared memory (192 KB)
+constexpr int SP_BUCKETS = 4096, SP_LIST = 1024;
+constexpr float SP_BUCKETS_PER_NAT = 92.3325f; // 64 to a factor of two
+constexpr int SP_SMEM_KEYS = 43008; // keys of one CTA that fit its shared memory beside the buckets (168 KB)
 constexpr double SP_ONE = 4398046511104.0; // 2^42: the weight of the row's maximum
 
 struct SampleArgs {
@@ -65,6 +73,13 @@ struct SampleShared {
   u64 found_above;
   uint32_t found_digit, found_count;
   int found_index;
+  double table[32];   // 2^(i/32)
+  u64 list[SP_LIST];  // (key, ~index), rank 0's
+  int n_list;
+  int bucket;         // that the cut falls into
+  u64 above, within;  // measure before it, and of it
+  uint32_t bound_key; // broadcast by rank 0
+  int bound_idx;
 };
 
 // Inclusive scan of v over the CTA's threads; returns this thread's, and the CTA's total in `all`.
@@ -92,8 +107,12 @@ __device__ __forceinline__ u64 block_scan(u64 v, SampleShared &sh, u64 &all) {
   return v + (warp ? before : 0);
 }
 
+// exp((x - max) / T) = 2^t, t = i/32 + f: the table's 2^(i/32) times the Taylor polynomial of 2^f up to f^5,
+// |f| <= 1/64: the remainder is below (ln2/64)^6 / 720 = 2.3e-15, a sixteenth of the 2^-43 that rounding to
+// whole multiples of 2^-42 allows for weights near one. exp() cost twice as much.
 struct Row {
-  double xmax, inv_t;
+  double c, minus; // t = x * c + minus
+  const double *table;
   uint32_t max_key;
   bool spike; // the maximum is +inf: only elements equal to it weigh anything
   __device__ __forceinline__ double weight(uint32_t key) const {
@@ -101,13 +120,46 @@ struct Row {
       return 1.0;
     if (spike || key <= KEY_NEG_INF)
       return 0.0;
-    return exp((static_cast<double>(from_key(key)) - xmax) * inv_t);
+    const double t = fma(static_cast<double>(from_key(key)), c, minus);
+    if (!(t > -64.0)) // counts as zero (2^-43 and below)
+      return 0.0;
+    const double shift = 0x1.8p52 / 32; // adding it rounds t to a multiple of 1/32
+    const double r = t + shift;
+    const int i = __double2loint(r);
+    const double f = t - (r - shift);
+    double p = fma(f, 0x1.5d87fe78a6731p-10, 0x1.3b2ab6fba4e77p-7); // ln2^k / k!
+    p = fma(f, p, 0x1.c6b08d704a0c0p-5);
+    p = fma(f, p, 0x1.ebfbdff82c58fp-3);
+    p = fma(f, p, 0x1.62e42fefa39efp-1);
+    p = fma(f, p, 1.0) * table[i & 31];
+    return __hiloint2double(__double2hiint(p) + ((i >> 5) << 20), __double2loint(p));
   }
-  __device__ __forceinline__ u64 fixed(uint32_t key) const { return __double2ull_rn(weight(key) * SP_ONE); }
+  // rounded to a multiple of 2^-42, as that multiple
+  __device__ __forceinline__ static u64 whole(double w) {
+    return static_cast<u64>(__double_as_longlong(fma(w, SP_ONE, 0x1p52))) & 0xfffffffffffffull;
+  }
+  __device__ __forceinline__ u64 fixed(uint32_t key) const { return whole(weight(key)); }
 };
 
+// Sorts v[0 .. n) (n a power of two up to SP_THREADS) in descending order.
+__device__ __forceinline__ void sort_desc(u64 *v, int n) {
+  const int i = threadIdx.x;
+  for (int k = 2; k <= n; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      __syncthreads();
+      const int o = i ^ j;
+      if (i < n && o > i) {
+        const u64 x = v[i], y = v[o];
+        if ((x < y) == ((i & k) == 0))
+          v[i] = y, v[o] = x;
+      }
+    }
+  __syncthreads();
+}
+
 template <typename T> __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a) {
-  extern __shared__ uint32_t keys[];
+  extern __shared__ __align__(16) uint32_t buckets[]; // [2][SP_BUCKETS], then the keys
+  uint32_t *const keys = buckets + 2 * SP_BUCKETS;
   __shared__ SampleShared sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), rank = cluster.block_rank();
@@ -119,6 +171,13 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS) sample_kerne
 #pragma unroll
     for (int b = 0; b < 2; ++b)
       sh.cnt[b][i] = sh.lo[b][i] = sh.hi[b][i] = 0;
+
+  for (int i = tid; i < 2 * SP_BUCKETS / 4; i += SP_THREADS)
+    reinterpret_cast<uint4 *>(buckets)[i] = make_uint4(0, 0, 0, 0);
+  if (tid < 32)
+    sh.table[tid] = exp2(tid / 32.0);
+  if (tid == 0)
+    sh.n_list = 0;
 
   uint32_t top = 0;
   for (int i = tid; i < n; i += SP_THREADS) {
@@ -187,7 +246,9 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS) sample_kerne
   } else {
     Row rw;
     rw.max_key = top, rw.spike = top == KEY_POS_INF;
-    rw.xmax = from_key(top), rw.inv_t = 1.0 / static_cast<double>(T_row);
+    const float xmax = from_key(top);
+    rw.table = sh.table;
+    rw.c = 1.4426950408889634 / static_cast<double>(T_row), rw.minus = -static_cast<double>(xmax) * rw.c;
     // kept: key > bound_key, or equal to it at an index up to bound_idx
     uint32_t bound_key = 0;
     int bound_idx = INT_MAX;
@@ -274,7 +335,7 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS) sample_kerne
         if (kept(k, i)) {
           const double w = rw.weight(k);
           if (w >= floor_w)
-            mine += __double2ull_rn(w * SP_ONE);
+            mine += Row::whole(w);
         }
       }
       before = block_scan(mine, sh, all) - mine;
@@ -293,22 +354,162 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS) sample_kerne
     };
 
     const int k = a.top_k ? a.top_k[row] : 0;
-    if (k > 0 && k < a.cols)
-      cut(k, false);
-    u64 mine, before;
     const float p = a.top_p ? a.top_p[row] : 1.f;
-    if (p < 1.f) {
-      const u64 all = weight_of_kept(0.0, mine, before);
-      const double target = ceil(static_cast<double>(p) * static_cast<double>(all));
-      cut(target >= 1.0 ? static_cast<u64>(target) : 1ull, true);
-    }
-    const float mp = a.min_p ? a.min_p[row] : 0.f;
-    const u64 all = weight_of_kept(mp > 0.f ? fmin(static_cast<double>(mp), 1.0) : 0.0, mine, before);
+    const bool by_count = k > 0 && k < a.cols;
+    const float per_unit = by_count ? SP_BUCKETS_PER_NAT : SP_BUCKETS_PER_NAT / T_row;
+    auto bucket_of = [&](uint32_t key) { return min(SP_BUCKETS - 1, static_cast<int>((xmax - from_key(key)) * per_unit)); };
+    // Fills the buckets and finds the one in which the measure (elements, or weight) reaches the target,
+    // which `target_of` gives from the row's total.
+    auto find_bucket = [&](bool weight, auto target_of) {
+      for (int i = tid; i < n; i += SP_THREADS) {
+        const uint32_t key = key_at(i);
+        const int b = bucket_of(key);
+        if (!weight) {
+          atomicAdd(&buckets[b], 1u);
+          continue;
+        }
+        const u64 w = rw.fixed(key);
+        if (w == 0)
+          continue;
+        const uint32_t wl = static_cast<uint32_t>(w), old = atomicAdd(&buckets[b], wl);
+        const uint32_t wh = static_cast<uint32_t>(w >> 32) + (old + wl < old ? 1u : 0u);
+        if (wh)
+          atomicAdd(&buckets[SP_BUCKETS + b], wh);
+      }
+      cluster.sync();
+      u64 v[4] = {0, 0, 0, 0}, all;
+      for (int r = 0; r < C; ++r) {
+        const uint32_t *from = cluster.map_shared_rank(buckets, r) + 4 * tid;
+        const uint4 lo = *reinterpret_cast<const uint4 *>(from);
+        v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
+        if (weight) {
+          const uint4 hi = *reinterpret_cast<const uint4 *>(from + SP_BUCKETS);
+          v[0] += static_cast<u64>(hi.x) << 32, v[1] += static_cast<u64>(hi.y) << 32;
+          v[2] += static_cast<u64>(hi.z) << 32, v[3] += static_cast<u64>(hi.w) << 32;
+        }
+      }
+      const u64 sum = v[0] + v[1] + v[2] + v[3];
+      u64 at = block_scan(sum, sh, all) - sum;
+      const u64 target = target_of(all);
+      if (at < target && at + sum >= target) {
+        int j = 0;
+        while (at + v[j] < target)
+          at += v[j++];
+        sh.bucket = 4 * tid + j, sh.above = at, sh.within = v[j];
+      }
+      __syncthreads();
+      return target;
+    };
+    // Puts the elements whose bucket passes into rank 0's list; their number over the row.
+    auto gather = [&](auto passes) {
+      int *const count = cluster.map_shared_rank(&sh.n_list, 0);
+      u64 *const list = cluster.map_shared_rank(sh.list, 0);
+      for (int i = tid; i < n; i += SP_THREADS) {
+        const uint32_t key = key_at(i);
+        if (passes(bucket_of(key))) {
+          const int at = atomicAdd(count, 1);
+          if (at < SP_LIST)
+            list[at] = static_cast<u64>(key) << 32 | static_cast<uint32_t>(~(s0 + i));
+        }
+      }
+      cluster.sync();
+      return *count;
+    };
+    // rank 0: the list in descending order (largest key, then lowest index), one element to a thread
+    auto sorted = [&](int count) {
+      int m = 1;
+      while (m < count)
+        m <<= 1;
+      if (tid >= count && tid < m)
+        sh.list[tid] = 0;
+      sort_desc(sh.list, m);
+      return tid < count ? sh.list[tid] : 0ull;
+    };
+    const float mp = a.min_p && a.min_p[row] > 0.f ? fminf(a.min_p[row], 1.f) : 0.f;
     const float u = a.u[row];
-    double at = u > 0.f ? static_cast<double>(u) * static_cast<double>(all) : 0.0;
-    const u64 want = at >= static_cast<double>(all) ? all - 1 : static_cast<u64>(at);
+    auto draw = [&](u64 all) { // the whole weight that lies before the drawn token's end
+      const double at = u > 0.f ? static_cast<double>(u) * static_cast<double>(all) : 0.0;
+      return at >= static_cast<double>(all) ? all - 1 : static_cast<u64>(at);
+    };
+    auto share_of = [&](u64 all) { // top_p of a sum, rounded up
+      const double t = ceil(static_cast<double>(p) * static_cast<double>(all));
+      return t >= 1.0 ? static_cast<u64>(t) : 1ull;
+    };
+
+    if (by_count) {
+      find_bucket(false, [&](u64) { return static_cast<u64>(k); });
+      const int last = sh.bucket;
+      // elements down to the cut's bucket: the list has room, or nobody gathers
+      const int count = sh.above + sh.within <= SP_LIST ? gather([&](int b) { return b <= last; }) : SP_LIST + 1;
+      if (count <= SP_LIST) {
+        if (rank == 0) {
+          const u64 e = sorted(count);
+          const uint32_t key = static_cast<uint32_t>(e >> 32);
+          const double w = rw.weight(key);
+          bool in = tid < min(k, count);
+          u64 all;
+          if (p < 1.f) {
+            const u64 mine = in ? Row::whole(w) : 0, before = block_scan(mine, sh, all) - mine;
+            in = in && before < share_of(all);
+          }
+          in = in && (!(mp > 0.f) || w >= mp);
+          // in index order: sort by ~index, descending; the position rides along
+          __syncthreads();
+          int m = 1;
+          while (m < count)
+            m <<= 1;
+          if (tid < m)
+            sh.list[tid] = in ? (e << 32) | key : 0ull;
+          sort_desc(sh.list, m);
+          const u64 f = tid < m ? sh.list[tid] : 0ull;
+          const uint32_t fk = static_cast<uint32_t>(f);
+          const double fw = f ? rw.weight(fk) : 0.0;
+          const u64 mine = f ? Row::whole(fw) : 0, upto = block_scan(mine, sh, all);
+          const u64 want = draw(all);
+          if (upto - mine <= want && want < upto) {
+            a.idx[row] = static_cast<int>(~static_cast<uint32_t>(f >> 32));
+            if (a.prob)
+              a.prob[row] = static_cast<float>(fw * SP_ONE / static_cast<double>(all));
+          }
+        }
+        cluster.sync();
+        return;
+      }
+      cut(k, false);
+    }
+    u64 mine, before;
+    if (p < 1.f) {
+      bool done = false;
+      if (!by_count) {
+        const u64 target = find_bucket(true, share_of);
+        const int last = sh.bucket;
+        const u64 above = sh.above;
+        const int count = gather([&](int b) { return b == last; });
+        if (count <= SP_LIST) {
+          done = true;
+          if (rank == 0) {
+            const u64 e = sorted(count);
+            const u64 w = tid < count ? rw.fixed(static_cast<uint32_t>(e >> 32)) : 0;
+            u64 all;
+            const u64 ahead = above + block_scan(w, sh, all) - w;
+            // the last of those before which less than the target lies
+            if (tid < count && ahead < target && (ahead + w >= target || tid == count - 1))
+              for (int r = 0; r < C; ++r) {
+                *cluster.map_shared_rank(&sh.bound_key, r) = static_cast<uint32_t>(e >> 32);
+                *cluster.map_shared_rank(&sh.bound_idx, r) = static_cast<int>(~static_cast<uint32_t>(e));
+              }
+          }
+          cluster.sync();
+          bound_key = sh.bound_key, bound_idx = sh.bound_idx;
+        }
+      }
+      if (!done)
+        cut(share_of(weight_of_kept(0.0, mine, before)), true);
+    }
+    const double floor_w = mp > 0.f ? static_cast<double>(mp) : 0.0;
+    const u64 all = weight_of_kept(floor_w, mine, before);
+    const u64 want = draw(all);
     if (before <= want && want < before + mine) {
-      const double floor_w = mp > 0.f ? fmin(static_cast<double>(mp), 1.0) : 0.0;
       u64 c = before;
       for (int i = i0; i < i1; ++i) {
         const uint32_t key = key_at(i);
@@ -317,7 +518,7 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS) sample_kerne
         const double w = rw.weight(key);
         if (w < floor_w)
           continue;
-        c += __double2ull_rn(w * SP_ONE);
+        c += Row::whole(w);
         if (c > want) {
           a.idx[row] = s0 + i;
           if (a.prob)
@@ -334,7 +535,8 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS) sample_kerne
 template <typename T> int launch_sample_t(SampleArgs a, int rows, int num_sms, cudaStream_t st) {
   static PerDeviceOnce once;
   if (once.get() < 0) {
-    if (cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * SP_SMEM_KEYS) !=
+    if (cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             4 * (2 * SP_BUCKETS + SP_SMEM_KEYS)) !=
         cudaSuccess)
       return 2;
     once.set(1);
@@ -349,7 +551,7 @@ template <typename T> int launch_sample_t(SampleArgs a, int rows, int num_sms, c
   a.in_smem = a.per_cta <= SP_SMEM_KEYS;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows) * C), cfg.blockDim = dim3(SP_THREADS);
-  cfg.dynamicSmemBytes = a.in_smem ? 4ull * a.per_cta : 0, cfg.stream = st;
+  cfg.dynamicSmemBytes = 4ull * (2 * SP_BUCKETS + (a.in_smem ? a.per_cta : 0)), cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = C, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
