@@ -212,6 +212,7 @@ struct AppendArgs {
   int num_pages, page_size, H, D;
   FastDiv by_page;
   int block_tokens; // tokens per CTA
+  int unit_blocks;  // CTAs that share a block of tokens
   unsigned dv, dv_magic; // vectors per row and ceil(2^32 / dv)
   int *status;
 };
@@ -243,6 +244,22 @@ template <typename T, int VE> struct RowVec {
     }
   }
 };
+// Largest magnitude of a vector as the bits of a float, infinities and NaN among them: two bfloat16 at a time.
+template <typename T, int VE> __device__ __forceinline__ uint32_t amax_any(const RowVec<T, VE> &r, uint32_t m) {
+  if constexpr (VE == 8 && sizeof(T) == 2) { // m: the largest of either half
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      m = __vmaxu2(m, r.w[i] & 0x7fff7fffu);
+  } else {
+#pragma unroll
+    for (int i = 0; i < RowVec<T, VE>::WORDS; ++i)
+      m = max(m, r.w[i] & 0x7fffffffu);
+  }
+  return m;
+}
+template <typename T, int VE> __device__ __forceinline__ uint32_t amax_whole(uint32_t m) {
+  return VE == 8 && sizeof(T) == 2 ? max(m & 0xffff0000u, m << 16) : m;
+}
 // largest finite magnitude, as bits (ordered like the values)
 template <int VE> __device__ __forceinline__ uint32_t amax_bits(const float (&f)[VE], uint32_t m) {
 #pragma unroll
@@ -276,33 +293,54 @@ __device__ __forceinline__ float on_e4m3_grid(double v) {
   const int e = max(((__double2hiint(v) >> 20) & 0x7ff) - 1023, -6) - 3;
   return static_cast<float>(rint(v * __hiloint2double((1023 - e) << 20, 0)) * __hiloint2double((1023 + e) << 20, 0));
 }
-// Rows leave as v / s. A power of two's reciprocal is exact, so the product rounds once, in the
-// conversion; any other scale is divided by in 64 bits, or the quotient would be rounded twice.
-struct Divisor {
-  float s, inv;
-  bool pow2;
-  __device__ __forceinline__ explicit Divisor(float scale) : s(scale) {
-    pow2 = (__float_as_uint(scale) & 0x7fffffu) == 0;
-    inv = 1.0f / scale;
-  }
-  __device__ __forceinline__ uint32_t code2(float a, float b) const {
-    if (pow2)
-      return e4m3x2(a * inv, b * inv);
-    return e4m3x2(on_e4m3_grid(static_cast<double>(a) / s), on_e4m3_grid(static_cast<double>(b) / s));
-  }
-};
-template <int VE>
-__device__ __forceinline__ void store_row_vec(uint8_t *dst, const float (&f)[VE], const Divisor &div) {
+// Rows leave as v / s. A power of two's reciprocal is exact, so the product rounds once, in the conversion.
+template <int VE> __device__ __forceinline__ void store_row_vec(uint8_t *dst, const float (&f)[VE], float inv) {
   if constexpr (VE == 8) {
     uint2 u;
-    u.x = div.code2(f[0], f[1]) | (div.code2(f[2], f[3]) << 16);
-    u.y = div.code2(f[4], f[5]) | (div.code2(f[6], f[7]) << 16);
+    u.x = e4m3x2(f[0] * inv, f[1] * inv) | (e4m3x2(f[2] * inv, f[3] * inv) << 16);
+    u.y = e4m3x2(f[4] * inv, f[5] * inv) | (e4m3x2(f[6] * inv, f[7] * inv) << 16);
     *reinterpret_cast<uint2 *>(dst) = u;
   } else {
 #pragma unroll
     for (int i = 0; i < VE; ++i)
-      dst[i] = static_cast<uint8_t>(div.code2(f[i], 0.f) & 0xffu);
+      dst[i] = static_cast<uint8_t>(e4m3x2(f[i] * inv, 0.f) & 0xffu);
   }
+}
+// v / s for a scale that is no power of two, such that rounding it to e4m3's grid gives what the quotient itself
+// would: in 64 bits, by the reciprocal; where that comes out next to a half step that v is an exact multiple of,
+// the half step is the quotient. (A double division would be a call, and its registers the kernel's.)
+__device__ __forceinline__ double exact_quotient(float v, float s, double recip) {
+  const double q = v * recip;
+  if (!(fabs(q) < 1e6))
+    return q;
+  const int e = max(((__double2hiint(q) >> 20) & 0x7ff) - 1023, -6) - 4; // half steps
+  const double t = rint(q * __hiloint2double((1023 - e) << 20, 0)) * __hiloint2double((1023 + e) << 20, 0);
+  return t * s == v ? t : q; // a half step has five bits: its product with s is exact
+}
+__device__ __forceinline__ double reciprocal(float s) {
+  double r = 1.f / s;
+  r = fma(r, fma(-r, static_cast<double>(s), 1.0), r);
+  return fma(r, fma(-r, static_cast<double>(s), 1.0), r);
+}
+// What a page held, times held scale / new scale.
+__device__ __forceinline__ void requantise(uint8_t *tile, int bytes, float held, float now, int tid, int team) {
+  // the new scale is a power of two, so q * f is exact in float for a held power of two and in double for any other
+  const double f = held > 0.f ? static_cast<double>(held) * static_cast<double>(1.f / now) : 0.0;
+  const bool pow2 = (__float_as_uint(held) & 0x7fffffu) == 0;
+  const float ff = static_cast<float>(f);
+  auto again = [&](uint32_t two) -> uint32_t {
+    const float2 p = e4m3x2_to_float2(two);
+    return pow2 ? e4m3x2(p.x * ff, p.y * ff) : e4m3x2(on_e4m3_grid(p.x * f), on_e4m3_grid(p.y * f));
+  };
+  uint32_t *w = reinterpret_cast<uint32_t *>(tile);
+#pragma unroll 1
+  for (int k = tid; k < bytes / 4; k += team) {
+    const uint32_t u = w[k];
+    w[k] = again(u & 0xffffu) | (again(u >> 16) << 16);
+  }
+#pragma unroll 1
+  for (int k = (bytes & ~3) + tid; k < bytes; k += team)
+    tile[k] = static_cast<uint8_t>(again(tile[k]) & 0xffu);
 }
 
 // First set bit of `bits` at or after `from`, `n` if none below n.
@@ -318,16 +356,17 @@ __device__ __forceinline__ int next_bit(const uint32_t *bits, int from, int n) {
 }
 
 template <typename T, int VE, int TEAM>
-__global__ void __launch_bounds__(AP_THREADS, VE == 8 ? (sizeof(T) == 2 ? 8 : 5) : 4) kv_append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(AP_THREADS, VE == 8 ? (sizeof(T) == 2 ? (TEAM == 32 ? 6 : 8) : 5) : 4) kv_append_kernel(AppendArgs a) {
   // window of slots: the CTA's tokens and as many as one page holds after them
   extern __shared__ int sm[];
-  const int win = min(a.block_tokens + a.page_size, a.n_tokens - static_cast<int>(blockIdx.x) * a.block_tokens);
+  const int token_block = blockIdx.x / a.unit_blocks, unit_block = blockIdx.x - token_block * a.unit_blocks;
+  const int win = min(a.block_tokens + a.page_size, a.n_tokens - token_block * a.block_tokens);
   const int words = (a.block_tokens + a.page_size + 31) / 32;
   int *slot = sm;                                                             // [win]
   uint32_t *starts = reinterpret_cast<uint32_t *>(sm + a.block_tokens + a.page_size); // token begins a run (or none)
   uint32_t *disorder = starts + words;                                        // token continues a run at a lower offset
   __shared__ uint32_t red[AP_WARPS];
-  const int t0 = blockIdx.x * a.block_tokens;
+  const int t0 = token_block * a.block_tokens;
   const int ps = a.page_size, n_slots = a.num_pages * ps; // a slot fits 31 bits
   for (int i = threadIdx.x; i < words * 32; i += AP_THREADS) { // whole warps: the ballots need every lane
     int s = -1, before = -1;
@@ -335,11 +374,11 @@ __global__ void __launch_bounds__(AP_THREADS, VE == 8 ? (sizeof(T) == 2 ? 8 : 5)
       s = a.slots[t0 + i];
       before = t0 + i > 0 ? a.slots[t0 + i - 1] : -1;
       if (s >= n_slots) {
-        if (blockIdx.y == 0)
+        if (unit_block == 0)
           atomicCAS(a.status, 0, MU_DEV_BAD_PAGE);
         s = -1;
       }
-      if (s < -1 && blockIdx.y == 0)
+      if (s < -1 && unit_block == 0)
         atomicCAS(a.status, 0, MU_DEV_BAD_PAGE);
       if (before >= n_slots)
         before = -1;
@@ -354,17 +393,17 @@ __global__ void __launch_bounds__(AP_THREADS, VE == 8 ? (sizeof(T) == 2 ? 8 : 5)
 
   // this team's head of K or V
   const int tid = TEAM == AP_THREADS ? threadIdx.x : threadIdx.x & 31;
-  const int unit = TEAM == AP_THREADS ? blockIdx.y : blockIdx.y * AP_WARPS + (threadIdx.x >> 5);
+  const int unit = TEAM == AP_THREADS ? unit_block : unit_block * AP_WARPS + (threadIdx.x >> 5);
   if (unit >= 2 * a.H)
     return; // only whole warps of a CTA that meets no more at a barrier
   const int which = unit & 1, h = unit >> 1;
+  const T *x = static_cast<const T *>(which ? a.x[1] : a.x[0]) + 1ll * h * a.D;
   auto team_sync = [] {
     if constexpr (TEAM == AP_THREADS)
       __syncthreads();
     else
       __syncwarp();
   };
-  const T *x = static_cast<const T *>(a.x[which]) + 1ll * h * a.D;
   // row of vector v: exact for v < 2^18, dv <= 2^8
   auto row_of = [&](unsigned v) { return a.dv == 1 ? v : __umulhi(v, a.dv_magic); };
   for (int i = next_bit(starts, 0, a.block_tokens); i < a.block_tokens && i < win;
@@ -387,98 +426,101 @@ __global__ void __launch_bounds__(AP_THREADS, VE == 8 ? (sizeof(T) == 2 ? 8 : 5)
       }
       n = j - i;
     }
-    uint8_t *tile = a.cache[which] + (1ull * page * a.H + h) * ps * a.D;
-    float *scale = a.scale[which] + 1ull * page * a.H + h;
+    uint8_t *tile = (which ? a.cache[1] : a.cache[0]) + (1ull * page * a.H + h) * ps * a.D;
+    float *scale = (which ? a.scale[1] : a.scale[0]) + 1ull * page * a.H + h;
     const float held = low > 0 ? *scale : 0.f;
     const T *rows = x + (1ll * t0 + i) * a.ld;
-    const long long total = 1ll * n * a.dv;
+
+    // vector tid + k TEAM of the run is (row, col); the next one is a few rows further
+    struct At {
+      int row, col;
+    };
+    const int dv = a.dv, row_step = TEAM / dv, col_step = TEAM % dv;
+    auto step = [&](At &at) {
+      at.row += row_step, at.col += col_step;
+      if (at.col >= dv)
+        at.col -= dv, ++at.row;
+    };
+    const At begin{static_cast<int>(row_of(tid)), tid - static_cast<int>(row_of(tid)) * dv};
 
     RowVec<T, VE> keep[AP_REGS];
     uint32_t m = 0;
+    At at = begin;
 #pragma unroll
-    for (int k = 0; k < AP_REGS; ++k) {
-      const unsigned v = tid + k * TEAM;
-      if (v < total) {
-        const unsigned row = row_of(v);
-        keep[k].load(rows + row * a.ld + (v - row * a.dv) * VE);
-      }
+    for (int k = 0; k < AP_REGS; ++k, step(at))
+      if (at.row < n)
+        keep[k].load(rows + at.row * a.ld + at.col * VE);
+    const At behind = at; // what the registers do not hold
+    at = begin;
+#pragma unroll
+    for (int k = 0; k < AP_REGS; ++k, step(at))
+      if (at.row < n)
+        m = amax_any<T, VE>(keep[k], m);
+#pragma unroll 1
+    for (at = behind; at.row < n; step(at)) {
+      RowVec<T, VE> r;
+      r.load(rows + at.row * a.ld + at.col * VE);
+      m = amax_any<T, VE>(r, m);
     }
+    auto team_max = [&](uint32_t mine) {
+      mine = __reduce_max_sync(~0u, mine);
+      if constexpr (TEAM == AP_THREADS) {
+        __syncthreads(); // red[] may still be read
+        if ((tid & 31) == 0)
+          red[tid >> 5] = mine;
+        __syncthreads();
 #pragma unroll
-    for (int k = 0; k < AP_REGS; ++k)
-      if (tid + k * TEAM < total) {
+        for (int w = 0; w < AP_WARPS; ++w)
+          mine = max(mine, red[w]);
+      }
+      return mine;
+    };
+    m = team_max(amax_whole<T, VE>(m));
+    if (m >= 0x7f800000u) { // infinities or NaN: once more, without them
+      m = 0;
+#pragma unroll 1
+      for (at = begin; at.row < n; step(at)) {
+        RowVec<T, VE> r;
         float f[VE];
-        keep[k].floats(f);
+        r.load(rows + at.row * a.ld + at.col * VE);
+        r.floats(f);
         m = amax_bits<VE>(f, m);
       }
-    for (long long v = tid + AP_REGS * TEAM; v < total; v += TEAM) {
-      RowVec<T, VE> r;
-      float f[VE];
-      r.load(rows + (v / a.dv) * a.ld + (v % a.dv) * VE);
-      r.floats(f);
-      m = amax_bits<VE>(f, m);
-    }
-    m = __reduce_max_sync(~0u, m);
-    if constexpr (TEAM == AP_THREADS) {
-      if ((tid & 31) == 0)
-        red[tid >> 5] = m;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < AP_WARPS; ++w)
-        m = max(m, red[w]);
+      m = team_max(m);
     }
     const float now = fmaxf(held, page_scale(m));
     if (tid == 0)
       *scale = now;
-    if (low > 0 && now > held) { // what the page held: low * D bytes from the tile's start
-      // now is a power of two here, so q * (held / now) is exact in float for a held power of two and in
-      // double for any other
-      const double f = held > 0.f ? static_cast<double>(held) / now : 0.0;
-      const bool pow2 = (__float_as_uint(held) & 0x7fffffu) == 0;
-      const float ff = static_cast<float>(f);
-      const int bytes = low * a.D;
-      auto again = [&](uint32_t two) -> uint32_t {
-        const float2 p = e4m3x2_to_float2(two);
-        return pow2 ? e4m3x2(p.x * ff, p.y * ff) : e4m3x2(on_e4m3_grid(p.x * f), on_e4m3_grid(p.y * f));
-      };
-      uint32_t *w = reinterpret_cast<uint32_t *>(tile);
-      for (int k = tid; k < bytes / 4; k += TEAM) {
-        const uint32_t u = w[k];
-        w[k] = again(u & 0xffffu) | (again(u >> 16) << 16);
-      }
-      for (int k = (bytes & ~3) + tid; k < bytes; k += TEAM)
-        tile[k] = static_cast<uint8_t>(again(tile[k]) & 0xffu);
-    }
-    const Divisor div(now);
-    if (ordered) {
+    if (low > 0 && now > held) // the tokens before the new ones: low * D bytes from the tile's start
+      requantise(tile, low * a.D, held, now, tid, TEAM);
+    if (ordered && (__float_as_uint(now) & 0x7fffffu) == 0) {
+      const float inv = 1.f / now;
+      at = begin;
 #pragma unroll
-      for (int k = 0; k < AP_REGS; ++k) {
-        const unsigned v = tid + k * TEAM;
-        if (v < total) {
-          const unsigned row = row_of(v);
+      for (int k = 0; k < AP_REGS; ++k, step(at))
+        if (at.row < n) {
           float f[VE];
           keep[k].floats(f);
-          store_row_vec<VE>(tile + (slot[i + row] - page0) * a.D + (v - row * a.dv) * VE, f, div);
+          store_row_vec<VE>(tile + (slot[i + at.row] - page0) * a.D + at.col * VE, f, inv);
         }
-      }
-      for (unsigned v = tid + AP_REGS * TEAM; v < total; v += TEAM) {
-        const unsigned row = row_of(v);
+#pragma unroll 1
+      for (at = behind; at.row < n; step(at)) {
         RowVec<T, VE> r;
         float f[VE];
-        r.load(rows + row * a.ld + (v - row * a.dv) * VE);
+        r.load(rows + at.row * a.ld + at.col * VE);
         r.floats(f);
-        store_row_vec<VE>(tile + (slot[i + row] - page0) * a.D + (v - row * a.dv) * VE, f, div);
+        store_row_vec<VE>(tile + (slot[i + at.row] - page0) * a.D + at.col * VE, f, inv);
       }
     } else {
+      const double recip = reciprocal(now);
+#pragma unroll 1
       for (int j = 0; j < n; ++j) {
         team_sync(); // the requantised bytes and the token before are in place
-        const int s = a.slots[t0 + i + j];
-        for (unsigned v = tid; v < a.dv; v += TEAM) {
-          RowVec<T, VE> r;
-          float f[VE];
-          r.load(rows + j * a.ld + v * VE);
-          r.floats(f);
-          store_row_vec<VE>(tile + (s - page0) * a.D + v * VE, f, div);
-        }
+        uint8_t *dst = tile + (a.slots[t0 + i + j] - page0) * a.D;
+#pragma unroll 1
+        for (int d = tid; d < a.D; d += TEAM)
+          dst[d] = static_cast<uint8_t>(
+              e4m3x2(on_e4m3_grid(exact_quotient(static_cast<float>(rows[j * a.ld + d]), now, recip)), 0.f) & 0xffu);
       }
     }
     team_sync(); // red[] is free again
@@ -523,8 +565,11 @@ int launch_kv_append(AppendArgs a, int dtype, int num_sms, cudaStream_t st) {
   a.block_tokens = static_cast<int>(tb);
   const int span = a.block_tokens + a.page_size, words = (span + 31) / 32;
   const size_t smem = sizeof(int) * (span + 2ull * words);
-  const int heads = team == 32 ? (2 * a.H + AP_WARPS - 1) / AP_WARPS : 2 * a.H;
-  const dim3 grid(static_cast<unsigned>((a.n_tokens + tb - 1) / tb), static_cast<unsigned>(heads));
+  // The heads of one block of tokens are neighbours in the grid: their rows are neighbours in memory (256 bytes
+  // a head, kilobytes between tokens), so DRAM pages are read while they are open.
+  a.unit_blocks = team == 32 ? (2 * a.H + AP_WARPS - 1) / AP_WARPS : 2 * a.H;
+  const long long blocks = (a.n_tokens + tb - 1) / tb;
+  const dim3 grid(static_cast<unsigned>(blocks * a.unit_blocks));
   if (dtype == F32)
     launch_append_t<float>(a, vec, team, grid, smem, st);
   else

@@ -28,7 +28,7 @@ namespace cg = cooperative_groups;
 namespace mu {
 
 constexpr int SP_THREADS = 1024, SP_WARPS = SP_THREADS / 32, SP_MAX_CLUSTER = 8;
-constexpr int SP_BUCKETS = 4096, SP_LIST = 1024;
+constexpr int SP_BUCKETS = 4096, SP_LIST = 1024, SP_RANKED = 256;
 constexpr float SP_BUCKETS_PER_NAT = 92.3325f; // 64 to a factor of two
 constexpr int SP_SMEM_KEYS = 43008; // keys of one CTA that fit its shared memory beside the buckets (168 KB)
 constexpr double SP_ONE = 4398046511104.0; // 2^42: the weight of the row's maximum
@@ -75,6 +75,7 @@ struct SampleShared {
   int found_index;
   double table[32];   // 2^(i/32)
   u64 list[SP_LIST];  // (key, ~index), rank 0's
+  int ranks[SP_RANKED];
   int n_list;
   int bucket;         // that the cut falls into
   u64 above, within;  // measure before it, and of it
@@ -141,19 +142,43 @@ struct Row {
   __device__ __forceinline__ u64 fixed(uint32_t key) const { return whole(weight(key)); }
 };
 
-// Sorts v[0 .. n) (n a power of two up to SP_THREADS) in descending order.
-__device__ __forceinline__ void sort_desc(u64 *v, int n) {
+// Sorts v[0 .. n) in descending order; n a power of two up to SP_THREADS, non-zero values distinct. Short lists
+// by counting what is larger than each (all threads share that, three barriers), others by bitonic merges.
+__device__ __forceinline__ void sort_desc(u64 *v, int *ranks, int n) {
   const int i = threadIdx.x;
-  for (int k = 2; k <= n; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      __syncthreads();
-      const int o = i ^ j;
-      if (i < n && o > i) {
-        const u64 x = v[i], y = v[o];
-        if ((x < y) == ((i & k) == 0))
-          v[i] = y, v[o] = x;
-      }
+  __syncthreads();
+  if (n <= SP_RANKED) {
+    const int e = i & (n - 1), share = max(1, n * n / SP_THREADS), from = i / n * share;
+    const u64 x = v[e];
+    if (i < n)
+      ranks[i] = 0;
+    __syncthreads();
+    if (from < n) {
+      int larger = 0;
+      for (int j = from; j < from + share; ++j)
+        larger += v[j] > x;
+      if (larger)
+        atomicAdd(&ranks[e], larger);
     }
+    __syncthreads();
+    if (i < n)
+      v[i] = 0;
+    const int at = i < n ? ranks[i] : 0;
+    __syncthreads();
+    if (i < n && x)
+      v[at] = x;
+  } else {
+    for (int k = 2; k <= n; k <<= 1)
+      for (int j = k >> 1; j > 0; j >>= 1) {
+        const int o = i ^ j;
+        if (i < n && o > i) {
+          const u64 x = v[i], y = v[o];
+          if ((x < y) == ((i & k) == 0))
+            v[i] = y, v[o] = x;
+        }
+        __syncthreads();
+      }
+  }
   __syncthreads();
 }
 
@@ -180,11 +205,43 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS) sample_kerne
     sh.n_list = 0;
 
   uint32_t top = 0;
-  for (int i = tid; i < n; i += SP_THREADS) {
-    const uint32_t k = to_key(load_logit(x, i));
-    if (a.in_smem)
-      keys[i] = k;
-    top = max(top, k);
+  {
+    auto take = [&](int i, uint32_t k) {
+      if (a.in_smem)
+        keys[i] = k;
+      top = max(top, k);
+    };
+    // 16 bytes a thread from the first 16-byte boundary on, several loads in flight; the ends one by one
+    constexpr int E = 16 / sizeof(T), U = 4;
+    const int head = min(n, static_cast<int>((16 - reinterpret_cast<uintptr_t>(x) % 16) % 16 / sizeof(T)));
+    const int packs = (n - head) / E;
+    const uint4 *body = reinterpret_cast<const uint4 *>(x + head);
+    for (int q0 = tid; q0 < packs; q0 += U * SP_THREADS) {
+      uint4 v[U];
+#pragma unroll
+      for (int e = 0; e < U; ++e)
+        if (q0 + e * SP_THREADS < packs)
+          v[e] = __ldcs(body + q0 + e * SP_THREADS);
+#pragma unroll
+      for (int e = 0; e < U; ++e)
+        if (const int q = q0 + e * SP_THREADS; q < packs) {
+          const uint32_t w[4] = {v[e].x, v[e].y, v[e].z, v[e].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (sizeof(T) == 4) {
+              take(head + 4 * q + j, to_key(__uint_as_float(w[j])));
+            } else {
+              take(head + 8 * q + 2 * j, to_key(bf16_lo(w[j])));
+              take(head + 8 * q + 2 * j + 1, to_key(bf16_hi(w[j])));
+            }
+          }
+        }
+    }
+    const int rest = n - head - packs * E; // fewer than E on either side
+    if (tid < head)
+      take(tid, to_key(load_logit(x, tid)));
+    if (tid < rest)
+      take(n - rest + tid, to_key(load_logit(x, n - rest + tid)));
   }
   top = __reduce_max_sync(~0u, top);
   if (lane == 0)
@@ -378,15 +435,21 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS) sample_kerne
       }
       cluster.sync();
       u64 v[4] = {0, 0, 0, 0}, all;
-      for (int r = 0; r < C; ++r) {
-        const uint32_t *from = cluster.map_shared_rank(buckets, r) + 4 * tid;
-        const uint4 lo = *reinterpret_cast<const uint4 *>(from);
-        v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
-        if (weight) {
-          const uint4 hi = *reinterpret_cast<const uint4 *>(from + SP_BUCKETS);
-          v[0] += static_cast<u64>(hi.x) << 32, v[1] += static_cast<u64>(hi.y) << 32;
-          v[2] += static_cast<u64>(hi.z) << 32, v[3] += static_cast<u64>(hi.w) << 32;
+      uint4 lo[SP_MAX_CLUSTER], hi[SP_MAX_CLUSTER]; // all remote loads before the first sum
+#pragma unroll
+      for (int r = 0; r < SP_MAX_CLUSTER; ++r) {
+        lo[r] = hi[r] = make_uint4(0, 0, 0, 0);
+        if (r < C) {
+          const uint32_t *from = cluster.map_shared_rank(buckets, r) + 4 * tid;
+          lo[r] = *reinterpret_cast<const uint4 *>(from);
+          if (weight)
+            hi[r] = *reinterpret_cast<const uint4 *>(from + SP_BUCKETS);
         }
+      }
+#pragma unroll
+      for (int r = 0; r < SP_MAX_CLUSTER; ++r) {
+        v[0] += lo[r].x + (static_cast<u64>(hi[r].x) << 32), v[1] += lo[r].y + (static_cast<u64>(hi[r].y) << 32);
+        v[2] += lo[r].z + (static_cast<u64>(hi[r].z) << 32), v[3] += lo[r].w + (static_cast<u64>(hi[r].w) << 32);
       }
       const u64 sum = v[0] + v[1] + v[2] + v[3];
       u64 at = block_scan(sum, sh, all) - sum;
@@ -422,7 +485,7 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS) sample_kerne
         m <<= 1;
       if (tid >= count && tid < m)
         sh.list[tid] = 0;
-      sort_desc(sh.list, m);
+      sort_desc(sh.list, sh.ranks, m);
       return tid < count ? sh.list[tid] : 0ull;
     };
     const float mp = a.min_p && a.min_p[row] > 0.f ? fminf(a.min_p[row], 1.f) : 0.f;
@@ -460,7 +523,7 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS) sample_kerne
             m <<= 1;
           if (tid < m)
             sh.list[tid] = in ? (e << 32) | key : 0ull;
-          sort_desc(sh.list, m);
+          sort_desc(sh.list, sh.ranks, m);
           const u64 f = tid < m ? sh.list[tid] : 0ull;
           const uint32_t fk = static_cast<uint32_t>(f);
           const double fw = f ? rw.weight(fk) : 0.0;
