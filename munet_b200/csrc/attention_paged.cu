@@ -14,8 +14,7 @@
 // in which workers run. Every item counts a few units more than its chunks, for what starting a segment
 // costs: without it the workers that got many short requests finished last.
 #include "../../include/munet_b200.h"
-#include "common.h"
-#include "ptx.cuh"
+#include "attention_paged.cuh"
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -24,57 +23,6 @@
 
 namespace mu {
 
-struct PagedArgs {
-  const void *q;
-  void *out;
-  long long q_ld, out_ld; // elements between tokens
-  const uint8_t *kc, *vc;
-  const float *ks, *vs;
-  const int *table;
-  int table_stride;
-  const int *query_start, *seq_lens;
-  int B, n_tokens, Hq, Hkv, G, D, num_pages, page_size, causal;
-  FastDiv by_group, by_page;
-  float scale_log2; // log2(e) / sqrt(D)
-  struct SplitItem *items; // by the worker that holds the first chunk
-  int2 *notes;             // per worker: rows of the split item it begins (0: none), worker that began the
-                           // item its first segment continues (-1: none)
-  float2 *part_ml;
-  float *part_o;
-  int rows_per_tile; // stride of the partial results
-  int *status;
-};
-
-// A (request, head, row tile) whose chunks went to more than one worker; entry w belongs to the worker
-// that holds its first chunk. Its later pieces are the first segments of workers w+1 .. last.
-struct SplitItem {
-  int first_slot, last, row0, n_rows, q0, head;
-};
-
-constexpr int START_UNITS = 3; // what beginning an item counts for, in chunks (1: 69.3 us, 2: 67.3, 3: 66.3 for 64 requests)
-
-struct Seq {
-  int q0, nq, len;  // first row of q, new tokens, tokens in the cache (as given)
-  int seen;         // tokens the block table can address
-};
-__device__ __forceinline__ Seq load_seq(const PagedArgs &a, int b) {
-  Seq s;
-  s.q0 = a.query_start[b];
-  const int q1 = a.query_start[b + 1];
-  s.nq = q1 - s.q0;
-  s.len = a.seq_lens[b];
-  if (s.q0 < 0 || q1 < s.q0 || q1 > a.n_tokens || s.len < 0) {
-    atomicCAS(a.status, 0, MU_DEV_BAD_LENGTH);
-    s.nq = 0, s.len = 0;
-  }
-  const long long room = 1ll * a.table_stride * a.page_size;
-  s.seen = s.len;
-  if (s.nq > 0 && s.len > room) {
-    atomicCAS(a.status, 0, MU_DEV_BAD_PAGE);
-    s.seen = static_cast<int>(room);
-  }
-  return s;
-}
 template <int CHUNK> __device__ __forceinline__ int chunks_of(const Seq &s) {
   return s.seen > 0 ? (s.seen - 1) / CHUNK + 1 : 1;
 }
@@ -84,15 +32,6 @@ template <int R, int CHUNK> __device__ __forceinline__ long long units_of(const 
   const unsigned rows = static_cast<unsigned>(s.nq) * a.G; // n_tokens * Hq fits 31 bits
   return 1ll * a.Hkv * ((rows + R - 1) / R) * (chunks_of<CHUNK>(s) + START_UNITS);
 }
-// Keys row `row` of a request may see.
-__device__ __forceinline__ int row_limit(const PagedArgs &a, const Seq &s, int row) {
-  if (row >= s.nq * a.G)
-    return 0;
-  if (!a.causal)
-    return s.seen;
-  return max(0, min(s.seen, s.len - s.nq + a.by_group.div(row) + 1));
-}
-
 // Inclusive prefix of units over the requests into shared memory; returns the total.
 template <int THREADS, int R, int CHUNK>
 __device__ __forceinline__ long long scan_units(const PagedArgs &a, long long *upto, long long *warp_sum) {
@@ -125,24 +64,6 @@ __device__ __forceinline__ long long scan_units(const PagedArgs &a, long long *u
     upto[b] += before;
   __syncthreads();
   return total;
-}
-
-struct Segment {
-  int b, head, n_rows, row0; // request, KV head, rows of the tile that exist, first of them
-  int chunk0, chunks;        // range of this worker
-  int slot;                  // -1: complete
-};
-
-// Unit counts hardly ever need 64 bits, and a 64-bit division costs a hundred instructions.
-__device__ __forceinline__ long long div64(long long x, long long d) {
-  if (((x | d) >> 32) == 0)
-    return static_cast<unsigned>(x) / static_cast<unsigned>(d);
-  return x / d;
-}
-__device__ __forceinline__ long long div_rem(long long x, int d, int &rem) {
-  const long long q = div64(x, d);
-  rem = static_cast<int>(x - q * d);
-  return q;
 }
 
 // Walks one worker's share of the unit list.
@@ -209,13 +130,6 @@ template <int R, int CHUNK> struct Walk {
     return true;
   }
 };
-
-__device__ __forceinline__ void store_out(float *p, float v) { *p = v; }
-__device__ __forceinline__ void store_out(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
-__device__ __forceinline__ float load_in(const float *p) { return *p; }
-__device__ __forceinline__ float load_in(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
-// weight of a piece whose running maximum is m where the whole's is M
-__device__ __forceinline__ float rel_weight(float m, float M) { return M == -INFINITY ? 1.f : ex2_approx(m - M); }
 
 // ---- CUDA-core kernel: head sizes that are no multiple of 16 ---------------------------------------
 // float32 products and sums. Per warp a tile of 32 keys: for the scores a lane owns a key (its row is D
@@ -479,21 +393,6 @@ template <int DP, int NR, int TEAM, bool SPLIT> struct MmaCfg {
   static constexpr int KW = DP / 16, VW = DP / 32, NT = DP / 16; // 32-bit words of K / V a lane reads per key; d-tiles
 };
 
-__device__ __forceinline__ uint32_t f16x2_of_e4m3_lo(uint32_t w) {
-  uint32_t d;
-  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(d) : "r"(w));
-  return d;
-}
-__device__ __forceinline__ uint32_t f16x2_of_e4m3_hi(uint32_t w) {
-  uint32_t d;
-  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(d) : "r"(w));
-  return d;
-}
-__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
-  uint32_t d;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
-  return d;
-}
 // what is left of two floats after their rounding to fp16
 __device__ __forceinline__ uint32_t f16x2_rest(float lo, float hi, uint32_t h) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
@@ -553,10 +452,6 @@ __device__ __forceinline__ void read_words(uint32_t (&w)[N], const unsigned char
     }
   }
 }
-__device__ __forceinline__ bool has_nan_e4m3(uint32_t w) {
-  return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
-}
-
 template <typename T, int DP, int NR, int TEAM>
 __global__ void __launch_bounds__(MmaCfg<DP, NR, TEAM, sizeof(T) == 4>::THREADS,
                                   MmaCfg<DP, NR, TEAM, sizeof(T) == 4>::CTAS_PER_SM)
@@ -1146,8 +1041,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) attention_paged_join_kernel(Page
   // Few pieces: a warp joins a row. With one worker to the CTA its warps share the rows, with four each has
   // a worker of its own.
   {
-    const int me = blockIdx.x * per_cta + (per_cta > 1 ? warp : 0), part = per_cta > 1 ? 0 : warp;
-    const int parts = per_cta > 1 ? 1 : JOIN_WARPS;
+    const int me = blockIdx.x * per_cta + (per_cta > 1 ? warp : 0);
+    const int part = per_cta > 1 ? 0 : blockIdx.y * JOIN_WARPS + warp, parts = per_cta > 1 ? 1 : gridDim.y * JOIN_WARPS;
     const int2 note = me < workers ? a.notes[me] : make_int2(0, -1);
     bool many = false;
 #pragma unroll 1
@@ -1186,7 +1081,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) attention_paged_join_kernel(Page
       const int pieces = it.last - owner + 1, share = min(pieces, it.n_rows);
       if (pieces <= FEW)
         continue;
-      for (int r = me - owner; r < it.n_rows; r += share) {
+      for (int r = me - owner + blockIdx.y * share; r < it.n_rows; r += gridDim.y * share) {
         const Joined j = join_pieces(a, it, owner, r, warp, JOIN_WARPS, pieces);
         if (lane == 0)
           red_ml[warp] = make_float2(j.M, j.sum);
@@ -1217,18 +1112,29 @@ __global__ void __launch_bounds__(JOIN_THREADS) attention_paged_join_kernel(Page
 constexpr int SIMT_CTAS_PER_SM = 4;
 constexpr int MAX_WORKERS_PER_SM = 12;
 
-// Rows of partial results over all workers: 12 workers of 8 rows, 8 of 16, or 4 CTAs of 8 per SM, two each.
-constexpr size_t MAX_PART_ROWS_PER_SM = 2 * 128;
-
-size_t paged_workspace_bytes(int num_sms, int D) {
-  const size_t rows = static_cast<size_t>(num_sms) * MAX_PART_ROWS_PER_SM;
-  return rows * (sizeof(float) * D + sizeof(float2)) + (sizeof(SplitItem) + sizeof(int2)) * num_sms * MAX_WORKERS_PER_SM;
+// Rows of partial results per SM, two pieces a worker: 12 workers of 8 rows, 8 of 16, 4 CTAs of 8; one of 256
+// for prompt chunks.
+constexpr int MAX_PART_ROWS_PER_SM = 2 * 128;
+// Requests with this many rows (new tokens x heads of a group) or more go to the prompt-chunk kernel: below, a
+// tile of 256 rows would be mostly empty, and reading the keys once per 16 rows costs less.
+constexpr int TILE_KERNEL_ROWS = 64;
+bool uses_tile_kernel(int n_tokens, int B, int G, int D, int dtype) {
+  return dtype == BF16 && (D == 64 || D == 128) && n_tokens > B && B <= MU_PAGED_TILE_MAX_REQUESTS &&
+         1ll * n_tokens * G >= TILE_KERNEL_ROWS;
+}
+size_t part_rows(int num_sms, int n_tokens, int B, int G, int D, int dtype) {
+  return static_cast<size_t>(num_sms) *
+         (uses_tile_kernel(n_tokens, B, G, D, dtype) ? 2 * PAGED_TILE_ROWS : MAX_PART_ROWS_PER_SM);
+}
+size_t paged_workspace_bytes(int num_sms, int n_tokens, int B, int G, int D, int dtype) {
+  return part_rows(num_sms, n_tokens, B, G, D, dtype) * (sizeof(float) * D + sizeof(float2)) +
+         (sizeof(SplitItem) + sizeof(int2)) * num_sms * MAX_WORKERS_PER_SM;
 }
 
-// per_cta: workers that a CTA of the join stands for, 1 or JOIN_WARPS
-template <typename T> int launch_join(const PagedArgs &a, int workers, int per_cta, cudaStream_t st) {
+// per_cta: workers that a CTA of the join stands for, 1 or JOIN_WARPS; ctas: CTAs that share one worker's rows
+template <typename T> int launch_join(const PagedArgs &a, int workers, int per_cta, int ctas, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((workers + per_cta - 1) / per_cta), cfg.blockDim = dim3(JOIN_THREADS), cfg.stream = st;
+  cfg.gridDim = dim3((workers + per_cta - 1) / per_cta, ctas), cfg.blockDim = dim3(JOIN_THREADS), cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -1252,7 +1158,7 @@ template <typename T, int RT, int VB, int NA> int launch_simt(PagedArgs a, int n
   attention_paged_simt_kernel<T, RT, VB, NA><<<ctas, SIMT_THREADS, smem, st>>>(a);
   if (cudaGetLastError() != cudaSuccess)
     return 2;
-  return launch_join<T>(a, ctas, 1, st);
+  return launch_join<T>(a, ctas, 1, 1, st);
 }
 template <typename T, int VB, int NA> int launch_simt_rows(const PagedArgs &a, int num_sms, cudaStream_t st) {
   // rows that share a key: the group's heads for single tokens, up to 8 otherwise
@@ -1282,7 +1188,7 @@ template <typename T, int DP, int NR, int TEAM> int launch_mma_team(PagedArgs a,
   attention_paged_mma_kernel<T, DP, NR, TEAM><<<ctas, Cfg::THREADS, ring + 8ull * a.B, st>>>(a);
   if (cudaGetLastError() != cudaSuccess)
     return 2;
-  return launch_join<T>(a, ctas * Cfg::WARPS / TEAM, TEAM == 1 ? JOIN_WARPS : 1, st);
+  return launch_join<T>(a, ctas * Cfg::WARPS / TEAM, TEAM == 1 ? JOIN_WARPS : 1, 1, st);
 }
 template <typename T, int DP, int NR> int launch_mma(const PagedArgs &a, int num_sms, cudaStream_t st) {
   // Items (an upper bound) against warps: below an eighth every item would be cut into more than eight
@@ -1315,7 +1221,7 @@ template <typename T> int launch_by_dim(const PagedArgs &a, int num_sms, cudaStr
 
 // 0 ok, 1 dtype not implemented, 2 CUDA error
 int launch_attention_paged(PagedArgs a, void *workspace, int dtype, int num_sms, cudaStream_t st) {
-  const size_t rows = static_cast<size_t>(num_sms) * MAX_PART_ROWS_PER_SM;
+  const size_t rows = part_rows(num_sms, a.n_tokens, a.B, a.G, a.D, dtype);
   unsigned char *w = static_cast<unsigned char *>(workspace);
   a.part_o = reinterpret_cast<float *>(w);
   w += sizeof(float) * rows * a.D;
@@ -1324,6 +1230,14 @@ int launch_attention_paged(PagedArgs a, void *workspace, int dtype, int num_sms,
   a.notes = reinterpret_cast<int2 *>(w);
   w += sizeof(int2) * num_sms * MAX_WORKERS_PER_SM;
   a.items = reinterpret_cast<SplitItem *>(w);
+  a.rows_from = 1, a.rows_to = INT_MAX;
+  if (uses_tile_kernel(a.n_tokens, a.B, a.G, a.D, dtype)) {
+    PagedArgs t = a;
+    t.rows_from = TILE_KERNEL_ROWS, t.rows_per_tile = PAGED_TILE_ROWS;
+    if (launch_attention_paged_tile(t, num_sms, st) || launch_join<__nv_bfloat16>(t, num_sms, 1, 8, st))
+      return 2;
+    a.rows_to = TILE_KERNEL_ROWS - 1;
+  }
   if (dtype == F32)
     return launch_by_dim<float>(a, num_sms, st);
   if (dtype == BF16)
@@ -1341,10 +1255,9 @@ int mu_ctx_num_sms(const mu_ctx *ctx);
 int *mu_ctx_status_ptr(mu_ctx *ctx);
 
 size_t mu_attention_paged_workspace_bytes(const mu_ctx *ctx, int n_tokens, int B, int Hq, int Hkv, int D, int dtype) {
-  (void)dtype;
   if (!ctx || n_tokens <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0)
     return 0;
-  return mu::paged_workspace_bytes(mu_ctx_num_sms(ctx), D);
+  return mu::paged_workspace_bytes(mu_ctx_num_sms(ctx), n_tokens, B, Hq / Hkv, D, dtype);
 }
 
 int mu_attention_paged(mu_ctx *ctx, const void *q, long long q_ld, void *out, long long out_ld, const void *k_cache,

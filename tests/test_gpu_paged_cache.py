@@ -278,7 +278,8 @@ def check_attention(pr, out, dtype, causal, page):
     sums over keys are pieces of at most 2^-23 a step; the output is rounded once to its type. fp16's
     smallest step is 2^-24: the tensor-core kernel (head sizes that are multiples of 16) holds p_j vs_j with the
     row's largest at 2^15, for float32 as a sum of two, so each is off by up to half of 2^-24 * 2^-15 of the
-    largest, and multiplies a code of at most 448."""
+    largest, and multiplies a code of at most 448. The prompt-chunk kernel (bfloat16, head size 64 or 128, more
+    rows than requests) holds the largest between 2^7 and 2^15."""
     n_live = int(pr["qs"][-1])
     D = out.shape[2]
     want, weight, spread, top = ref.attention(pr["qx"], pr["kc"], pr["vc"], pr["ks"].astype(np.float64),
@@ -288,7 +289,8 @@ def check_attention(pr, out, dtype, causal, page):
     L = int(pr["seq"].max(initial=1))
     prob = 2 * (D + 4) * 2.0 ** -23 * spread + 2.0 ** -20 + (2.0 ** -11 if dtype == BF16 else 2.0 ** -22) + L * 2.0 ** -23
     half = 2.0 ** -8 if dtype == BF16 else 2.0 ** -24
-    low = L * 448 * 2.0 ** -40 * top if D % 16 == 0 else 0 * top
+    chunks = dtype == BF16 and D in (64, 128) and out.shape[0] > len(pr["seq"])
+    low = L * 448 * (2.0 ** -32 if chunks else 2.0 ** -40) * top if D % 16 == 0 else 0 * top
     bound = half * np.abs(want) + 2 * prob[..., None] * weight + low[..., None] + 1e-30
     err = np.abs(got - want)[:n_live]
     assert np.isfinite(got).all()
@@ -317,6 +319,10 @@ CASES = [
     (40, 2, 2, 64, 16, list(range(1, 41)), [1] * 40),
     (1, 2, 1, 128, 64, [6000], [1]),
     (2, 8, 2, 128, 64, [1000, 700], [300, 1]),
+    (3, 4, 4, 64, 16, [513, 90, 700], [257, 90, 64]),
+    (1, 8, 1, 128, 16, [3000], [33]),
+    (2, 14, 2, 128, 32, [600, 1300], [513, 37]),
+    (1, 70, 1, 64, 16, [300], [2]),
     (2, 4, 2, 48, 16, [70, 33], [1, 1]),
     (2, 4, 4, 112, 32, [70, 333], [3, 1]),
     (1, 1, 1, 16, 16, [100], [1]),
@@ -350,12 +356,12 @@ def test_attention_rows_that_see_nothing(ctx, dtype, D):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("D,G", [(64, 1), (128, 4), (40, 2)])
-def test_attention_ignores_what_it_must_not_see(ctx, dtype, D, G):
+@pytest.mark.parametrize("D,G,new", [(64, 1, 6), (128, 4, 6), (40, 2, 6), (128, 4, 40), (64, 8, 33)])
+def test_attention_ignores_what_it_must_not_see(ctx, dtype, D, G, new):
     """NaN behind the last token of a page, and in tokens that a causal row may not see yet."""
     rng = np.random.default_rng(4)
     B, page, Hkv = 2, 16, 2
-    pr = make_problem(rng, dtype, B, Hkv * G, Hkv, D, page, [37, 50], [1, 6])
+    pr = make_problem(rng, dtype, B, Hkv * G, Hkv, D, page, [37, 50], [1, new])
     clean = run_attention(ctx, pr, dtype, True, Hkv, page).clone()
     weight = ref.attention(pr["qx"], pr["kc"], pr["vc"], pr["ks"].astype(float), pr["vs"].astype(float), pr["table"],
                            pr["qs"], pr["seq"], page, True)[1]
@@ -371,17 +377,17 @@ def test_attention_ignores_what_it_must_not_see(ctx, dtype, D, G):
             pr["vc"][last, :, L % page:] = 127
     p49 = pr["table"][1, 49 // page]
     pr["vc"][p49, :, 49 % page, 5] = 0xFF  # the last token of request 1: only its own row sees it
-    pr["kc"][pr["table"][1, 48 // page], 1, 48 % page, :] = 127  # key of token 48, head 1: rows 4 and 5
+    pr["kc"][pr["table"][1, 48 // page], 1, 48 % page, :] = 127  # key of token 48, head 1: the last two rows
     out = run_attention(ctx, pr, dtype, True, Hkv, page)
     ctx.check()
     a, b = clean.double().cpu().numpy(), out.double().cpu().numpy()
-    rows = pr["qs"][1] + np.arange(6)
+    rows = pr["qs"][1] + np.arange(new)
     assert np.array_equal(a[0], b[0])
-    assert same(a[rows[:4]], b[rows[:4]], weight[rows[:4]])
-    assert same(a[rows[4], :G], b[rows[4], :G], weight[rows[4], :G]) and np.isnan(b[rows[4], G:]).all()
-    assert np.isnan(b[rows[5], :G, 5]).all() and np.isnan(b[rows[5], G:]).all()
+    assert same(a[rows[:-2]], b[rows[:-2]], weight[rows[:-2]])
+    assert same(a[rows[-2], :G], b[rows[-2], :G], weight[rows[-2], :G]) and np.isnan(b[rows[-2], G:]).all()
+    assert np.isnan(b[rows[-1], :G, 5]).all() and np.isnan(b[rows[-1], G:]).all()
     keep = [d for d in range(D) if d != 5]
-    assert same(a[rows[5], :G][:, keep], b[rows[5], :G][:, keep], weight[rows[5], :G][:, keep])
+    assert same(a[rows[-1], :G][:, keep], b[rows[-1], :G][:, keep], weight[rows[-1], :G][:, keep])
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
