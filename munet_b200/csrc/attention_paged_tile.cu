@@ -1,11 +1,11 @@
 // Prompt chunks over the paged e4m3 cache: the tensor-core form of attention_paged.cu for requests with
 // many rows (new tokens x query heads of a KV head), bfloat16, head size 64 or 128.
 //
-// Bound by the tensor pipe and the softmax in front of it. Persistent, one CTA per SM, 13 warps:
+// Bound by the softmax in front of the tensor pipe. Persistent, one CTA per SM, 16 warps:
 //   warp 0      issues every tcgen05.mma (fp16 operands, fp32 accumulators in tensor memory)
-//   warps 1-4   bring keys and values in: e4m3 bytes from their pages, turned into fp16 (exact) and
+//   warps 1-7   bring keys and values in: e4m3 bytes from their pages, turned into fp16 (exact) and
 //               written where a TMA with 128-byte swizzle would have put them
-//   warps 5-12  the softmax of query tiles A and B (128 rows each, one thread per row), as in the
+//   warps 8-15  the softmax of query tiles A and B (128 rows each, one thread per row), as in the
 //               prompt kernel of attention_tcgen05.cu: S in tensor memory, P written back over it as
 //               fp16, O rescaled in place only when a row's maximum grew by more than 2^8
 // A and B share every key tile of 128. Rows are (token, head) pairs, heads of a group next to each other.
@@ -24,7 +24,7 @@
 namespace mu {
 
 constexpr int PT_BQ = 128, PT_BK = 128, PT_ROWS = 2 * PT_BQ; // a row tile is the pair A, B
-constexpr int PT_LOADERS = 4, PT_THREADS = 32 * (1 + PT_LOADERS + 8);
+constexpr int PT_LOADERS = 7, PT_THREADS = 32 * (1 + PT_LOADERS + 8);
 constexpr int PT_UNIT = 8, PT_START = 16; // keys of a unit; units that beginning an item counts for
 constexpr int PT_SLOTS = 4;               // key tiles whose page scales are kept
 constexpr float PT_W_EXP = 7.f;           // a row's reference weight is 2^7: with the 2^8 the maximum may lead, 2^15
@@ -32,8 +32,8 @@ constexpr float PT_W_EXP = 7.f;           // a row's reference weight is 2^7: wi
 template <int D> struct PtCfg {
   static constexpr int Q_BYTES = PT_BQ * D * 2, K_BYTES = PT_BK * D * 2, DB = D / 64;
   static constexpr int SMEM = 2 * Q_BYTES + 4 * K_BYTES; // Q_A, Q_B, two K and two V tiles
-  static constexpr int BARS = 24;
-  static constexpr int TAIL = BARS * 8 + PT_SLOTS * 8 * 16 + PT_SLOTS * PT_LOADERS * 4 + 16;
+  static constexpr int BARS = 28;
+  static constexpr int TAIL = BARS * 8 + PT_SLOTS * 8 * 16 + PT_SLOTS * 32 + 16;
 };
 
 // Row tile costs of one request: tile t counts first + t * slope units, no fewer than the keys it sees / 8.
@@ -134,6 +134,12 @@ struct TileWalk {
   }
 };
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 template <int D>
 __global__ void __launch_bounds__(PT_THREADS, 1) attention_paged_tile_kernel(PagedArgs a) {
   using Cfg = PtCfg<D>;
@@ -145,12 +151,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_paged_tile_kernel(Pag
   uint64_t *bars = reinterpret_cast<uint64_t *>(sV + 2 * Cfg::K_BYTES);
   uint64_t *q_full = bars, *q_empty = bars + 2, *k_full = bars + 4, *k_empty = bars + 6, *v_full = bars + 8,
            *v_empty = bars + 10, *s_full = bars + 12, *p_full = bars + 14, *o_full = bars + 16, *o_free = bars + 18,
-           *m_full = bars + 20; // [PT_SLOTS]
-  static_assert(20 + PT_SLOTS <= Cfg::BARS, "barriers");
+           *m_full = bars + 20, *n_full = m_full + PT_SLOTS; // [PT_SLOTS]: scales, NaN flags
+  static_assert(20 + 2 * PT_SLOTS <= Cfg::BARS, "barriers");
   float4 *scales = reinterpret_cast<float4 *>(bars + Cfg::BARS); // [PT_SLOTS][8]: K scale, log2 and 1 / V scale
-  int4 *v_nan = reinterpret_cast<int4 *>(scales + PT_SLOTS * 8); // [PT_SLOTS]: by loader, some value of the tile is NaN
-  static_assert(PT_LOADERS == 4, "one flag each");
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(v_nan + PT_SLOTS);
+  int4 *v_nan = reinterpret_cast<int4 *>(scales + PT_SLOTS * 8); // [PT_SLOTS][2]: by loader, some value of the tile is NaN
+  static_assert(PT_LOADERS <= 8, "one flag each");
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(v_nan + 2 * PT_SLOTS);
   long long *upto = reinterpret_cast<long long *>(smem + Cfg::SMEM + (Cfg::TAIL + 15) / 16 * 16);
   __shared__ long long warp_sum[PT_THREADS / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, me = blockIdx.x;
@@ -204,7 +210,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_paged_tile_kernel(Pag
       mbar_init(&o_full[x], 1), mbar_init(&o_free[x], 4);
     }
     for (int i = 0; i < PT_SLOTS; ++i)
-      mbar_init(&m_full[i], PT_LOADERS);
+      mbar_init(&m_full[i], 1), mbar_init(&n_full[i], PT_LOADERS);
+    for (int i = 0; i < 2 * PT_SLOTS; ++i)
+      v_nan[i] = make_int4(0, 0, 0, 0);
     fence_barrier_init();
   }
   __syncthreads();
@@ -325,105 +333,149 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_paged_tile_kernel(Pag
     __syncwarp();
   } else if (warp <= PT_LOADERS) {
     // ------------------------------ keys and values ---------------------------
-    constexpr int CPK = D / 16, STEP = 32 * PT_LOADERS / CPK, N = PT_BK / STEP; // chunks per key; keys per sweep; sweeps
-    const int lt = tid - 32, chunk = lt % CPK, key_of = lt / CPK;
-    uint32_t t = 0; // key tiles so far
-    while (ok && walk.next(a, upto, g, s, false)) {
-      const int nk = max(tiles_of(0), tiles_of(1));
-      for (int j = 0; j < nk && ok; ++j, ++t) {
-        const int key0 = (g.chunk0 + j) * PT_BK, slot = t & (PT_SLOTS - 1);
-        const int *pages = a.table + 1ll * g.b * a.table_stride;
-        auto page_of = [&](int key) {
-          int page = -1;
-          if (key < s.seen) {
-            page = pages[a.by_page.div(key)];
-            if (page < 0 || page >= a.num_pages) {
-              atomicCAS(a.status, 0, MU_DEV_BAD_PAGE);
-              page = -1;
-            }
-          }
-          return page;
-        };
-        int page[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          page[i] = page_of(key0 + key_of + i * STEP);
-        uint4 kr[N], vr[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
-          if (page[i] >= 0) {
-            const long long at = ((1ll * page[i] * a.Hkv + g.head) * a.page_size + a.by_page.mod(key0 + key_of + i * STEP)) * D +
-                                 chunk * 16;
-            kr[i] = __ldg(reinterpret_cast<const uint4 *>(a.kc + at));
-            vr[i] = __ldg(reinterpret_cast<const uint4 *>(a.vc + at));
-          }
+    // piece i of a thread: 16 bytes, chunk p % CPK of key p / CPK with p = lt + 224 i
+    constexpr int CPK = D / 16, SWEEP = 32 * PT_LOADERS, N = (PT_BK * CPK + SWEEP - 1) / SWEEP;
+    const int lt = tid - 32;
+    // Three tiles are under way: K and V of tile t are written to shared memory as their stages come free,
+    // those of t + 1 are then requested into the same registers, and the pages of t + 2 are looked up. Lane g
+    // of every warp keeps group g of 16 keys (one page): where its bytes begin, and how many keys are live.
+    struct Tile {
+      const int *pages; // the request's row of the block table
+      int head, key0, seen;
+      bool any;
+      int page;       // of group `lane`, as it is in the table
+      long long base; // bytes before the group, or -1
+    };
+    int j = 0, nk = 0;
+    auto next_tile = [&](Tile &n) { // and the look-up of its pages
+      n.any = true;
+      while (j >= nk) {
+        if (!walk.next(a, upto, g, s, false)) {
+          n.any = false;
+          break;
         }
-        if (lt < 8) { // scales of the tile's groups of 16 keys; no page: no weight
-          const int p = page_of(key0 + 16 * lt);
-          float4 sc = make_float4(0.f, -INFINITY, 0.f, 0.f);
-          if (p >= 0) {
-            const float vs = fmaxf(a.vs[1ll * p * a.Hkv + g.head], 0x1p-64f);
-            sc = make_float4(a.ks[1ll * p * a.Hkv + g.head], log2f(vs), 1.f / vs, 0.f);
-          }
-          scales[slot * 8 + lt] = sc;
-        }
-        // NaN values become zeros here; the rows that see them are marked by the softmax warps
-        bool nan = false;
+        j = 0, nk = max(tiles_of(0), tiles_of(1));
+      }
+      n.pages = a.table + 1ll * g.b * a.table_stride;
+      n.head = g.head, n.key0 = (g.chunk0 + j) * PT_BK, n.seen = n.any ? s.seen : 0;
+      n.page = -1;
+      if (lane < 8 && n.key0 + 16 * lane < n.seen)
+        n.page = n.pages[a.by_page.div(n.key0 + 16 * lane)];
+      ++j;
+    };
+    auto settle = [&](Tile &n) { // the pages have arrived
+      const int key = n.key0 + 16 * lane;
+      const bool wanted = lane < 8 && key < n.seen, good = wanted && n.page >= 0 && n.page < a.num_pages;
+      if (wanted && !good)
+        atomicCAS(a.status, 0, MU_DEV_BAD_PAGE);
+      n.base = good ? ((1ll * n.page * a.Hkv + n.head) * a.page_size + a.by_page.mod(key)) * D : -1;
+    };
+    auto request = [&](const uint8_t *cache, const Tile &n, uint4 (&r)[N]) {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-          nan |= has_nan_e4m3(vr[i].x) | has_nan_e4m3(vr[i].y) | has_nan_e4m3(vr[i].z) | has_nan_e4m3(vr[i].w);
-        nan = __any_sync(~0u, nan);
-        if (lane == 0)
-          reinterpret_cast<int *>(v_nan + slot)[warp - 1] = nan;
-        if (nan) {
-          auto clean = [](uint32_t w) {
-#pragma unroll
-            for (int k = 0; k < 32; k += 8)
-              if (((w >> k) & 0x7fu) == 0x7fu)
-                w &= ~(0xffu << k);
-            return w;
-          };
-#pragma unroll
-          for (int i = 0; i < N; ++i)
-            vr[i] = make_uint4(clean(vr[i].x), clean(vr[i].y), clean(vr[i].z), clean(vr[i].w));
-        }
+      for (int i = 0; i < N; ++i) {
+        const int piece = lt + SWEEP * i, key = piece / CPK;
+        const long long base = __shfl_sync(~0u, n.base, (key >> 4) & 7);
+        const bool live = key < PT_BK && base >= 0 && n.key0 + key < n.seen;
+        const uint4 *at = reinterpret_cast<const uint4 *>(cache + (live ? base + (piece & (16 * CPK - 1)) * 16 : 0));
+        // zeros first: written after the load they would wait for it, and every load for the one before
+        r[i] = make_uint4(0, 0, 0, 0);
+        if (live)
+          r[i] = __ldg(at);
+      }
+    };
+    auto put = [&](uint8_t *dst, const uint4 &r, int row, int cc) { // 16 elements: two swizzled 16-byte chunks
+      *reinterpret_cast<uint4 *>(dst + row * 128 + ((cc ^ (row & 7)) << 4)) =
+          make_uint4(f16x2_of_e4m3_lo(r.x), f16x2_of_e4m3_hi(r.x), f16x2_of_e4m3_lo(r.y), f16x2_of_e4m3_hi(r.y));
+      *reinterpret_cast<uint4 *>(dst + row * 128 + (((cc + 1) ^ (row & 7)) << 4)) =
+          make_uint4(f16x2_of_e4m3_lo(r.z), f16x2_of_e4m3_hi(r.z), f16x2_of_e4m3_lo(r.w), f16x2_of_e4m3_hi(r.w));
+    };
+    Tile now, soon;
+    uint4 kr[N], vr[N];
+    float ks = 0.f, vs = 0.f; // this lane's group of the tile `now`
+    auto request_scales = [&](const Tile &n) {
+      ks = vs = 0.f;
+      if (warp == 1 && n.base >= 0) {
+        const long long at = 1ll * n.page * a.Hkv + n.head;
+        ks = a.ks[at], vs = a.vs[at];
+      }
+    };
+    next_tile(now);
+    settle(now);
+    if (now.any) {
+      request(a.kc, now, kr);
+      request(a.vc, now, vr);
+      request_scales(now);
+      next_tile(soon);
+    }
+    for (uint32_t t = 0; ok && now.any; ++t) {
+      const int slot = t & (PT_SLOTS - 1), stage = t & 1;
+      if (warp == 1) { // no page: no weight
+        if (lane < 8)
+          scales[slot * 8 + lane] = now.base >= 0
+                                        ? make_float4(ks, log2f(fmaxf(vs, 0x1p-64f)), 1.f / fmaxf(vs, 0x1p-64f), 0.f)
+                                        : make_float4(0.f, -INFINITY, 0.f, 0.f);
         __syncwarp();
         if (lane == 0)
           mbar_arrive(&m_full[slot]);
-
-        auto put = [&](uint8_t *dst, const uint4 &r, int row, int cc) { // 16 elements: two swizzled 16-byte chunks
-          *reinterpret_cast<uint4 *>(dst + row * 128 + ((cc ^ (row & 7)) << 4)) =
-              make_uint4(f16x2_of_e4m3_lo(r.x), f16x2_of_e4m3_hi(r.x), f16x2_of_e4m3_lo(r.y), f16x2_of_e4m3_hi(r.y));
-          *reinterpret_cast<uint4 *>(dst + row * 128 + (((cc + 1) ^ (row & 7)) << 4)) =
-              make_uint4(f16x2_of_e4m3_lo(r.z), f16x2_of_e4m3_hi(r.z), f16x2_of_e4m3_lo(r.w), f16x2_of_e4m3_hi(r.w));
+      }
+      settle(soon);
+      if (!wait(&k_empty[stage], ((t >> 1) & 1) ^ 1, MU_DEV_TIMEOUT_PRODUCER))
+        break;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int piece = lt + SWEEP * i, key = piece / CPK, chunk = piece % CPK;
+        if (key < PT_BK)
+          put(sK + stage * Cfg::K_BYTES + chunk / 4 * (PT_BK * 128), kr[i], key, chunk % 4 * 2);
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0)
+        mbar_arrive(&k_full[stage]);
+      request(a.kc, soon, kr);
+      // NaN values become zeros here; the rows that see them are marked by the softmax warps
+      bool nan = false;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        nan |= has_nan_e4m3(vr[i].x) | has_nan_e4m3(vr[i].y) | has_nan_e4m3(vr[i].z) | has_nan_e4m3(vr[i].w);
+      nan = __any_sync(~0u, nan);
+      if (nan) {
+        auto clean = [](uint32_t w) {
+#pragma unroll
+          for (int k = 0; k < 32; k += 8)
+            if (((w >> k) & 0x7fu) == 0x7fu)
+              w &= ~(0xffu << k);
+          return w;
         };
-        const int stage = t & 1, db = chunk / 4, cc = chunk % 4 * 2;
-        if (!wait(&k_empty[stage], ((t >> 1) & 1) ^ 1, MU_DEV_TIMEOUT_PRODUCER))
-          break;
 #pragma unroll
         for (int i = 0; i < N; ++i)
-          put(sK + stage * Cfg::K_BYTES + db * (PT_BK * 128), kr[i], key_of + i * STEP, cc);
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0)
-          mbar_arrive(&k_full[stage]);
-        if (!wait(&v_empty[stage], ((t >> 1) & 1) ^ 1, MU_DEV_TIMEOUT_PRODUCER))
-          break;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int key = key_of + i * STEP;
-          put(sV + stage * Cfg::K_BYTES + ((key >> 6) * DB + db) * 8192, vr[i], key & 63, cc);
-        }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0)
-          mbar_arrive(&v_full[stage]);
+          vr[i] = make_uint4(clean(vr[i].x), clean(vr[i].y), clean(vr[i].z), clean(vr[i].w));
       }
+      if (lane == 0) {
+        reinterpret_cast<int *>(v_nan + 2 * slot)[warp - 1] = nan;
+        mbar_arrive(&n_full[slot]);
+      }
+      __syncwarp();
+      if (!wait(&v_empty[stage], ((t >> 1) & 1) ^ 1, MU_DEV_TIMEOUT_PRODUCER))
+        break;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int piece = lt + SWEEP * i, key = piece / CPK, chunk = piece % CPK;
+        if (key < PT_BK)
+          put(sV + stage * Cfg::K_BYTES + ((key >> 6) * DB + chunk / 4) * 8192, vr[i], key & 63, chunk % 4 * 2);
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0)
+        mbar_arrive(&v_full[stage]);
+      request(a.vc, soon, vr);
+      request_scales(soon);
+      now = soon;
+      if (now.any)
+        next_tile(soon);
     }
   } else {
-    // ---------------- softmax and output: warps 5-8 tile A, warps 9-12 tile B ----------------
-    const int x = (warp - 5) >> 2;
+    // ---------------- softmax and output: warps 8-11 tile A, warps 12-15 tile B ----------------
+    const int x = (warp - 8) >> 2;
     const int q = warp & 3; // tensor-memory lane quarter this warp may access
     const int row = q * 32 + lane;
     const uint32_t lane_sel = static_cast<uint32_t>(q * 32) << 16;
@@ -433,7 +485,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_paged_tile_kernel(Pag
       const int nk_all = max(tiles_of(0), tiles_of(1)), nk = tiles_of(x);
       const int my_row = g.row0 + x * PT_BQ + row; // of the request
       const bool live = x * PT_BQ + row < g.n_rows;
-      const int limit = live ? row_limit(a, s, my_row) : 0;
+      const int limit = live ? row_limit(a, s, my_row) : s.seen + PT_BK; // a row that is not there needs no mask
       const int token = a.by_group.div(my_row), head = g.head * a.G + a.by_group.mod(my_row);
       const uint32_t tile0 = t0;
       t0 += nk_all;
@@ -490,30 +542,42 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_paged_tile_kernel(Pag
           tc_fence_after();
           const float4 *sc = scales + slot * 8;
           const bool edge = __any_sync(~0u, lim < PT_BK); // some row of the warp does not see the whole tile
+          // 32 columns at a time, the next 32 on their way
+          auto sweep = [&](auto &&each) {
+            uint32_t r[2][32];
+            tmem_ld_32x32(s_addr, r[0]);
+            tmem_ld_wait();
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              if (h < 3)
+                tmem_ld_32x32(s_addr + (h + 1) * 32, r[(h + 1) & 1]);
+              each(h, r[h & 1]);
+              if (h < 3)
+                tmem_ld_wait();
+            }
+          };
           // pass 1: the row's maximum
           float mx = m_ref;
           auto maxima = [&](auto masked) {
-#pragma unroll
-            for (int h = 0; h < 4; ++h) {
-              uint32_t r[32];
-              tmem_ld_32x32(s_addr + h * 32, r);
-              tmem_ld_wait();
+            sweep([&](int h, const uint32_t (&r)[32]) {
 #pragma unroll
               for (int gr = 0; gr < 2; ++gr) {
-                float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                float best[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                  float v = __uint_as_float(r[gr * 16 + k]);
-                  if (decltype(masked)::value && h * 32 + gr * 16 + k >= lim)
-                    v = -INFINITY;
-                  top4[k & 3] = fmaxf(top4[k & 3], v);
+                for (int k = 0; k < 16; k += 2) {
+                  float v0 = __uint_as_float(r[gr * 16 + k]), v1 = __uint_as_float(r[gr * 16 + k + 1]);
+                  if (decltype(masked)::value) {
+                    const int col = h * 32 + gr * 16 + k;
+                    v0 = col < lim ? v0 : -INFINITY, v1 = col + 1 < lim ? v1 : -INFINITY;
+                  }
+                  best[k >> 1 & 1] = max3(best[k >> 1 & 1], v0, v1);
                 }
                 const float4 c = sc[2 * h + gr];
-                const float best = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
-                if (!decltype(masked)::value || best > -INFINITY) // nothing seen: 0 * inf is no maximum
-                  mx = fmaxf(mx, fmaf(best, c.x * fac, c.y));
+                const float top = fmaxf(best[0], best[1]);
+                if (!decltype(masked)::value || top > -INFINITY) // nothing seen: 0 * inf is no maximum
+                  mx = fmaxf(mx, fmaf(top, c.x * fac, c.y));
               }
-            }
+            });
           };
           if (edge)
             maxima(std::true_type{});
@@ -525,7 +589,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_paged_tile_kernel(Pag
             const bool grow = mx > m_ref + 8.f;
             if (__any_sync(~0u, grow)) { // the previous P.V is complete: s_full was committed after it
               const float f2 = grow ? ex2_approx(m_ref - mx) : 1.f;
-#pragma unroll
+#pragma unroll 1
               for (int c = 0; c < D / 32; ++c) {
                 uint32_t r[32];
                 tmem_ld_32x32(o_addr + c * 32, r);
@@ -542,13 +606,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_paged_tile_kernel(Pag
             }
           }
           const float shift = m_ref == -INFINITY ? 0.f : PT_W_EXP - m_ref;
-          // pass 2: weights, back over the scores already read
+          // pass 2: weights, back over scores already read
           auto weights = [&](auto masked) {
-#pragma unroll
-            for (int h = 0; h < 4; ++h) {
-              uint32_t r[32], pk[16];
-              tmem_ld_32x32(s_addr + h * 32, r);
-              tmem_ld_wait();
+            sweep([&](int h, const uint32_t (&r)[32]) {
+              uint32_t pk[16];
 #pragma unroll
               for (int gr = 0; gr < 2; ++gr) {
                 const float4 c = sc[2 * h + gr];
@@ -572,16 +633,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_paged_tile_kernel(Pag
                 f32x2_unpack(sum2, s0, s1);
                 l_run = fmaf(s0 + s1, c.z, l_run);
               }
-              tmem_st_32x16(s_addr + h * 16, pk);
-            }
+              tmem_st_32x16(s_addr + h * 16, pk); // columns below 16 (h + 1): read, or in registers
+            });
           };
           if (edge)
             weights(std::true_type{});
           else
             weights(std::false_type{});
-          const int4 some = v_nan[slot];
-          if (some.x | some.y | some.z | some.w) { // which dimensions of the keys this row sees are NaN
-            const int see = min(PT_BK, lim), key0 = (g.chunk0 + j) * PT_BK;
+          if (!wait(&n_full[slot], ((tile0 + j) / PT_SLOTS) & 1, MU_DEV_TIMEOUT_EPILOGUE))
+            break;
+          const int4 some = v_nan[2 * slot], more = v_nan[2 * slot + 1];
+          if (some.x | some.y | some.z | some.w | more.x | more.y | more.z) { // which dimensions of the keys this row sees are NaN
+            const int key0 = (g.chunk0 + j) * PT_BK, see = min(min(PT_BK, lim), s.seen - key0);
             for (int k = 0; k < see; ++k) {
               const int page = a.table[1ll * g.b * a.table_stride + a.by_page.div(key0 + k)];
               if (page < 0 || page >= a.num_pages)
