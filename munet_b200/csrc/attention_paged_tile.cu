@@ -25,7 +25,8 @@ namespace mu {
 
 constexpr int PT_BQ = 128, PT_BK = 128, PT_ROWS = 2 * PT_BQ; // a row tile is the pair A, B
 constexpr int PT_LOADERS = 7, PT_THREADS = 32 * (1 + PT_LOADERS + 8);
-constexpr int PT_UNIT = 8, PT_START = 16; // keys of a unit; units that beginning an item counts for
+constexpr int PT_UNIT = 8, PT_START = 112; // keys of a unit; units that beginning an item counts for: seven key tiles
+                                           // (16 units: 823 us for the mixed chunks below, 48: 770, 80: 717, 128: 712)
 constexpr int PT_SLOTS = 4;               // key tiles whose page scales are kept
 constexpr float PT_W_EXP = 7.f;           // a row's reference weight is 2^7: with the 2^8 the maximum may lead, 2^15
 
@@ -495,16 +496,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_paged_tile_kernel(Pag
       for (int i = 0; i < D / 32; ++i)
         nan_mask[i] = 0;
       if (nk > 0) {
-        // this row of Q, scaled by a power of two to at most 2^15, as fp16
         if (!wait(&q_empty[x], (wx & 1) ^ 1, MU_DEV_TIMEOUT_EPILOGUE))
           break;
+        // this row of Q, scaled by a power of two to at most 2^15, as fp16. Loops that run once per work are
+        // kept short: unrolled, they took longer to fetch as instructions than to execute.
         const __nv_bfloat16 *qp = static_cast<const __nv_bfloat16 *>(a.q) +
                                   (live ? 1ll * (s.q0 + token) * a.q_ld + 1ll * head * D : 0);
         const bool vec = (reinterpret_cast<uintptr_t>(qp) & 15u) == 0;
         auto load8 = [&](int c) { // elements 8c ..
           uint4 u = make_uint4(0, 0, 0, 0);
-          if (live && vec) {
-            u = *(reinterpret_cast<const uint4 *>(qp) + c);
+          if (vec) {
+            if (live)
+              u = *(reinterpret_cast<const uint4 *>(qp) + c);
           } else if (live) {
             const unsigned short *e = reinterpret_cast<const unsigned short *>(qp) + 8 * c;
             u = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
@@ -512,23 +515,30 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_paged_tile_kernel(Pag
           return u;
         };
         uint32_t top = 0;
+#pragma unroll 1
+        for (int c = 0; c < D / 8; c += 8) { // a 128-byte line, its loads together
+          uint4 u[8];
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          const uint4 u = load8(c);
-          top = __vmaxu2(top, __vmaxu2(__vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu),
-                                       __vmaxu2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu)));
+          for (int k = 0; k < 8; ++k)
+            u[k] = load8(c + k);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            top = __vmaxu2(top, __vmaxu2(__vmaxu2(u[k].x & 0x7fff7fffu, u[k].y & 0x7fff7fffu),
+                                         __vmaxu2(u[k].z & 0x7fff7fffu, u[k].w & 0x7fff7fffu)));
         }
         top = max(top >> 16, top & 0xffffu) << 16;
         const int e = min(max(static_cast<int>(top >> 23) - 127 - 14, -100), 113);
         const float f = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
         const float fac = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * a.scale_log2;
+#pragma unroll 1
+        for (int c = 0; c < D / 8; c += 2)
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          const uint4 u = load8(c);
-          auto two = [&](uint32_t w) { return f16x2(bf16_lo(w) * f, bf16_hi(w) * f); };
-          *reinterpret_cast<uint4 *>(sQ + x * Cfg::Q_BYTES + (c >> 3) * (PT_BQ * 128) + row * 128 +
-                                     (((c & 7) ^ (row & 7)) << 4)) = make_uint4(two(u.x), two(u.y), two(u.z), two(u.w));
-        }
+          for (int k = 0; k < 2; ++k) {
+            const uint4 u = load8(c + k);
+            auto two = [&](uint32_t w) { return f16x2(bf16_lo(w) * f, bf16_hi(w) * f); };
+            *reinterpret_cast<uint4 *>(sQ + x * Cfg::Q_BYTES + ((c + k) >> 3) * (PT_BQ * 128) + row * 128 +
+                                       ((((c + k) & 7) ^ (row & 7)) << 4)) = make_uint4(two(u.x), two(u.y), two(u.z), two(u.w));
+          }
         fence_proxy_async();
         __syncwarp();
         if (lane == 0)
@@ -671,12 +681,26 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_paged_tile_kernel(Pag
           break;
         tc_fence_after();
       }
-      // ---- output: rows of bfloat16, or a piece for the join
+      // ---- output: rows of bfloat16, or a piece for the join. Through this warp's rows of Q's tile (every
+      // product that reads them is done), so that rows leave 16 lanes at a time: 16-byte stores a row apart
+      // wait on each other's latency.
       const float inv = g.slot >= 0 ? 1.f : l_run == 0.f ? 0.f : 1.f / l_run;
       const long long pr = 1ll * max(g.slot, 0) * a.rows_per_tile + x * PT_BQ + row;
-      __nv_bfloat16 *op = static_cast<__nv_bfloat16 *>(a.out) + (live ? 1ll * (s.q0 + token) * a.out_ld + 1ll * head * D : 0);
-      const bool ovec = (reinterpret_cast<uintptr_t>(op) & 15u) == 0;
-#pragma unroll
+      uint8_t *stage = sQ + x * Cfg::Q_BYTES + q * 32 * D * 2; // 32 rows of D * 2 bytes
+      constexpr int ROW = D * 2, PER_ROW = ROW / 16;           // bytes, 16-byte words
+      auto cell = [&](int r, int c) { return reinterpret_cast<uint4 *>(stage + r * ROW + ((c ^ (r & 7)) << 4)); };
+      const long long my_out = live ? 1ll * (s.q0 + token) * a.out_ld + 1ll * head * D : -1;
+      auto rows_out = [&](auto &&to) { // the staged rows, coalesced: to(row of the warp, word) takes 16 bytes
+        __syncwarp();
+#pragma unroll 2
+        for (int i = 0; i < PER_ROW; ++i) {
+          const int r = i * (32 / PER_ROW) + lane / PER_ROW, c = lane % PER_ROW;
+          to(r, c, *cell(r, c));
+        }
+        __syncwarp();
+      };
+      const bool piece = g.slot >= 0;
+#pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t r[32];
         if (nk > 0) {
@@ -687,30 +711,49 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_paged_tile_kernel(Pag
           for (int k = 0; k < 32; ++k)
             r[k] = 0;
         }
-        if (!live)
-          continue;
+        uint32_t nan = 0;
 #pragma unroll
-        for (int k = 0; k < 32; ++k) {
-          r[k] = __float_as_uint(__uint_as_float(r[k]) * inv);
-          if (nan_mask[c] >> k & 1u)
-            r[k] = 0x7fffffffu;
-        }
-        if (g.slot >= 0) {
-#pragma unroll
-          for (int k = 0; k < 32; k += 4)
-            *reinterpret_cast<uint4 *>(a.part_o + pr * D + c * 32 + k) = make_uint4(r[k], r[k + 1], r[k + 2], r[k + 3]);
-        } else if (ovec) {
-#pragma unroll
-          for (int k = 0; k < 32; k += 8) {
-            auto two = [&](int i) { return pack_bf16x2(__uint_as_float(r[k + i]), __uint_as_float(r[k + i + 1])); };
-            *reinterpret_cast<uint4 *>(op + c * 32 + k) = make_uint4(two(0), two(2), two(4), two(6));
-          }
-        } else {
+        for (int i = 0; i < D / 32; ++i)
+          nan = c == i ? nan_mask[i] : nan;
+        if (__any_sync(~0u, nan != 0))
 #pragma unroll
           for (int k = 0; k < 32; ++k)
-            op[c * 32 + k] = __float2bfloat16_rn(__uint_as_float(r[k]));
+            r[k] = nan >> k & 1u ? 0x7fffffffu : r[k];
+        if (piece) { // a half of the dimensions as floats fills the row
+#pragma unroll
+          for (int k = 0; k < 32; k += 4)
+            *cell(lane, c % (D / 64) * 8 + k / 4) = make_uint4(r[k], r[k + 1], r[k + 2], r[k + 3]);
+          if (c % (D / 64) == D / 64 - 1)
+            rows_out([&](int w, int word, const uint4 &v) {
+              if (x * PT_BQ + q * 32 + w < g.n_rows)
+                *reinterpret_cast<uint4 *>(a.part_o + (pr - lane + w) * D + c / (D / 64) * (D / 2) + word * 4) = v;
+            });
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; k += 8) {
+            auto two = [&](int i) {
+              return pack_bf16x2(__uint_as_float(r[k + i]) * inv, __uint_as_float(r[k + i + 1]) * inv);
+            };
+            *cell(lane, c * 4 + k / 8) = make_uint4(two(0), two(2), two(4), two(6));
+          }
         }
       }
+      if (!piece)
+        rows_out([&](int w, int word, const uint4 &v) {
+          const long long off = __shfl_sync(~0u, my_out, w);
+          if (off < 0)
+            return;
+          __nv_bfloat16 *op = static_cast<__nv_bfloat16 *>(a.out) + off + 8 * word;
+          if ((reinterpret_cast<uintptr_t>(op) & 15u) == 0) {
+            *reinterpret_cast<uint4 *>(op) = v;
+          } else {
+            unsigned short *e = reinterpret_cast<unsigned short *>(op);
+            const uint32_t half[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              e[k] = static_cast<unsigned short>(half[k >> 1] >> (16 * (k & 1)));
+          }
+        });
       if (live && g.slot >= 0)
         a.part_ml[pr] = make_float2(m_ref == -INFINITY ? -INFINITY : m_ref - PT_W_EXP, l_run);
       if (nk > 0) {
