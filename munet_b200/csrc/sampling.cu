@@ -27,10 +27,11 @@ namespace cg = cooperative_groups;
 
 namespace mu {
 
-constexpr int SP_THREADS = 1024, SP_WARPS = SP_THREADS / 32, SP_MAX_CLUSTER = 8;
-constexpr int SP_BUCKETS = 4096, SP_LIST = 1024, SP_RANKED = 256;
+constexpr int SP_THREADS = 512, SP_WARPS = SP_THREADS / 32, SP_MAX_CLUSTER = 8;
+constexpr int SP_BUCKETS = 4096, SP_LIST = 512, SP_RANKED = 128;
 constexpr float SP_BUCKETS_PER_NAT = 92.3325f; // 64 to a factor of two
 constexpr int SP_SMEM_KEYS = 43008; // keys of one CTA that fit its shared memory beside the buckets (168 KB)
+constexpr int SP_PAIR_KEYS = 15360; // and of one of two CTAs of an SM: one loads while the other computes
 constexpr double SP_ONE = 4398046511104.0; // 2^42: the weight of the row's maximum
 
 struct SampleArgs {
@@ -44,7 +45,7 @@ struct SampleArgs {
   int cols, per_cta, in_smem;
 };
 
-constexpr uint32_t KEY_NEG_INF = 0x007fffffu, KEY_POS_INF = 0xff800000u;
+constexpr uint32_t KEY_NEG_INF = 0x007fffffu;
 // Order-preserving image of a float; NaN counts as -inf, -0 as +0.
 __device__ __forceinline__ uint32_t to_key(float v) {
   if (v != v)
@@ -96,7 +97,7 @@ __device__ __forceinline__ u64 block_scan(u64 v, SampleShared &sh, u64 &all) {
   if (lane == 31)
     sh.warp_sum[warp] = v;
   __syncthreads();
-  u64 w = sh.warp_sum[lane];
+  u64 w = lane < SP_WARPS ? sh.warp_sum[lane] : 0;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
     const u64 t = __shfl_up_sync(~0u, w, d);
@@ -115,15 +116,12 @@ struct Row {
   double c, minus; // t = x * c + minus
   const double *table;
   uint32_t max_key;
-  bool spike; // the maximum is +inf: only elements equal to it weigh anything
+  // No branches, so that several run at a time. What has no t counts as zero: -inf, and next to a maximum of
+  // +inf everything but the elements equal to it.
   __device__ __forceinline__ double weight(uint32_t key) const {
-    if (key == max_key)
-      return 1.0;
-    if (spike || key <= KEY_NEG_INF)
-      return 0.0;
-    const double t = fma(static_cast<double>(from_key(key)), c, minus);
-    if (!(t > -64.0)) // counts as zero (2^-43 and below)
-      return 0.0;
+    const double t0 = fma(static_cast<double>(from_key(key)), c, minus);
+    const bool some = t0 > -64.0; // below: 2^-43 or less
+    const double t = some ? t0 : -64.0;
     const double shift = 0x1.8p52 / 32; // adding it rounds t to a multiple of 1/32
     const double r = t + shift;
     const int i = __double2loint(r);
@@ -133,7 +131,8 @@ struct Row {
     p = fma(f, p, 0x1.ebfbdff82c58fp-3);
     p = fma(f, p, 0x1.62e42fefa39efp-1);
     p = fma(f, p, 1.0) * table[i & 31];
-    return __hiloint2double(__double2hiint(p) + ((i >> 5) << 20), __double2loint(p));
+    const double w = __hiloint2double(__double2hiint(p) + ((i >> 5) << 20), __double2loint(p));
+    return key == max_key ? 1.0 : some ? w : 0.0;
   }
   // rounded to a multiple of 2^-42, as that multiple
   __device__ __forceinline__ static u64 whole(double w) {
@@ -182,7 +181,7 @@ __device__ __forceinline__ void sort_desc(u64 *v, int *ranks, int n) {
   __syncthreads();
 }
 
-template <typename T> __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a) {
+template <typename T> __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
   extern __shared__ __align__(16) uint32_t buckets[]; // [2][SP_BUCKETS], then the keys
   uint32_t *const keys = buckets + 2 * SP_BUCKETS;
   __shared__ SampleShared sh;
@@ -248,7 +247,7 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS) sample_kerne
     sh.warp_max[warp] = top;
   __syncthreads();
   if (warp == 0) {
-    top = __reduce_max_sync(~0u, sh.warp_max[lane]);
+    top = __reduce_max_sync(~0u, lane < SP_WARPS ? sh.warp_max[lane] : 0u);
     if (lane == 0)
       sh.cta_max = top;
   }
@@ -302,7 +301,7 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS) sample_kerne
     }
   } else {
     Row rw;
-    rw.max_key = top, rw.spike = top == KEY_POS_INF;
+    rw.max_key = top;
     const float xmax = from_key(top);
     rw.table = sh.table;
     rw.c = 1.4426950408889634 / static_cast<double>(T_row), rw.minus = -static_cast<double>(xmax) * rw.c;
@@ -387,13 +386,11 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS) sample_kerne
     auto weight_of_kept = [&](double floor_w, u64 &mine, u64 &before) { // sum over the row
       mine = 0;
       u64 all;
+#pragma unroll 4
       for (int i = i0; i < i1; ++i) {
         const uint32_t k = key_at(i);
-        if (kept(k, i)) {
-          const double w = rw.weight(k);
-          if (w >= floor_w)
-            mine += Row::whole(w);
-        }
+        const double w = rw.weight(k);
+        mine += kept(k, i) && w >= floor_w ? Row::whole(w) : 0;
       }
       before = block_scan(mine, sh, all) - mine;
       if (tid == 0)
@@ -418,49 +415,80 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS) sample_kerne
     // Fills the buckets and finds the one in which the measure (elements, or weight) reaches the target,
     // which `target_of` gives from the row's total.
     auto find_bucket = [&](bool weight, auto target_of) {
-      for (int i = tid; i < n; i += SP_THREADS) {
-        const uint32_t key = key_at(i);
-        const int b = bucket_of(key);
-        if (!weight) {
-          atomicAdd(&buckets[b], 1u);
-          continue;
+      if (weight) {
+#pragma unroll 4
+        for (int i = tid; i < n; i += SP_THREADS) {
+          const uint32_t key = key_at(i);
+          const int b = bucket_of(key);
+          const u64 w = rw.fixed(key);
+          if (w) {
+            const uint32_t wl = static_cast<uint32_t>(w), old = atomicAdd(&buckets[b], wl);
+            const uint32_t wh = static_cast<uint32_t>(w >> 32) + (old + wl < old ? 1u : 0u);
+            if (wh)
+              atomicAdd(&buckets[SP_BUCKETS + b], wh);
+          }
         }
-        const u64 w = rw.fixed(key);
-        if (w == 0)
-          continue;
-        const uint32_t wl = static_cast<uint32_t>(w), old = atomicAdd(&buckets[b], wl);
-        const uint32_t wh = static_cast<uint32_t>(w >> 32) + (old + wl < old ? 1u : 0u);
-        if (wh)
-          atomicAdd(&buckets[SP_BUCKETS + b], wh);
+      } else {
+#pragma unroll 4
+        for (int i = tid; i < n; i += SP_THREADS)
+          atomicAdd(&buckets[bucket_of(key_at(i))], 1u);
       }
       cluster.sync();
-      u64 v[4] = {0, 0, 0, 0}, all;
-      uint4 lo[SP_MAX_CLUSTER], hi[SP_MAX_CLUSTER]; // all remote loads before the first sum
+      // Rank r sums up the cluster's buckets [r, r + 1) * SP_BUCKETS / C; the ranks' totals say whose hold the cut.
+      const int share = SP_BUCKETS / C, per_thread = (share + SP_THREADS - 1) / SP_THREADS; // 1 .. 8
+      const int b0 = rank * share + tid * per_thread;
+      u64 v[SP_BUCKETS / SP_THREADS], sum = 0, all;
 #pragma unroll
-      for (int r = 0; r < SP_MAX_CLUSTER; ++r) {
-        lo[r] = hi[r] = make_uint4(0, 0, 0, 0);
-        if (r < C) {
-          const uint32_t *from = cluster.map_shared_rank(buckets, r) + 4 * tid;
-          lo[r] = *reinterpret_cast<const uint4 *>(from);
-          if (weight)
-            hi[r] = *reinterpret_cast<const uint4 *>(from + SP_BUCKETS);
+      for (int j = 0; j < SP_BUCKETS / SP_THREADS; ++j) {
+        v[j] = 0;
+        if (j < per_thread && tid * per_thread + j < share) {
+          uint32_t lo[SP_MAX_CLUSTER], hi[SP_MAX_CLUSTER]; // all remote loads before the first sum
+#pragma unroll
+          for (int r = 0; r < SP_MAX_CLUSTER; ++r) {
+            lo[r] = hi[r] = 0;
+            if (r < C) {
+              const uint32_t *from = cluster.map_shared_rank(buckets, r) + b0 + j;
+              lo[r] = from[0];
+              if (weight)
+                hi[r] = from[SP_BUCKETS];
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < SP_MAX_CLUSTER; ++r)
+            v[j] += lo[r] + (static_cast<u64>(hi[r]) << 32);
         }
+        sum += v[j];
       }
-#pragma unroll
-      for (int r = 0; r < SP_MAX_CLUSTER; ++r) {
-        v[0] += lo[r].x + (static_cast<u64>(hi[r].x) << 32), v[1] += lo[r].y + (static_cast<u64>(hi[r].y) << 32);
-        v[2] += lo[r].z + (static_cast<u64>(hi[r].z) << 32), v[3] += lo[r].w + (static_cast<u64>(hi[r].w) << 32);
-      }
-      const u64 sum = v[0] + v[1] + v[2] + v[3];
       u64 at = block_scan(sum, sh, all) - sum;
-      const u64 target = target_of(all);
+      if (tid == 0)
+        sh.total[total_turn] = all;
+      cluster.sync();
+      u64 whole = 0, lower = 0;
+      for (int r = 0; r < C; ++r) {
+        const u64 t = *cluster.map_shared_rank(&sh.total[total_turn], r);
+        whole += t;
+        if (r < rank)
+          lower += t;
+      }
+      total_turn ^= 1;
+      at += lower;
+      const u64 target = target_of(whole);
       if (at < target && at + sum >= target) {
         int j = 0;
-        while (at + v[j] < target)
-          at += v[j++];
-        sh.bucket = 4 * tid + j, sh.above = at, sh.within = v[j];
+        u64 within = 0;
+#pragma unroll
+        for (int e = 0; e < SP_BUCKETS / SP_THREADS; ++e)
+          if (e == j) {
+            within = v[e];
+            if (at + within < target)
+              at += within, ++j;
+          }
+        for (int r = 0; r < C; ++r) {
+          SampleShared &o = *cluster.map_shared_rank(&sh, r);
+          o.bucket = b0 + j, o.above = at, o.within = within;
+        }
       }
-      __syncthreads();
+      cluster.sync();
       return target;
     };
     // Puts the elements whose bucket passes into rank 0's list; their number over the row.
@@ -604,11 +632,11 @@ template <typename T> int launch_sample_t(SampleArgs a, int rows, int num_sms, c
       return 2;
     once.set(1);
   }
-  // As few CTAs per row as hold it in shared memory; more while the rows alone would leave SMs idle
-  // and a CTA still has a few keys per thread.
+  // As few CTAs per row as leave room for a second one on their SM (or at least hold the row); more while the
+  // rows alone would leave SMs idle and a CTA still has a few keys per thread.
   int C = 1;
-  while (C < SP_MAX_CLUSTER &&
-         ((a.cols + C - 1) / C > SP_SMEM_KEYS || (1ll * rows * C * 2 <= num_sms && a.cols / C > 4 * SP_THREADS)))
+  while (C < SP_MAX_CLUSTER && ((a.cols + C - 1) / C > SP_PAIR_KEYS ||
+                                (1ll * rows * C <= num_sms && a.cols / C > 4 * SP_THREADS)))
     C *= 2;
   a.per_cta = ((a.cols + C - 1) / C + 7) & ~7;
   a.in_smem = a.per_cta <= SP_SMEM_KEYS;
