@@ -1129,7 +1129,7 @@ size_t part_rows(int num_sms, int n_tokens, int B, int G, int D, int dtype) {
 }
 size_t paged_workspace_bytes(int num_sms, int n_tokens, int B, int G, int D, int dtype) {
   return part_rows(num_sms, n_tokens, B, G, D, dtype) * (sizeof(float) * D + sizeof(float2)) +
-         (sizeof(SplitItem) + sizeof(int2)) * num_sms * MAX_WORKERS_PER_SM;
+         (sizeof(SplitItem) + sizeof(int2)) * num_sms * MAX_WORKERS_PER_SM + 64;
 }
 
 // per_cta: workers that a CTA of the join stands for, 1 or JOIN_WARPS; ctas: CTAs that share one worker's rows
@@ -1296,6 +1296,8 @@ int mu_attention_paged(mu_ctx *ctx, const void *q, long long q_ld, void *out, lo
                         "(mu_attention_paged_workspace_bytes)");
   if (mu_ctx_select_device(ctx) != MU_OK)
     return mu_set_error(ctx, MU_ERR_CUDA, "attention_paged: cannot select device");
+  if (num_pages == 0) // every page id is out of range: nothing is read, but addresses are formed
+    k_cache = v_cache = workspace;
   mu::PagedArgs a{};
   a.q = q, a.out = out, a.q_ld = q_ld, a.out_ld = out_ld;
   a.kc = static_cast<const uint8_t *>(k_cache), a.vc = static_cast<const uint8_t *>(v_cache);

@@ -54,7 +54,8 @@ __device__ __forceinline__ Seq load_seq(const PagedArgs &a, int b) {
   }
   if (s.nq * a.G < a.rows_from || s.nq * a.G > a.rows_to)
     s.nq = 0;
-  const long long room = 1ll * a.table_stride * a.page_size;
+  // what the table can address; key numbers a few tiles behind the last one must not leave 31 bits either
+  const long long room = min(1ll * a.table_stride * a.page_size, 1ll * INT_MAX - 65536);
   s.seen = s.len;
   if (s.nq > 0 && s.len > room) {
     atomicCAS(a.status, 0, MU_DEV_BAD_PAGE);

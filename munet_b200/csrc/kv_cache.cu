@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(PM_THREADS) page_map_kernel(PageMapArgs a) {
     if (r >= a.B)
       break;
     const ReqLens q = req_lens(a, r);
-    const int j = f - (page_end[r] - q.new_pages);
+    const int j = f - (r ? page_end[r - 1] : 0); // the sum before r is at most f, so it is not saturated
     int page = f < a.n_free ? a.free_pages[f] : -1;
     if (f < a.n_free && (page < 0 || page >= a.num_pages)) {
       atomicCAS(a.status, 0, MU_DEV_BAD_PAGE);
@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(PM_THREADS) page_map_kernel(PageMapArgs a) {
     if (t < limit) {
       const int r = upper_bound(tok_end, a.B, t);
       const ReqLens q = req_lens(a, r);
-      pos = q.ctx + (t - (tok_end[r] - q.add));
+      pos = q.ctx + (t - (r ? tok_end[r - 1] : 0));
       const int pi = static_cast<int>(static_cast<unsigned>(pos) / ps);
       int page = -1;
       bool known = false;
@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(PM_THREADS) page_map_kernel(PageMapArgs a) {
         page = a.block_table[1ll * r * a.table_stride + pi];
         known = true;
       } else if (pi < q.old_pages + q.new_pages) {
-        const int f = page_end[r] - q.new_pages + (pi - q.old_pages);
+        const long long f = (r ? page_end[r - 1] : 0ll) + (pi - q.old_pages); // saturated: beyond any free list
         if (f < a.n_free)
           page = a.free_pages[f], known = true;
       }
@@ -628,6 +628,8 @@ int mu_kv_cache_append(mu_ctx *ctx, const void *k, const void *v, long long ld, 
     return mu_set_error(ctx, MU_ERR_INVALID, "kv_cache_append: row stride below Hkv * D");
   if (1ll * num_pages * page_size > INT_MAX)
     return mu_set_error(ctx, MU_ERR_SIZE, "kv_cache_append: num_pages * page_size does not fit a 32-bit slot");
+  if ((n_tokens / 16 + 1ll) * 2 * Hkv > INT_MAX)
+    return mu_set_error(ctx, MU_ERR_SIZE, "kv_cache_append: tokens x heads beyond one launch");
   if (n_tokens == 0)
     return MU_OK;
   if (!k || !v || !slots || !k_cache || !v_cache || !k_scale || !v_scale)

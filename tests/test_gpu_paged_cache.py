@@ -119,6 +119,23 @@ def test_page_map_reports_what_does_not_fit(ctx, what, code):
         assert o["qs"].tolist() == [0, 20, 20, 60] and o["seq"].tolist() == [36, 0, 40]
 
 
+def test_page_map_sums_beyond_32_bits(ctx):
+    """Lengths whose sums pass 2^31: what fits the slots is right, the rest is reported."""
+    import munet_b200 as mb
+    big = 2 ** 30
+    table = np.full((4, 2), -1, np.int32)
+    table[0, 0] = 5
+    t, o = run_page_map(ctx, [16, 0, 0, 2 ** 31 - 1], [8, big, big, 5], [7, 6, 4, 3, 2], table, 16, 8, 40)
+    with pytest.raises(mb.MuNetError) as e:
+        ctx.check()
+    assert e.value.code in (5, 6)
+    assert t.tolist() == [[5, 7], [6, 4], [3, 2], [-1, -1]]
+    assert o["slots"].tolist() == [7 * 16 + i for i in range(8)] + [6 * 16 + i for i in range(16)] + [4 * 16 + i for i in range(16)]
+    assert o["pos"].tolist() == [16 + i for i in range(8)] + list(range(32))
+    assert o["qs"].tolist() == [0, 8, 8 + big, 2 ** 31 - 1, 2 ** 31 - 1] and o["taken"][0] == 5
+    assert o["seq"].tolist() == [24, big, big, 0]  # the last request's sum does not fit: it counts as empty
+
+
 # ---- append ---------------------------------------------------------------------------------------
 
 
@@ -456,6 +473,32 @@ def test_attention_bad_pages_and_ranges(ctx):
                 want = ref.attention(pr["qx"], pr["kc"], pr["vc"], pr["ks"].astype(float), pr["vs"].astype(float), t,
                                      pr["qs"], pr2["seq"], 16, True)[0]
                 assert np.abs(got[:4] - want[:4]).max() <= 0.02 * np.abs(want[:4]).max()
+
+
+def test_attention_without_a_pool(ctx):
+    import munet_b200 as mb
+    rng = np.random.default_rng(14)
+    for dtype, D in ((F32, 64), (BF16, 128), (BF16, 40)):
+        pr = make_problem(rng, dtype, 2, 2, 1, D, 16, [20, 3], [1, 1])
+        q, out = pr["q"], pr["q"].clone().fill_(7.0)
+        n = ctx.attention_paged_workspace_bytes(4, 2, 2, 1, D, dtype)
+        ws = dev(np.zeros(n, np.uint8))
+        ctx.attention_paged(q, q.stride(0), out, out.stride(0), None, None, None, None, ints(pr["table"]),
+                            pr["table"].shape[1], ints(pr["qs"]), ints(pr["seq"]), 2, 4, 2, 1, D, 0, 16, True, dtype, ws, n)
+        with pytest.raises(mb.MuNetError) as e:
+            ctx.check()
+        assert e.value.code == 5
+        assert (out[:2] == 0).all() and (out[2:] == 7).all()
+
+
+@pytest.mark.parametrize("B,new", [(5000, 1), (3600, 2), (400, 3)])
+def test_attention_many_requests(ctx, B, new):
+    rng = np.random.default_rng(15)
+    lens = rng.integers(new, 40, B).tolist()
+    pr = make_problem(rng, BF16, B, 2, 1, 64, 16, lens, [new] * B)
+    out = run_attention(ctx, pr, BF16, True, 1, 16)
+    ctx.check()
+    check_attention(pr, out, BF16, True, 16)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])

@@ -48,6 +48,7 @@ REFUSED = [
     (append, dict(page=24), UNSUPPORTED), (append, dict(page=1040), UNSUPPORTED),
     (append, dict(D=264, ld=4096), UNSUPPORTED), (append, dict(dtype=F16), UNSUPPORTED),
     (append, dict(vc=P + 8), INVALID), (append, dict(pages=1 << 27), SIZE),
+    (append, dict(n=1 << 30, H=1024, ld=1 << 20), SIZE),
     (attend, dict(B=-1), INVALID), (attend, dict(Hq=3), INVALID), (attend, dict(q_ld=63), INVALID),
     (attend, dict(out_ld=63), INVALID), (attend, dict(page=8), UNSUPPORTED), (attend, dict(D=257, q_ld=2048), UNSUPPORTED),
     (attend, dict(dtype=F16), UNSUPPORTED), (attend, dict(dtype=3), UNSUPPORTED), (attend, dict(out=None), INVALID),
