@@ -323,7 +323,7 @@ __device__ __forceinline__ double reciprocal(float s) {
   return fma(r, fma(-r, static_cast<double>(s), 1.0), r);
 }
 // What a page held, times held scale / new scale.
-__device__ __forceinline__ void requantise(uint8_t *tile, int bytes, float held, float now, int tid, int team) {
+template <int TEAM> __device__ __forceinline__ void requantise(uint8_t *tile, int bytes, float held, float now, int tid) {
   // the new scale is a power of two, so q * f is exact in float for a held power of two and in double for any other
   const double f = held > 0.f ? static_cast<double>(held) * static_cast<double>(1.f / now) : 0.0;
   const bool pow2 = (__float_as_uint(held) & 0x7fffffu) == 0;
@@ -332,14 +332,25 @@ __device__ __forceinline__ void requantise(uint8_t *tile, int bytes, float held,
     const float2 p = e4m3x2_to_float2(two);
     return pow2 ? e4m3x2(p.x * ff, p.y * ff) : e4m3x2(on_e4m3_grid(p.x * f), on_e4m3_grid(p.y * f));
   };
-  uint32_t *w = reinterpret_cast<uint32_t *>(tile);
+  auto word = [&](uint32_t u) { return again(u & 0xffffu) | (again(u >> 16) << 16); };
+  // 16 bytes a thread; a lone warp has four loads under way (a page of 64 x 128 took it 32 us word by word)
+  constexpr int E = TEAM == 32 ? 4 : 1;
+  uint4 *w = reinterpret_cast<uint4 *>(tile);
+  const int words = bytes / 16;
 #pragma unroll 1
-  for (int k = tid; k < bytes / 4; k += team) {
-    const uint32_t u = w[k];
-    w[k] = again(u & 0xffffu) | (again(u >> 16) << 16);
+  for (int k = tid; k < words; k += E * TEAM) {
+    uint4 u[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (k + e * TEAM < words)
+        u[e] = w[k + e * TEAM];
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (k + e * TEAM < words)
+        w[k + e * TEAM] = make_uint4(word(u[e].x), word(u[e].y), word(u[e].z), word(u[e].w));
   }
 #pragma unroll 1
-  for (int k = (bytes & ~3) + tid; k < bytes; k += team)
+  for (int k = (bytes & ~15) + tid; k < bytes; k += TEAM)
     tile[k] = static_cast<uint8_t>(again(tile[k]) & 0xffu);
 }
 
@@ -356,7 +367,7 @@ __device__ __forceinline__ int next_bit(const uint32_t *bits, int from, int n) {
 }
 
 template <typename T, int VE, int TEAM>
-__global__ void __launch_bounds__(AP_THREADS, VE == 8 ? (sizeof(T) == 2 ? (TEAM == 32 ? 6 : 8) : 5) : 4) kv_append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(AP_THREADS, VE == 8 ? (sizeof(T) == 2 ? (TEAM == 32 ? 4 : 8) : 4) : 4) kv_append_kernel(AppendArgs a) {
   // window of slots: the CTA's tokens and as many as one page holds after them
   extern __shared__ int sm[];
   const int token_block = blockIdx.x / a.unit_blocks, unit_block = blockIdx.x - token_block * a.unit_blocks;
@@ -491,9 +502,8 @@ __global__ void __launch_bounds__(AP_THREADS, VE == 8 ? (sizeof(T) == 2 ? (TEAM 
     const float now = fmaxf(held, page_scale(m));
     if (tid == 0)
       *scale = now;
-    if (low > 0 && now > held) // the tokens before the new ones: low * D bytes from the tile's start
-      requantise(tile, low * a.D, held, now, tid, TEAM);
-    if (ordered && (__float_as_uint(now) & 0x7fffffu) == 0) {
+    const bool fast = ordered && (__float_as_uint(now) & 0x7fffffu) == 0;
+    if (fast) {
       const float inv = 1.f / now;
       at = begin;
 #pragma unroll
@@ -511,7 +521,11 @@ __global__ void __launch_bounds__(AP_THREADS, VE == 8 ? (sizeof(T) == 2 ? (TEAM 
         r.floats(f);
         store_row_vec<VE>(tile + (slot[i + at.row] - page0) * a.D + at.col * VE, f, inv);
       }
-    } else {
+    }
+    // the tokens before the new ones, low * D bytes from the tile's start: now that the rows' registers are free
+    if (low > 0 && now > held)
+      requantise<TEAM>(tile, low * a.D, held, now, tid);
+    if (!fast) {
       const double recip = reciprocal(now);
 #pragma unroll 1
       for (int j = 0; j < n; ++j) {

@@ -28,7 +28,7 @@ namespace cg = cooperative_groups;
 namespace mu {
 
 constexpr int SP_THREADS = 512, SP_WARPS = SP_THREADS / 32, SP_MAX_CLUSTER = 8;
-constexpr int SP_BUCKETS = 4096, SP_LIST = 512, SP_RANKED = 128;
+constexpr int SP_BUCKETS = 4096, SP_LIST = 512, SP_RANKED = 256;
 constexpr float SP_BUCKETS_PER_NAT = 92.3325f; // 64 to a factor of two
 constexpr int SP_SMEM_KEYS = 43008; // keys of one CTA that fit its shared memory beside the buckets (168 KB)
 constexpr int SP_PAIR_KEYS = 15360; // and of one of two CTAs of an SM: one loads while the other computes
@@ -154,6 +154,7 @@ __device__ __forceinline__ void sort_desc(u64 *v, int *ranks, int n) {
     __syncthreads();
     if (from < n) {
       int larger = 0;
+#pragma unroll 8
       for (int j = from; j < from + share; ++j)
         larger += v[j] > x;
       if (larger)
@@ -415,23 +416,30 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS, 2) sample_ke
     // Fills the buckets and finds the one in which the measure (elements, or weight) reaches the target,
     // which `target_of` gives from the row's total.
     auto find_bucket = [&](bool weight, auto target_of) {
-      if (weight) {
-#pragma unroll 4
-        for (int i = tid; i < n; i += SP_THREADS) {
-          const uint32_t key = key_at(i);
-          const int b = bucket_of(key);
-          const u64 w = rw.fixed(key);
-          if (w) {
-            const uint32_t wl = static_cast<uint32_t>(w), old = atomicAdd(&buckets[b], wl);
-            const uint32_t wh = static_cast<uint32_t>(w >> 32) + (old + wl < old ? 1u : 0u);
+      // Four keys and weights at a time before the first addition: to the compiler an atomic may change the keys.
+      constexpr int U = 4;
+      for (int i = tid; i < n; i += U * SP_THREADS) {
+        uint32_t key[U];
+        u64 w[U];
+#pragma unroll
+        for (int e = 0; e < U; ++e)
+          key[e] = i + e * SP_THREADS < n ? key_at(i + e * SP_THREADS) : KEY_NEG_INF;
+#pragma unroll
+        for (int e = 0; e < U; ++e)
+          w[e] = weight ? rw.fixed(key[e]) : 0;
+#pragma unroll
+        for (int e = 0; e < U; ++e) {
+          const int b = bucket_of(key[e]);
+          if (!weight) {
+            if (i + e * SP_THREADS < n)
+              atomicAdd(&buckets[b], 1u);
+          } else if (w[e]) {
+            const uint32_t wl = static_cast<uint32_t>(w[e]), old = atomicAdd(&buckets[b], wl);
+            const uint32_t wh = static_cast<uint32_t>(w[e] >> 32) + (old + wl < old ? 1u : 0u);
             if (wh)
               atomicAdd(&buckets[SP_BUCKETS + b], wh);
           }
         }
-      } else {
-#pragma unroll 4
-        for (int i = tid; i < n; i += SP_THREADS)
-          atomicAdd(&buckets[bucket_of(key_at(i))], 1u);
       }
       cluster.sync();
       // Rank r sums up the cluster's buckets [r, r + 1) * SP_BUCKETS / C; the ranks' totals say whose hold the cut.
@@ -495,13 +503,19 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS, 2) sample_ke
     auto gather = [&](auto passes) {
       int *const count = cluster.map_shared_rank(&sh.n_list, 0);
       u64 *const list = cluster.map_shared_rank(sh.list, 0);
-      for (int i = tid; i < n; i += SP_THREADS) {
-        const uint32_t key = key_at(i);
-        if (passes(bucket_of(key))) {
-          const int at = atomicAdd(count, 1);
-          if (at < SP_LIST)
-            list[at] = static_cast<u64>(key) << 32 | static_cast<uint32_t>(~(s0 + i));
-        }
+      constexpr int U = 8;
+      for (int i = tid; i < n; i += U * SP_THREADS) {
+        uint32_t key[U];
+#pragma unroll
+        for (int e = 0; e < U; ++e)
+          key[e] = i + e * SP_THREADS < n ? key_at(i + e * SP_THREADS) : 0;
+#pragma unroll
+        for (int e = 0; e < U; ++e)
+          if (i + e * SP_THREADS < n && passes(bucket_of(key[e]))) {
+            const int at = atomicAdd(count, 1);
+            if (at < SP_LIST)
+              list[at] = static_cast<u64>(key[e]) << 32 | static_cast<uint32_t>(~(s0 + i + e * SP_THREADS));
+          }
       }
       cluster.sync();
       return *count;
