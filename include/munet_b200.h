@@ -232,8 +232,8 @@ int mu_kv_cache_append(mu_ctx *ctx, const void *k, const void *v, long long ld, 
  * row i of n sees the keys up to position seq_len - n + i; a row that sees none gives zeros. Rows of
  * `out` behind query_start[B] are left as they are. Keys on a page id outside the pool, or beyond
  * table_stride pages, are left out and latch MU_ERR_INDEX; so do contradictory row ranges, whose
- * request is skipped. What lies in a page behind its request's last token is never read as a value. `out`
- * must not overlap q.
+ * request is skipped. What lies in a page behind its request's last token is never read as a value. Scales
+ * from 2^-64 to 2^64 keep every bit of their values (V scales below count as 2^-64). `out` must not overlap q.
  * workspace (16-byte aligned, mu_attention_paged_workspace_bytes) holds pieces of long requests during the
  * call only; calls that may overlap on the GPU need one each. At most MU_ATTENTION_PAGED_MAX_REQUESTS
  * requests. */

@@ -64,7 +64,7 @@ struct TileWalk {
   int workers, me, b;
   bool first;
   __device__ __forceinline__ TileWalk(long long total_, int me_, int grid) : total(total_), me(me_), b(0), first(true) {
-    // a share is never so small that it holds no chunk (16 units, a few more by rounding) of an item
+    // several chunks to a share (16 units each)
     workers = static_cast<int>(min(static_cast<long long>(grid), max(1ll, total / 64)));
     u = end = 0;
     if (me < workers) {
@@ -115,7 +115,9 @@ struct TileWalk {
       };
       g.chunk0 = chunk_at(at);
       g.chunks = chunk_at(to) - g.chunk0;
-      if (g.chunks == 0)
+      // A share without a chunk is a piece all the same behind the item's first one (which the join counts by
+      // workers): the units of a row that a short block table cuts off are more than its chunks.
+      if (g.chunks == 0 && g.chunk0 == 0)
         continue;
       g.slot = -1;
       if (g.chunks < nc) {

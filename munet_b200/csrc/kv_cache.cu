@@ -474,9 +474,9 @@ __global__ void __launch_bounds__(AP_THREADS, VE == 8 ? (sizeof(T) == 2 ? (TEAM 
       m = amax_any<T, VE>(r, m);
     }
     auto team_max = [&](uint32_t mine) {
+      team_sync(); // the held scale has been read by all, and red[] is free
       mine = __reduce_max_sync(~0u, mine);
       if constexpr (TEAM == AP_THREADS) {
-        __syncthreads(); // red[] may still be read
         if ((tid & 31) == 0)
           red[tid >> 5] = mine;
         __syncthreads();

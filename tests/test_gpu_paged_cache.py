@@ -491,6 +491,44 @@ def test_attention_without_a_pool(ctx):
         assert (out[:2] == 0).all() and (out[2:] == 7).all()
 
 
+@pytest.mark.parametrize("D,new", [(64, 64), (128, 200)])
+def test_attention_length_far_beyond_the_table(ctx, D, new):
+    """A prompt chunk whose length says a million keys where the table holds 256: those are attended to, the rest is
+    reported, and no share of the work that turns out to hold no key leaves its place in the workspace unwritten."""
+    import munet_b200 as mb
+    import torch
+    rng = np.random.default_rng(16)
+    pr = make_problem(rng, BF16, 1, 4, 1, D, 16, [256], [new])
+    n = ctx.attention_paged_workspace_bytes(new + 2, 1, 4, 1, D, BF16)
+    ws = torch.full((n,), 0xFF, dtype=torch.uint8, device="cuda")  # NaN, read as numbers
+    out = run_attention(ctx, dict(pr, seq=np.asarray([1_000_000], np.int32)), BF16, True, 1, 16, ws=ws)
+    with pytest.raises(mb.MuNetError) as e:
+        ctx.check()
+    assert e.value.code == 5
+    check_attention(pr, out, BF16, False, 16)
+
+
+def test_attention_two_calls_at_once(ctx):
+    """Calls on two streams, a workspace each, among them prompt chunks and single tokens."""
+    import torch
+    rng = np.random.default_rng(17)
+    a = make_problem(rng, BF16, 3, 8, 2, 128, 16, [1500, 700, 90], [300, 1, 40])
+    b = make_problem(rng, BF16, 3, 8, 2, 128, 16, [2900, 40, 1700], [1, 1, 1])
+    want = [run_attention(ctx, pr, BF16, True, 2, 16).clone() for pr in (a, b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    ws = [torch.full((ctx.attention_paged_workspace_bytes(pr["n"], 3, 8, 2, 128, BF16),), 0xFF, dtype=torch.uint8,
+                     device="cuda") for pr in (a, b)]
+    out = [torch.full_like(w, 7.0) for w in want]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for i, pr in enumerate((a, b)):
+            run_attention(ctx, pr, BF16, True, 2, 16, stream=streams[i], ws=ws[i], out=out[i])
+    torch.cuda.synchronize()
+    ctx.check()
+    assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
 @pytest.mark.parametrize("B,new", [(5000, 1), (3600, 2), (400, 3)])
 def test_attention_many_requests(ctx, B, new):
     rng = np.random.default_rng(15)
