@@ -20,6 +20,7 @@
 #include "../../include/munet_b200.h"
 #include "common.h"
 #include "ptx.cuh"
+#include <cfloat>
 #include <climits>
 #include <cooperative_groups.h>
 
@@ -54,7 +55,7 @@ __device__ __forceinline__ uint32_t to_key(float v) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float from_key(uint32_t k) {
-  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+  return __uint_as_float(k ^ (~static_cast<uint32_t>(static_cast<int>(k) >> 31) | 0x80000000u));
 }
 
 template <typename T> __device__ __forceinline__ float load_logit(const T *p, long long i);
@@ -113,15 +114,14 @@ __device__ __forceinline__ u64 block_scan(u64 v, SampleShared &sh, u64 &all) {
 // |f| <= 1/64: the remainder is below (ln2/64)^6 / 720 = 2.3e-15, a sixteenth of the 2^-43 that rounding to
 // whole multiples of 2^-42 allows for weights near one. exp() cost twice as much.
 struct Row {
-  double c, minus; // t = x * c + minus
+  double max, c; // t = (x - max) * c, exactly 0 for the maximum
   const double *table;
-  uint32_t max_key;
-  // No branches, so that several run at a time. What has no t counts as zero: -inf, and next to a maximum of
-  // +inf everything but the elements equal to it.
+  uint32_t floor_key; // below it t is under -64 (the weight under 2^-43), or there is no t: -inf, and next to a
+                      // maximum of +inf everything else
+  // No branches, so that several run at a time.
   __device__ __forceinline__ double weight(uint32_t key) const {
-    const double t0 = fma(static_cast<double>(from_key(key)), c, minus);
-    const bool some = t0 > -64.0; // below: 2^-43 or less
-    const double t = some ? t0 : -64.0;
+    const double t0 = (static_cast<double>(fminf(from_key(key), FLT_MAX)) - max) * c;
+    const double t = key >= floor_key ? t0 : -64.0;
     const double shift = 0x1.8p52 / 32; // adding it rounds t to a multiple of 1/32
     const double r = t + shift;
     const int i = __double2loint(r);
@@ -131,8 +131,7 @@ struct Row {
     p = fma(f, p, 0x1.ebfbdff82c58fp-3);
     p = fma(f, p, 0x1.62e42fefa39efp-1);
     p = fma(f, p, 1.0) * table[i & 31];
-    const double w = __hiloint2double(__double2hiint(p) + ((i >> 5) << 20), __double2loint(p));
-    return key == max_key ? 1.0 : some ? w : 0.0;
+    return __hiloint2double(__double2hiint(p) + ((i >> 5) << 20), __double2loint(p));
   }
   // rounded to a multiple of 2^-42, as that multiple
   __device__ __forceinline__ static u64 whole(double w) {
@@ -302,10 +301,13 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS, 2) sample_ke
     }
   } else {
     Row rw;
-    rw.max_key = top;
     const float xmax = from_key(top);
     rw.table = sh.table;
-    rw.c = 1.4426950408889634 / static_cast<double>(T_row), rw.minus = -static_cast<double>(xmax) * rw.c;
+    rw.max = static_cast<double>(fminf(xmax, FLT_MAX)), rw.c = 1.4426950408889634 / static_cast<double>(T_row);
+    // rounded to a float, which moves t by no more than from -64 to -128
+    rw.floor_key = xmax > FLT_MAX ? top
+                                  : max(to_key(static_cast<float>(rw.max - 44.3614195558365 * static_cast<double>(T_row))),
+                                        KEY_NEG_INF + 1);
     // kept: key > bound_key, or equal to it at an index up to bound_idx
     uint32_t bound_key = 0;
     int bound_idx = INT_MAX;
@@ -384,15 +386,8 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS, 2) sample_ke
       const int at = t < ties ? nth_equal(prefix, t) : bound_key == prefix ? bound_idx : INT_MAX;
       bound_key = prefix, bound_idx = at;
     };
-    auto weight_of_kept = [&](double floor_w, u64 &mine, u64 &before) { // sum over the row
-      mine = 0;
+    auto row_sum = [&](u64 mine, u64 &before) { // over the row, and over the threads before this one
       u64 all;
-#pragma unroll 4
-      for (int i = i0; i < i1; ++i) {
-        const uint32_t k = key_at(i);
-        const double w = rw.weight(k);
-        mine += kept(k, i) && w >= floor_w ? Row::whole(w) : 0;
-      }
       before = block_scan(mine, sh, all) - mine;
       if (tid == 0)
         sh.total[total_turn] = all;
@@ -406,6 +401,16 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS, 2) sample_ke
       }
       total_turn ^= 1;
       return sum;
+    };
+    auto weight_of_kept = [&](double floor_w, u64 &mine, u64 &before) {
+      mine = 0;
+#pragma unroll 4
+      for (int i = i0; i < i1; ++i) {
+        const uint32_t k = key_at(i);
+        const double w = rw.weight(k);
+        mine += kept(k, i) && w >= floor_w ? Row::whole(w) : 0;
+      }
+      return row_sum(mine, before);
     };
 
     const int k = a.top_k ? a.top_k[row] : 0;
@@ -499,10 +504,17 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS, 2) sample_ke
       cluster.sync();
       return target;
     };
-    // Puts the elements whose bucket passes into rank 0's list; their number over the row.
-    auto gather = [&](auto passes) {
-      int *const count = cluster.map_shared_rank(&sh.n_list, 0);
-      u64 *const list = cluster.map_shared_rank(sh.list, 0);
+    auto to_list = [&](uint32_t key, int i) { // rank 0's
+      const int at = atomicAdd(cluster.map_shared_rank(&sh.n_list, 0), 1);
+      if (at < SP_LIST)
+        cluster.map_shared_rank(sh.list, 0)[at] = static_cast<u64>(key) << 32 | static_cast<uint32_t>(~(s0 + i));
+    };
+    auto list_length = [&] {
+      cluster.sync();
+      return *cluster.map_shared_rank(&sh.n_list, 0);
+    };
+    // Puts the elements down to bucket `last` into the list; their number over the row.
+    auto gather = [&](int last) {
       constexpr int U = 8;
       for (int i = tid; i < n; i += U * SP_THREADS) {
         uint32_t key[U];
@@ -511,14 +523,10 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS, 2) sample_ke
           key[e] = i + e * SP_THREADS < n ? key_at(i + e * SP_THREADS) : 0;
 #pragma unroll
         for (int e = 0; e < U; ++e)
-          if (i + e * SP_THREADS < n && passes(bucket_of(key[e]))) {
-            const int at = atomicAdd(count, 1);
-            if (at < SP_LIST)
-              list[at] = static_cast<u64>(key[e]) << 32 | static_cast<uint32_t>(~(s0 + i + e * SP_THREADS));
-          }
+          if (i + e * SP_THREADS < n && bucket_of(key[e]) <= last)
+            to_list(key[e], i + e * SP_THREADS);
       }
-      cluster.sync();
-      return *count;
+      return list_length();
     };
     // rank 0: the list in descending order (largest key, then lowest index), one element to a thread
     auto sorted = [&](int count) {
@@ -545,7 +553,7 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS, 2) sample_ke
       find_bucket(false, [&](u64) { return static_cast<u64>(k); });
       const int last = sh.bucket;
       // elements down to the cut's bucket: the list has room, or nobody gathers
-      const int count = sh.above + sh.within <= SP_LIST ? gather([&](int b) { return b <= last; }) : SP_LIST + 1;
+      const int count = sh.above + sh.within <= SP_LIST ? gather(last) : SP_LIST + 1;
       if (count <= SP_LIST) {
         if (rank == 0) {
           const u64 e = sorted(count);
@@ -582,21 +590,36 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS, 2) sample_ke
       }
       cut(k, false);
     }
-    u64 mine, before;
+    const double floor_w = mp > 0.f ? static_cast<double>(mp) : 0.0;
+    u64 mine = 0, before, all = 0;
+    bool summed = false;
     if (p < 1.f) {
-      bool done = false;
       if (!by_count) {
         const u64 target = find_bucket(true, share_of);
         const int last = sh.bucket;
         const u64 above = sh.above;
-        const int count = gather([&](int b) { return b == last; });
+        // One pass sums up what lies above the cut's bucket and puts that bucket's elements into the list;
+        // which of those are kept is added when the list is sorted. Bit b: some element i0 + b + 64 m is one.
+        u64 open = 0;
+#pragma unroll 4
+        for (int i = i0; i < i1; ++i) {
+          const uint32_t key = key_at(i);
+          const int b = bucket_of(key);
+          const double w = rw.weight(key);
+          mine += b < last && w >= floor_w ? Row::whole(w) : 0;
+          if (b == last) {
+            open |= 1ull << ((i - i0) & 63);
+            to_list(key, i);
+          }
+        }
+        const int count = list_length();
         if (count <= SP_LIST) {
-          done = true;
+          summed = true;
           if (rank == 0) {
             const u64 e = sorted(count);
             const u64 w = tid < count ? rw.fixed(static_cast<uint32_t>(e >> 32)) : 0;
-            u64 all;
-            const u64 ahead = above + block_scan(w, sh, all) - w;
+            u64 sum;
+            const u64 ahead = above + block_scan(w, sh, sum) - w;
             // the last of those before which less than the target lies
             if (tid < count && ahead < target && (ahead + w >= target || tid == count - 1))
               for (int r = 0; r < C; ++r) {
@@ -606,32 +629,52 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS, 2) sample_ke
           }
           cluster.sync();
           bound_key = sh.bound_key, bound_idx = sh.bound_idx;
+          for (; open; open &= open - 1)
+            for (int i = i0 + __ffsll(static_cast<long long>(open)) - 1; i < i1; i += 64) {
+              const uint32_t key = key_at(i);
+              const double w = rw.weight(key);
+              mine += bucket_of(key) == last && kept(key, i) && w >= floor_w ? Row::whole(w) : 0;
+            }
+          all = row_sum(mine, before);
         }
       }
-      if (!done)
+      if (!summed)
         cut(share_of(weight_of_kept(0.0, mine, before)), true);
     }
-    const double floor_w = mp > 0.f ? static_cast<double>(mp) : 0.0;
-    const u64 all = weight_of_kept(floor_w, mine, before);
+    if (!summed)
+      all = weight_of_kept(floor_w, mine, before);
+    cluster.barrier_arrive(); // what follows reads nobody else's shared memory
     const u64 want = draw(all);
-    if (before <= want && want < before + mine) {
-      u64 c = before;
-      for (int i = i0; i < i1; ++i) {
-        const uint32_t key = key_at(i);
-        if (!kept(key, i))
-          continue;
-        const double w = rw.weight(key);
-        if (w < floor_w)
-          continue;
-        c += Row::whole(w);
-        if (c > want) {
-          a.idx[row] = s0 + i;
-          if (a.prob)
-            a.prob[row] = static_cast<float>(w * SP_ONE / static_cast<double>(all));
+    // the warp of the thread whose elements hold the drawn one walks through them
+    const unsigned who = __ballot_sync(~0u, before <= want && want < before + mine);
+    if (who) {
+      const int from = __ffs(who) - 1, j0 = __shfl_sync(~0u, i0, from), j1 = __shfl_sync(~0u, i1, from);
+      u64 c = __shfl_sync(~0u, before, from);
+      for (int j = j0; j < j1; j += 32) {
+        const int i = j + lane;
+        const uint32_t key = i < j1 ? key_at(i) : 0;
+        const double w = i < j1 ? rw.weight(key) : 0.0;
+        u64 inc = i < j1 && kept(key, i) && w >= floor_w ? Row::whole(w) : 0;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const u64 t = __shfl_up_sync(~0u, inc, d);
+          if (lane >= d)
+            inc += t;
+        }
+        const unsigned over = __ballot_sync(~0u, c + inc > want);
+        if (over) {
+          if (lane == __ffs(over) - 1) {
+            a.idx[row] = s0 + i;
+            if (a.prob)
+              a.prob[row] = static_cast<float>(w * SP_ONE / static_cast<double>(all));
+          }
           break;
         }
+        c += __shfl_sync(~0u, inc, 31);
       }
     }
+    cluster.barrier_wait();
+    return;
   }
   cluster.sync(); // nobody leaves while its shared memory may be read
 }
