@@ -115,10 +115,23 @@ struct TileWalk {
       };
       g.chunk0 = chunk_at(at);
       g.chunks = chunk_at(to) - g.chunk0;
-      // A share without a chunk is a piece all the same behind the item's first one (which the join counts by
-      // workers): the units of a row that a short block table cuts off are more than its chunks.
-      if (g.chunks == 0 && g.chunk0 == 0)
+      // the first chunk lies with whoever holds the last unit before it is complete
+      auto beginner = [&] { return owner(item0 + PT_START + (cost - PT_START + nc - 1) / nc - 1); };
+      if (g.chunks == 0) {
+        // A request that a short block table cuts off has more units than chunks: a share in its middle can hold
+        // none, but the join counts pieces by workers, so it leaves an empty one.
+        if (leader && g.chunk0 > 0) {
+          a.notes[me].y = beginner();
+          const long long pr = 2ll * me * a.rows_per_tile;
+#pragma unroll 1
+          for (int r = 0; r < g.n_rows; ++r)
+            a.part_ml[pr + r] = make_float2(-INFINITY, 0.f);
+#pragma unroll 1
+          for (int e = 0; e < g.n_rows * a.D; e += 4)
+            *reinterpret_cast<float4 *>(a.part_o + pr * a.D + e) = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
         continue;
+      }
       g.slot = -1;
       if (g.chunks < nc) {
         g.slot = 2 * me + (first ? 0 : 1);
@@ -127,8 +140,8 @@ struct TileWalk {
           it.first_slot = g.slot, it.last = owner(item0 + cost - 1);
           it.row0 = g.row0, it.n_rows = g.n_rows, it.q0 = s.q0, it.head = g.head;
           a.items[me] = it, a.notes[me].x = g.n_rows;
-        } else if (leader) { // the first chunk lies with whoever holds the last unit before it is complete
-          a.notes[me].y = owner(item0 + PT_START + (cost - PT_START + nc - 1) / nc - 1);
+        } else if (leader) {
+          a.notes[me].y = beginner();
         }
       }
       first = false;
