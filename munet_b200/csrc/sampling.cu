@@ -22,6 +22,7 @@
 #include "ptx.cuh"
 #include <cfloat>
 #include <climits>
+#include <type_traits>
 #include <cooperative_groups.h>
 
 namespace cg = cooperative_groups;
@@ -418,11 +419,12 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS, 2) sample_ke
     const int k = a.top_k ? a.top_k[row] : 0;
     const float p = a.top_p ? a.top_p[row] : 1.f;
     const bool by_count = k > 0 && k < a.cols;
-    const float per_unit = by_count ? SP_BUCKETS_PER_NAT : 2.f * SP_BUCKETS_PER_NAT / T_row;
+    float per_unit = by_count ? SP_BUCKETS_PER_NAT : 2.f * SP_BUCKETS_PER_NAT / T_row;
     auto bucket_of = [&](uint32_t key) { return min(SP_BUCKETS - 1, static_cast<int>((xmax - from_key(key)) * per_unit)); };
     // Fills the buckets and finds the one in which the measure (elements, or weight) reaches the target,
     // which `target_of` gives from the row's total.
-    auto find_bucket = [&](bool weight, auto target_of) {
+    // `filtered`: kept elements only.
+    auto find_bucket = [&](bool weight, auto filtered, auto target_of) {
       // Four keys and weights at a time before the first addition: to the compiler an atomic may change the keys.
       constexpr int U = 4;
       for (int i = tid; i < n; i += U * SP_THREADS) {
@@ -433,7 +435,7 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS, 2) sample_ke
           key[e] = i + e * SP_THREADS < n ? key_at(i + e * SP_THREADS) : KEY_NEG_INF;
 #pragma unroll
         for (int e = 0; e < U; ++e)
-          w[e] = weight ? rw.fixed(key[e]) : 0;
+          w[e] = weight && (!decltype(filtered)::value || kept(key[e], i + e * SP_THREADS)) ? rw.fixed(key[e]) : 0;
 #pragma unroll
         for (int e = 0; e < U; ++e) {
           const int b = bucket_of(key[e]);
@@ -515,8 +517,8 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS, 2) sample_ke
       cluster.sync();
       return *cluster.map_shared_rank(&sh.n_list, 0);
     };
-    // Puts the elements down to bucket `last` into the list; their number over the row.
-    auto gather = [&](int last) {
+    // Puts the elements of buckets first .. last into the list; their number over the row.
+    auto gather = [&](int first, int last) {
       constexpr int U = 8;
       for (int i = tid; i < n; i += U * SP_THREADS) {
         uint32_t key[U];
@@ -525,7 +527,7 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS, 2) sample_ke
           key[e] = i + e * SP_THREADS < n ? key_at(i + e * SP_THREADS) : 0;
 #pragma unroll
         for (int e = 0; e < U; ++e)
-          if (i + e * SP_THREADS < n && bucket_of(key[e]) <= last)
+          if (const int b = bucket_of(key[e]); i + e * SP_THREADS < n && b >= first && b <= last)
             to_list(key[e], i + e * SP_THREADS);
       }
       return list_length();
@@ -540,6 +542,22 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS, 2) sample_ke
       sort_desc(sh.list, sh.ranks, m);
       return tid < count ? sh.list[tid] : 0ull;
     };
+    // The bound: of the list's elements the last one before which less than the target lies.
+    auto bound_in_list = [&](int count, u64 above, u64 target, bool weight) {
+      if (rank == 0) {
+        const u64 e = sorted(count);
+        const u64 w = tid >= count ? 0 : weight ? rw.fixed(static_cast<uint32_t>(e >> 32)) : 1;
+        u64 sum;
+        const u64 ahead = above + block_scan(w, sh, sum) - w;
+        if (tid < count && ahead < target && (ahead + w >= target || tid == count - 1))
+          for (int r = 0; r < C; ++r) {
+            *cluster.map_shared_rank(&sh.bound_key, r) = static_cast<uint32_t>(e >> 32);
+            *cluster.map_shared_rank(&sh.bound_idx, r) = static_cast<int>(~static_cast<uint32_t>(e));
+          }
+      }
+      cluster.sync();
+      bound_key = sh.bound_key, bound_idx = sh.bound_idx;
+    };
     const float mp = a.min_p && a.min_p[row] > 0.f ? fminf(a.min_p[row], 1.f) : 0.f;
     const float u = a.u[row];
     auto draw = [&](u64 all) { // the whole weight that lies before the drawn token's end
@@ -552,10 +570,10 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS, 2) sample_ke
     };
 
     if (by_count) {
-      find_bucket(false, [&](u64) { return static_cast<u64>(k); });
+      find_bucket(false, std::false_type{}, [&](u64) { return static_cast<u64>(k); });
       const int last = sh.bucket;
       // elements down to the cut's bucket: the list has room, or nobody gathers
-      const int count = sh.above + sh.within <= SP_LIST ? gather(last) : SP_LIST + 1;
+      const int count = sh.above + sh.within <= SP_LIST ? gather(0, last) : SP_LIST + 1;
       if (count <= SP_LIST) {
         if (rank == 0) {
           const u64 e = sorted(count);
@@ -590,56 +608,60 @@ template <typename T> __global__ void __launch_bounds__(SP_THREADS, 2) sample_ke
         cluster.sync();
         return;
       }
-      cut(k, false);
+      if (sh.within <= SP_LIST) // a large k: the cut's bucket alone
+        bound_in_list(gather(last, last), sh.above, k, false);
+      else
+        cut(k, false);
+      // Everybody has passed a cluster.sync() since reading them: buckets and list start afresh for top-p.
+      if (p < 1.f) {
+        for (int i = tid; i < 2 * SP_BUCKETS / 4; i += SP_THREADS)
+          reinterpret_cast<uint4 *>(buckets)[i] = make_uint4(0, 0, 0, 0);
+        if (tid == 0)
+          sh.n_list = 0;
+        per_unit = 2.f * SP_BUCKETS_PER_NAT / T_row;
+        __syncthreads();
+      }
     }
     const double floor_w = mp > 0.f ? static_cast<double>(mp) : 0.0;
     u64 mine = 0, before, all = 0;
     bool summed = false;
-    if (p < 1.f) {
-      if (!by_count) {
-        const u64 target = find_bucket(true, share_of);
-        const int last = sh.bucket;
-        const u64 above = sh.above;
-        // One pass sums up what lies above the cut's bucket and puts that bucket's elements into the list;
-        // which of those are kept is added when the list is sorted. Bit b: some element i0 + b + 64 m is one.
-        u64 open = 0;
+    auto top_p = [&](auto filtered) {
+      const u64 target = find_bucket(true, filtered, share_of);
+      const int last = sh.bucket;
+      const u64 above = sh.above;
+      // One pass sums up what lies above the cut's bucket and puts that bucket's elements into the list;
+      // which of those are kept is added when the list is sorted. Bit b: some element i0 + b + 64 m is one.
+      u64 open = 0;
 #pragma unroll 4
-        for (int i = i0; i < i1; ++i) {
-          const uint32_t key = key_at(i);
-          const int b = bucket_of(key);
-          const double w = rw.weight(key);
-          mine += b < last && w >= floor_w ? Row::whole(w) : 0;
-          if (b == last) {
-            open |= 1ull << ((i - i0) & 63);
-            to_list(key, i);
-          }
-        }
-        const int count = list_length();
-        if (count <= SP_LIST) {
-          summed = true;
-          if (rank == 0) {
-            const u64 e = sorted(count);
-            const u64 w = tid < count ? rw.fixed(static_cast<uint32_t>(e >> 32)) : 0;
-            u64 sum;
-            const u64 ahead = above + block_scan(w, sh, sum) - w;
-            // the last of those before which less than the target lies
-            if (tid < count && ahead < target && (ahead + w >= target || tid == count - 1))
-              for (int r = 0; r < C; ++r) {
-                *cluster.map_shared_rank(&sh.bound_key, r) = static_cast<uint32_t>(e >> 32);
-                *cluster.map_shared_rank(&sh.bound_idx, r) = static_cast<int>(~static_cast<uint32_t>(e));
-              }
-          }
-          cluster.sync();
-          bound_key = sh.bound_key, bound_idx = sh.bound_idx;
-          for (; open; open &= open - 1)
-            for (int i = i0 + __ffsll(static_cast<long long>(open)) - 1; i < i1; i += 64) {
-              const uint32_t key = key_at(i);
-              const double w = rw.weight(key);
-              mine += bucket_of(key) == last && kept(key, i) && w >= floor_w ? Row::whole(w) : 0;
-            }
-          all = row_sum(mine, before);
+      for (int i = i0; i < i1; ++i) {
+        const uint32_t key = key_at(i);
+        const int b = bucket_of(key);
+        const double w = rw.weight(key);
+        const bool in = !decltype(filtered)::value || kept(key, i);
+        mine += in && b < last && w >= floor_w ? Row::whole(w) : 0;
+        if (in && b == last) {
+          open |= 1ull << ((i - i0) & 63);
+          to_list(key, i);
         }
       }
+      const int count = list_length();
+      if (count > SP_LIST)
+        return;
+      summed = true;
+      bound_in_list(count, above, target, true);
+      for (; open; open &= open - 1)
+        for (int i = i0 + __ffsll(static_cast<long long>(open)) - 1; i < i1; i += 64) {
+          const uint32_t key = key_at(i);
+          const double w = rw.weight(key);
+          mine += bucket_of(key) == last && kept(key, i) && w >= floor_w ? Row::whole(w) : 0;
+        }
+      all = row_sum(mine, before);
+    };
+    if (p < 1.f) {
+      if (by_count)
+        top_p(std::true_type{});
+      else
+        top_p(std::false_type{});
       if (!summed)
         cut(share_of(weight_of_kept(0.0, mine, before)), true);
     }
