@@ -144,7 +144,8 @@ struct Row {
 };
 
 // Sorts v[0 .. n) in descending order; n a power of two up to SP_THREADS, non-zero values distinct. Short lists
-// by counting what is larger than each (all threads share that, three barriers), others by bitonic merges.
+// by counting what is larger than each (all threads share that, three barriers); others in runs of 32 within a warp's
+// registers, then run by run: an element goes where its place in its own run and that in the other say.
 __device__ __forceinline__ void sort_desc(u64 *v, int *ranks, int n) {
   const int i = threadIdx.x;
   __syncthreads();
@@ -170,16 +171,35 @@ __device__ __forceinline__ void sort_desc(u64 *v, int *ranks, int n) {
     if (i < n && x)
       v[at] = x;
   } else {
-    for (int k = 2; k <= n; k <<= 1)
+    u64 x = i < n ? v[i] : 0;
+#pragma unroll
+    for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
       for (int j = k >> 1; j > 0; j >>= 1) {
-        const int o = i ^ j;
-        if (i < n && o > i) {
-          const u64 x = v[i], y = v[o];
-          if ((x < y) == ((i & k) == 0))
-            v[i] = y, v[o] = x;
-        }
-        __syncthreads();
+        const u64 y = __shfl_xor_sync(~0u, x, j);
+        x = ((i & j) == 0) == ((i & k & 31) == 0) ? max(x, y) : min(x, y);
       }
+    if (i < n)
+      v[i] = x;
+#pragma unroll 1
+    for (int length = 32; length < n; length <<= 1) {
+      __syncthreads();
+      int at = i & (length - 1);
+      x = i < n ? v[i] : 0;
+      if (i < n) { // how many of the other run come first: with equal ones (zeros) the first run's do
+        const bool second = i & length;
+        const u64 *other = v + ((i & -length) ^ length);
+        int lo = 0;
+#pragma unroll 1
+        for (int step = length; step > 0; step >>= 1)
+          if (lo + step <= length && (second ? other[lo + step - 1] >= x : other[lo + step - 1] > x))
+            lo += step;
+        at += lo + (i & -(2 * length));
+      }
+      __syncthreads();
+      if (i < n)
+        v[at] = x;
+    }
   }
   __syncthreads();
 }
