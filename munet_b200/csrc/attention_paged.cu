@@ -134,7 +134,8 @@ template <int R, int CHUNK> struct Walk {
 // ---- CUDA-core kernel: head sizes that are no multiple of 16 ---------------------------------------
 // float32 products and sums. Per warp a tile of 32 keys: for the scores a lane owns a key (its row is D
 // consecutive bytes), for the weighted values a lane owns four dimensions (one, where D is odd).
-// VB: bytes per load (4 or 1 by the head size), RT rows share every key, NA units per lane.
+// VB: bytes per load (4 or 1 by the head size), RT rows share every key, NA units per lane. Bound by the conversion
+// and fp32 products: 32 requests of 2048 keys, 8 heads of 100, bfloat16: 80 us (105 MB: 1.3 TB/s); of 40: 33 us.
 constexpr int SIMT_WARPS = 4, SIMT_THREADS = 32 * SIMT_WARPS, SIMT_CHUNK = 32 * SIMT_WARPS;
 
 __device__ __forceinline__ float2 fp8x2_to_float2(uint32_t two) {
@@ -358,7 +359,8 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_paged_simt_kernel(Page
 }
 
 // ---- tensor-core kernel: head sizes that are multiples of 16 ----------------------------------------
-// Bound by reading the cache. A warp walks its keys in tiles (32 of them, 16 for head sizes above 128),
+// Bound by reading the cache (64 requests of up to 2048 keys, 16 heads of 128: 311 MB in 66 us with the join,
+// 4.7 TB/s; 7 TB/s between the first tile and the first warp's end). A warp walks its keys in tiles (32 of them, 16 for head sizes above 128),
 // copies a tile's K and V bytes into its own two stages of shared memory (cp.async, 16 bytes a lane),
 // turns them into fp16 in registers and multiplies with mma.m16n8k16. Where requests x KV heads are many,
 // a warp is a worker of its own and nothing ever synchronises the CTA (TEAM 1). Where they are few, every
@@ -945,8 +947,8 @@ __global__ void __launch_bounds__(MmaCfg<DP, NR, TEAM, sizeof(T) == 4>::THREADS,
 // ---- joining the pieces ---------------------------------------------------------------------------
 // The rows of an item with P pieces are dealt out to the first P workers that have a piece of it, so that
 // one long request is not joined in one place; a CTA stands for one worker of the main kernel or for four.
-// Time here is latency (note -> item -> maxima ->
-// rows), so every step loads all it needs at once. Launched so that it may become resident while the main
+// Time here is latency (note -> item -> maxima -> rows; 3 to 4 us behind a decode step of 64 requests), so every
+// step loads all it needs at once. Launched so that it may become resident while the main
 // kernel drains; griddepcontrol.wait orders its reads after that kernel's writes.
 constexpr int JOIN_THREADS = 128, JOIN_WARPS = JOIN_THREADS / 32, JOIN_DIMS = 8; // dimensions per lane: D <= 256
 
@@ -1117,8 +1119,8 @@ constexpr int MAX_WORKERS_PER_SM = 12;
 constexpr int MAX_PART_ROWS_PER_SM = 2 * 128;
 // Requests with this many rows (new tokens x heads of a group) or more go to the prompt-chunk kernel: below, a
 // tile of 256 rows would be mostly empty, and reading the keys once per 16 rows costs less (8 requests of 4096
-// keys, 4 KV heads of 128: 64 rows 45 us against 69, 128 rows 81 against 64).
-constexpr int TILE_KERNEL_ROWS = 97;
+// keys, 4 KV heads of 128: 64 rows 45 us against 50, 96 rows 67 against 52, 128 rows 82 against 54).
+constexpr int TILE_KERNEL_ROWS = 81;
 bool uses_tile_kernel(int n_tokens, int B, int G, int D, int dtype) {
   return dtype == BF16 && (D == 64 || D == 128) && n_tokens > B && B <= MU_PAGED_TILE_MAX_REQUESTS &&
          1ll * n_tokens * G >= TILE_KERNEL_ROWS;

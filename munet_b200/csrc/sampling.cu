@@ -12,11 +12,16 @@
 // One cluster of 1, 2, 4 or 8 CTAs per row; each CTA keeps its slab of the row in shared memory as
 // order-preserving 32-bit keys, so HBM sees a row once and every later pass runs on chip.
 //
-// Where a cut falls is found in two steps: a histogram over 4096 buckets of the logits (1/64 of a factor
-// of two wide, from the maximum down: a monotone function, so buckets are ranges of the order) says in
-// which bucket, and that bucket's few elements are sorted. With top-k everything down to the cut goes into
-// the list, which then settles top-p, min-p and the draw as well. Rows whose bucket holds more than a list
-// (ties, logits of another scale) are cut eight bits of the key at a time.
+// Where a cut falls is found in two steps: a histogram over 4096 buckets of the logits (1/64 or 1/128
+// of a factor of two wide, from the maximum down: a monotone function, so buckets are ranges of the order) says
+// in which bucket, and that bucket's few elements are sorted. With a top-k of a few hundred at most everything
+// down to the cut goes into the list, which then settles top-p, min-p and the draw as well; a larger one is cut
+// by its bucket alone, and top-p then goes through the kept elements' buckets. Rows whose bucket holds more than
+// a list (ties, logits of another scale) are cut eight bits of the key at a time.
+//
+// A small batch is latency: one row of 32000 bfloat16 logits with top-k 50 takes 12 us over six cluster barriers.
+// A large one is bound by the instructions of the exact weights, formed twice, and by barriers: 256 rows of 100003
+// float32 logits with top-p 0.97 take 258 us (102 MB), 200 rows in bfloat16 with neither top-k nor top-p 94 us.
 #include "../../include/munet_b200.h"
 #include "common.h"
 #include "ptx.cuh"
