@@ -478,8 +478,10 @@ __global__ void __launch_bounds__(MmaCfg<DP, NR, TEAM, sizeof(T) == 4>::THREADS,
     a.notes[me] = make_int2(0, -1);
   __syncwarp();
   const long long total = scan_units<Cfg::THREADS, R, Cfg::CHUNK>(a, upto, warp_sum);
-  if (total == 0)
+  if (total == 0) {
+    asm volatile("griddepcontrol.wait;" ::: "memory"); // see the end
     return;
+  }
   Walk<R, Cfg::CHUNK> walk(total, me, gridDim.x * (Cfg::WARPS / TEAM));
   const int D = a.D;
   // The walk as a stream of batches: up to 32 half tiles of one segment, whose pages and scales the lanes
@@ -942,6 +944,9 @@ __global__ void __launch_bounds__(MmaCfg<DP, NR, TEAM, sizeof(T) == 4>::THREADS,
     cur = nxt, more = more_after;
   }
   cp_async_wait<0>();
+  // Behind the prompt-chunk kernel this one starts while that drains and reads nothing of it; the join, which waits for
+  // this grid, needs both.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // ---- joining the pieces ---------------------------------------------------------------------------
@@ -971,7 +976,7 @@ __device__ __forceinline__ Joined join_pieces(const PagedArgs &a, const SplitIte
   auto row_of = [&](int i) { return 1ll * (i == 0 ? it.first_slot : 2 * (owner + i)) * a.rows_per_tile + r; };
   for (int p0 = first; p0 < pieces; p0 += 32 * step) {
     const int mine = p0 + lane * step;
-    const float2 ml = mine < pieces ? a.part_ml[row_of(mine)] : make_float2(-INFINITY, 0.f);
+    const float2 ml = mine < pieces ? __ldcg(a.part_ml + row_of(mine)) : make_float2(-INFINITY, 0.f);
     float top = fmaxf(ml.x, j.M);
 #pragma unroll
     for (int d = 16; d; d >>= 1)
@@ -996,13 +1001,13 @@ __device__ __forceinline__ Joined join_pieces(const PagedArgs &a, const SplitIte
 #pragma unroll
           for (int v = 0; v < V; v += 4) {
             const int d = join_dim(a.D, lane, v);
-            const float4 q = d < a.D ? *reinterpret_cast<const float4 *>(src + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float4 q = d < a.D ? __ldcg(reinterpret_cast<const float4 *>(src + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
             x[e][v] = q.x, x[e][v + 1] = q.y, x[e][v + 2] = q.z, x[e][v + 3] = q.w;
           }
         } else {
 #pragma unroll
           for (int v = 0; v < V; ++v)
-            x[e][v] = lane + 32 * v < a.D ? src[lane + 32 * v] : 0.f;
+            x[e][v] = lane + 32 * v < a.D ? __ldcg(src + lane + 32 * v) : 0.f;
         }
       }
 #pragma unroll
@@ -1029,12 +1034,25 @@ __device__ __forceinline__ Joined join_pieces(const PagedArgs &a, const SplitIte
   return j;
 }
 
+// The workers of one main kernel: a CTA of the join stands for `per_cta` of them (1 or JOIN_WARPS), `ctas` CTAs share
+// the rows of one.
+struct JoinShare {
+  int workers, per_cta, ctas; // one of the last two is 1
+  int blocks() const { return (workers + per_cta - 1) / per_cta * ctas; }
+};
+// CTA (bx, by) of the join
 template <typename T>
-__global__ void __launch_bounds__(JOIN_THREADS) attention_paged_join_kernel(PagedArgs a, int workers, int per_cta) {
+__device__ __forceinline__ void join_rows(const PagedArgs &a, int workers, int per_cta, int ctas, int bx, int by) {
   __shared__ float red_o[JOIN_WARPS][32 * JOIN_DIMS];
   __shared__ float2 red_ml[JOIN_WARPS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  auto note_of = [&](int w) { return __ldcg(a.notes + w); };
+  auto item_of = [&](int w) {
+    const int2 *p = reinterpret_cast<const int2 *>(a.items + w);
+    const int2 x = __ldcg(p), y = __ldcg(p + 1), z = __ldcg(p + 2);
+    return SplitItem{x.x, x.y, y.x, y.y, z.x, z.y};
+  };
+  static_assert(sizeof(SplitItem) == 24, "three pairs");
   auto out_row = [&](const SplitItem &it, int r) {
     const int row = it.row0 + r;
     return static_cast<T *>(a.out) + (it.q0 + a.by_group.div(row)) * a.out_ld + (1ll * it.head * a.G + a.by_group.mod(row)) * a.D;
@@ -1043,16 +1061,16 @@ __global__ void __launch_bounds__(JOIN_THREADS) attention_paged_join_kernel(Page
   // Few pieces: a warp joins a row. With one worker to the CTA its warps share the rows, with four each has
   // a worker of its own.
   {
-    const int me = blockIdx.x * per_cta + (per_cta > 1 ? warp : 0);
-    const int part = per_cta > 1 ? 0 : blockIdx.y * JOIN_WARPS + warp, parts = per_cta > 1 ? 1 : gridDim.y * JOIN_WARPS;
-    const int2 note = me < workers ? a.notes[me] : make_int2(0, -1);
+    const int me = bx * per_cta + (per_cta > 1 ? warp : 0);
+    const int part = per_cta > 1 ? 0 : by * JOIN_WARPS + warp, parts = per_cta > 1 ? 1 : ctas * JOIN_WARPS;
+    const int2 note = me < workers ? note_of(me) : make_int2(0, -1);
     bool many = false;
 #pragma unroll 1
     for (int job = 0; job < 2; ++job) { // the item this worker began, the one its first segment continued
       const int owner = job == 0 ? me : note.y;
       if (job == 0 ? note.x == 0 : note.y < 0)
         continue;
-      const SplitItem it = a.items[owner];
+      const SplitItem it = item_of(owner);
       const int pieces = it.last - owner + 1, share = min(pieces, it.n_rows);
       if (pieces > FEW) {
         many = true;
@@ -1072,18 +1090,18 @@ __global__ void __launch_bounds__(JOIN_THREADS) attention_paged_join_kernel(Page
   }
   // Many pieces: all warps join a row.
 #pragma unroll 1
-  for (int me = blockIdx.x * per_cta; me < min((static_cast<int>(blockIdx.x) + 1) * per_cta, workers); ++me) {
-    const int2 note = a.notes[me];
+  for (int me = bx * per_cta; me < min((bx + 1) * per_cta, workers); ++me) {
+    const int2 note = note_of(me);
 #pragma unroll 1
     for (int job = 0; job < 2; ++job) {
       const int owner = job == 0 ? me : note.y;
       if (job == 0 ? note.x == 0 : note.y < 0)
         continue;
-      const SplitItem it = a.items[owner];
+      const SplitItem it = item_of(owner);
       const int pieces = it.last - owner + 1, share = min(pieces, it.n_rows);
       if (pieces <= FEW)
         continue;
-      for (int r = me - owner + blockIdx.y * share; r < it.n_rows; r += gridDim.y * share) {
+      for (int r = me - owner + by * share; r < it.n_rows; r += ctas * share) {
         const Joined j = join_pieces(a, it, owner, r, warp, JOIN_WARPS, pieces);
         if (lane == 0)
           red_ml[warp] = make_float2(j.M, j.sum);
@@ -1110,6 +1128,23 @@ __global__ void __launch_bounds__(JOIN_THREADS) attention_paged_join_kernel(Page
   }
 }
 
+template <typename T>
+__global__ void __launch_bounds__(JOIN_THREADS) attention_paged_join_kernel(PagedArgs a, JoinShare n) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  join_rows<T>(a, n.workers, n.per_cta, 1, blockIdx.x, 0);
+}
+// Both main kernels' pieces: two joins one after the other would be twice the latency.
+template <typename T>
+__global__ void __launch_bounds__(JOIN_THREADS)
+    attention_paged_join_both_kernel(PagedArgs a, JoinShare n, int blocks, PagedArgs b, JoinShare m) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int block = blockIdx.x;
+  if (block < blocks)
+    join_rows<T>(a, n.workers, 1, n.ctas, block / n.ctas, block % n.ctas);
+  else
+    join_rows<T>(b, m.workers, m.per_cta, 1, block - blocks, 0);
+}
+
 // ---- host -----------------------------------------------------------------------------------------
 constexpr int SIMT_CTAS_PER_SM = 4;
 constexpr int MAX_WORKERS_PER_SM = 12;
@@ -1125,24 +1160,45 @@ bool uses_tile_kernel(int n_tokens, int B, int G, int D, int dtype) {
   return dtype == BF16 && (D == 64 || D == 128) && n_tokens > B && B <= MU_PAGED_TILE_MAX_REQUESTS &&
          1ll * n_tokens * G >= TILE_KERNEL_ROWS;
 }
-size_t part_rows(int num_sms, int n_tokens, int B, int G, int D, int dtype) {
-  return static_cast<size_t>(num_sms) *
-         (uses_tile_kernel(n_tokens, B, G, D, dtype) ? 2 * PAGED_TILE_ROWS : MAX_PART_ROWS_PER_SM);
+// One kernel's part of the workspace: pieces, notes, split items.
+size_t part_bytes(size_t rows, int D, int workers) {
+  return (rows * (sizeof(float) * D + sizeof(float2)) + (sizeof(SplitItem) + sizeof(int2)) * workers + 63) & ~size_t(63);
 }
+size_t tile_part_bytes(int num_sms, int D) { return part_bytes(2ull * PAGED_TILE_ROWS * num_sms, D, num_sms); }
 size_t paged_workspace_bytes(int num_sms, int n_tokens, int B, int G, int D, int dtype) {
-  return part_rows(num_sms, n_tokens, B, G, D, dtype) * (sizeof(float) * D + sizeof(float2)) +
-         (sizeof(SplitItem) + sizeof(int2)) * num_sms * MAX_WORKERS_PER_SM + 64;
+  return part_bytes(1ull * MAX_PART_ROWS_PER_SM * num_sms, D, num_sms * MAX_WORKERS_PER_SM) +
+         (uses_tile_kernel(n_tokens, B, G, D, dtype) ? tile_part_bytes(num_sms, D) : 0) + 64;
+}
+void place_parts(PagedArgs &a, unsigned char *w, size_t rows, int workers) {
+  a.part_o = reinterpret_cast<float *>(w);
+  w += sizeof(float) * rows * a.D;
+  a.part_ml = reinterpret_cast<float2 *>(w);
+  w += sizeof(float2) * rows;
+  a.notes = reinterpret_cast<int2 *>(w);
+  w += sizeof(int2) * workers;
+  a.items = reinterpret_cast<SplitItem *>(w);
 }
 
-// per_cta: workers that a CTA of the join stands for, 1 or JOIN_WARPS; ctas: CTAs that share one worker's rows
-template <typename T> int launch_join(const PagedArgs &a, int workers, int per_cta, int ctas, cudaStream_t st) {
+// A launch that may begin while the kernel before it in the stream drains.
+template <typename... P, typename... A>
+int launch_behind(void (*kernel)(P...), int grid, int threads, size_t smem, bool early, cudaStream_t st, A... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((workers + per_cta - 1) / per_cta, ctas), cfg.blockDim = dim3(JOIN_THREADS), cfg.stream = st;
+  cfg.gridDim = dim3(grid), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at, cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attention_paged_join_kernel<T>, a, workers, per_cta) == cudaSuccess ? 0 : 2;
+  cfg.attrs = at, cfg.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? 0 : 2;
+}
+// `chunks`: the prompt-chunk kernel's arguments, where it went first
+constexpr int TILE_JOIN_CTAS = 8;
+template <typename T>
+int launch_join(const PagedArgs &a, const JoinShare &n, const PagedArgs *chunks, int num_sms, cudaStream_t st) {
+  if (!chunks)
+    return launch_behind(attention_paged_join_kernel<T>, n.blocks(), JOIN_THREADS, 0, true, st, a, n);
+  const JoinShare m{num_sms, 1, TILE_JOIN_CTAS};
+  return launch_behind(attention_paged_join_both_kernel<T>, m.blocks() + n.blocks(), JOIN_THREADS, 0, true, st, *chunks, m,
+                       m.blocks(), a, n);
 }
 
 template <typename T, int RT, int VB, int NA> int launch_simt(PagedArgs a, int num_sms, cudaStream_t st) {
@@ -1161,7 +1217,7 @@ template <typename T, int RT, int VB, int NA> int launch_simt(PagedArgs a, int n
   attention_paged_simt_kernel<T, RT, VB, NA><<<ctas, SIMT_THREADS, smem, st>>>(a);
   if (cudaGetLastError() != cudaSuccess)
     return 2;
-  return launch_join<T>(a, ctas, 1, 1, st);
+  return launch_join<T>(a, JoinShare{ctas, 1, 1}, nullptr, num_sms, st);
 }
 template <typename T, int VB, int NA> int launch_simt_rows(const PagedArgs &a, int num_sms, cudaStream_t st) {
   // rows that share a key: the group's heads for single tokens, up to 8 otherwise
@@ -1173,7 +1229,7 @@ template <typename T, int VB, int NA> int launch_simt_rows(const PagedArgs &a, i
   return launch_simt<T, 8, VB, NA>(a, num_sms, st);
 }
 
-template <typename T, int DP, int NR, int TEAM> int launch_mma_team(PagedArgs a, int num_sms, cudaStream_t st) {
+template <typename T, int DP, int NR, int TEAM> int launch_mma_team(PagedArgs a, const PagedArgs *chunks, int num_sms, cudaStream_t st) {
   using Cfg = MmaCfg<DP, NR, TEAM, sizeof(T) == 4>;
   constexpr size_t ring = Cfg::WARPS * Cfg::WARP_BYTES;
   static_assert(ring + 8 * MU_ATTENTION_PAGED_MAX_REQUESTS <= 227 * 1024, "shared memory");
@@ -1188,22 +1244,21 @@ template <typename T, int DP, int NR, int TEAM> int launch_mma_team(PagedArgs a,
   }
   const int ctas = num_sms * Cfg::CTAS_PER_SM;
   a.rows_per_tile = Cfg::R;
-  attention_paged_mma_kernel<T, DP, NR, TEAM><<<ctas, Cfg::THREADS, ring + 8ull * a.B, st>>>(a);
-  if (cudaGetLastError() != cudaSuccess)
+  if (launch_behind(attention_paged_mma_kernel<T, DP, NR, TEAM>, ctas, Cfg::THREADS, ring + 8ull * a.B, chunks != nullptr, st, a))
     return 2;
-  return launch_join<T>(a, ctas * Cfg::WARPS / TEAM, TEAM == 1 ? JOIN_WARPS : 1, 1, st);
+  return launch_join<T>(a, JoinShare{ctas * Cfg::WARPS / TEAM, TEAM == 1 ? JOIN_WARPS : 1, 1}, chunks, num_sms, st);
 }
-template <typename T, int DP, int NR> int launch_mma(const PagedArgs &a, int num_sms, cudaStream_t st) {
+template <typename T, int DP, int NR> int launch_mma(const PagedArgs &a, const PagedArgs *chunks, int num_sms, cudaStream_t st) {
   // Items (an upper bound) against warps: below an eighth every item would be cut into more than eight
   // pieces, and CTAs become the workers.
   const long long tiles = (1ll * a.n_tokens * a.G + 8 * NR - 1) / (8 * NR);
   const long long items = a.Hkv * (tiles > a.B ? tiles : a.B);
   if (items * 8 <= 1ll * num_sms * MmaCfg<DP, NR, 1, sizeof(T) == 4>::CTAS_PER_SM * MmaCfg<DP, NR, 1, sizeof(T) == 4>::WARPS)
-    return launch_mma_team<T, DP, NR, 4>(a, num_sms, st);
-  return launch_mma_team<T, DP, NR, 1>(a, num_sms, st);
+    return launch_mma_team<T, DP, NR, 4>(a, chunks, num_sms, st);
+  return launch_mma_team<T, DP, NR, 1>(a, chunks, num_sms, st);
 }
 
-template <typename T> int launch_by_dim(const PagedArgs &a, int num_sms, cudaStream_t st) {
+template <typename T> int launch_by_dim(const PagedArgs &a, const PagedArgs *chunks, int num_sms, cudaStream_t st) {
   if (a.D % 16 != 0) {
     if (a.D % 4 != 0)
       return launch_simt_rows<T, 1, 8>(a, num_sms, st);
@@ -1212,39 +1267,35 @@ template <typename T> int launch_by_dim(const PagedArgs &a, int num_sms, cudaStr
   // 8 rows share every key read for single tokens (the group's heads), 16 where there are more
   const bool more = a.n_tokens > a.B || a.G > 8;
   if (a.D > 128)
-    return launch_mma<T, 256, 1>(a, num_sms, st);
+    return launch_mma<T, 256, 1>(a, chunks, num_sms, st);
   if (a.D > 96)
-    return more ? launch_mma<T, 128, 2>(a, num_sms, st) : launch_mma<T, 128, 1>(a, num_sms, st);
+    return more ? launch_mma<T, 128, 2>(a, chunks, num_sms, st) : launch_mma<T, 128, 1>(a, chunks, num_sms, st);
   if (a.D > 64)
-    return more ? launch_mma<T, 96, 2>(a, num_sms, st) : launch_mma<T, 96, 1>(a, num_sms, st);
+    return more ? launch_mma<T, 96, 2>(a, chunks, num_sms, st) : launch_mma<T, 96, 1>(a, chunks, num_sms, st);
   if (a.D > 32)
-    return more ? launch_mma<T, 64, 2>(a, num_sms, st) : launch_mma<T, 64, 1>(a, num_sms, st);
-  return more ? launch_mma<T, 32, 2>(a, num_sms, st) : launch_mma<T, 32, 1>(a, num_sms, st);
+    return more ? launch_mma<T, 64, 2>(a, chunks, num_sms, st) : launch_mma<T, 64, 1>(a, chunks, num_sms, st);
+  return more ? launch_mma<T, 32, 2>(a, chunks, num_sms, st) : launch_mma<T, 32, 1>(a, chunks, num_sms, st);
 }
 
 // 0 ok, 1 dtype not implemented, 2 CUDA error
 int launch_attention_paged(PagedArgs a, void *workspace, int dtype, int num_sms, cudaStream_t st) {
-  const size_t rows = part_rows(num_sms, a.n_tokens, a.B, a.G, a.D, dtype);
   unsigned char *w = static_cast<unsigned char *>(workspace);
-  a.part_o = reinterpret_cast<float *>(w);
-  w += sizeof(float) * rows * a.D;
-  a.part_ml = reinterpret_cast<float2 *>(w);
-  w += sizeof(float2) * rows;
-  a.notes = reinterpret_cast<int2 *>(w);
-  w += sizeof(int2) * num_sms * MAX_WORKERS_PER_SM;
-  a.items = reinterpret_cast<SplitItem *>(w);
   a.rows_from = 1, a.rows_to = INT_MAX;
-  if (uses_tile_kernel(a.n_tokens, a.B, a.G, a.D, dtype)) {
-    PagedArgs t = a;
-    t.rows_from = TILE_KERNEL_ROWS, t.rows_per_tile = PAGED_TILE_ROWS;
-    if (launch_attention_paged_tile(t, num_sms, st) || launch_join<__nv_bfloat16>(t, num_sms, 1, 8, st))
+  PagedArgs chunks = a;
+  const bool tile = uses_tile_kernel(a.n_tokens, a.B, a.G, a.D, dtype);
+  if (tile) {
+    place_parts(chunks, w, 2ull * PAGED_TILE_ROWS * num_sms, num_sms);
+    w += tile_part_bytes(num_sms, a.D);
+    chunks.rows_from = TILE_KERNEL_ROWS, chunks.rows_per_tile = PAGED_TILE_ROWS;
+    if (launch_attention_paged_tile(chunks, num_sms, st))
       return 2;
     a.rows_to = TILE_KERNEL_ROWS - 1;
   }
+  place_parts(a, w, 1ull * MAX_PART_ROWS_PER_SM * num_sms, num_sms * MAX_WORKERS_PER_SM);
   if (dtype == F32)
-    return launch_by_dim<float>(a, num_sms, st);
+    return launch_by_dim<float>(a, nullptr, num_sms, st);
   if (dtype == BF16)
-    return launch_by_dim<__nv_bfloat16>(a, num_sms, st);
+    return launch_by_dim<__nv_bfloat16>(a, tile ? &chunks : nullptr, num_sms, st);
   return 1;
 }
 
