@@ -953,8 +953,9 @@ __global__ void __launch_bounds__(MmaCfg<DP, NR, TEAM, sizeof(T) == 4>::THREADS,
 // The rows of an item with P pieces are dealt out to the first P workers that have a piece of it, so that
 // one long request is not joined in one place; a CTA stands for one worker of the main kernel or for four.
 // Time here is latency (note -> item -> maxima -> rows; 3 to 4 us behind a decode step of 64 requests), so every
-// step loads all it needs at once. Launched so that it may become resident while the main
-// kernel drains; griddepcontrol.wait orders its reads after that kernel's writes.
+// step loads all it needs at once. Launched so that it may become resident while the main kernel drains;
+// griddepcontrol.wait orders its reads after that kernel's writes (loads go to L2: a line of an earlier call's pieces
+// may still be in L1).
 constexpr int JOIN_THREADS = 128, JOIN_WARPS = JOIN_THREADS / 32, JOIN_DIMS = 8; // dimensions per lane: D <= 256
 
 // Where lane `lane` keeps dimension v of its JOIN_DIMS: four in a row where rows are whole 16-byte words.

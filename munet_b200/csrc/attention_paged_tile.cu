@@ -2,7 +2,7 @@
 // many rows (new tokens x query heads of a KV head), bfloat16, head size 64 or 128.
 //
 // Bound by the softmax in front of the tensor pipe: eight requests of up to 8192 keys with chunks of up to 2048 new
-// tokens, 16 query and 4 KV heads of 128, take 710 us with the join (570 TFLOP/s; 730 between changes of work, which
+// tokens, 16 query and 4 KV heads of 128, take 687 us with the join (590 TFLOP/s; 730 between changes of work, which
 // cost 11 us each). Persistent, one CTA per SM, 16 warps:
 //   warp 0      issues every tcgen05.mma (fp16 operands, fp32 accumulators in tensor memory)
 //   warps 1-7   bring keys and values in: e4m3 bytes from their pages, turned into fp16 (exact) and
