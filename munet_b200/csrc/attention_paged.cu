@@ -360,10 +360,10 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_paged_simt_kernel(Page
 
 // ---- tensor-core kernel: head sizes that are multiples of 16 ----------------------------------------
 // Bound by reading the cache (64 requests of up to 2048 keys, 16 heads of 128: 311 MB in 66 us with the join,
-// 4.7 TB/s; 7 TB/s between the first tile and the first warp's end). A warp walks its keys in tiles (32 of them, 16 for head sizes above 128),
-// copies a tile's K and V bytes into its own two stages of shared memory (cp.async, 16 bytes a lane),
-// turns them into fp16 in registers and multiplies with mma.m16n8k16. Where requests x KV heads are many,
-// a warp is a worker of its own and nothing ever synchronises the CTA (TEAM 1). Where they are few, every
+// 4.7 TB/s; 7 TB/s between the first tile and the first warp's end). A warp walks its keys in tiles (32 of them, 16
+// for head sizes above 128), copies a tile's K and V bytes into its own two stages of shared memory (cp.async, 16
+// bytes a lane), turns them into fp16 in registers and multiplies with mma.m16n8k16. Where requests x KV heads are
+// many, a warp is a worker of its own and nothing ever synchronises the CTA (TEAM 1). Where they are few, every
 // item is cut into many pieces whose join would cost as much as the rest (3 requests x 2 heads: 296 pieces
 // each); there the four warps of a CTA are one worker, take every fourth tile and join in shared memory
 // (TEAM 4).

@@ -669,6 +669,33 @@ def test_generation_steps_in_a_graph(ctx, dtype, H, G, D):
     ctx.check()
 
 
+@pytest.mark.parametrize("D,Hq,Hkv", [(64, 8, 2), (128, 4, 4)])
+def test_mixed_call_in_a_graph(ctx, D, Hq, Hkv):
+    """Prompt chunks and single tokens in one captured call, whose kernels overlap: what follows in the graph finds
+    every row, and the next replay may write the same rows and workspace again."""
+    import torch
+    rng = np.random.default_rng(18)
+    pr = make_problem(rng, BF16, 6, Hq, Hkv, D, 16, [1300, 70, 900, 400, 33, 2100], [260, 1, 1, 200, 1, 30])
+    want = run_attention(ctx, pr, BF16, True, Hkv, 16).clone()
+    check_attention(pr, want, BF16, True, 16)
+    ws = torch.full((ctx.attention_paged_workspace_bytes(pr["n"], 6, Hq, Hkv, D, BF16),), 0xFF, dtype=torch.uint8,
+                    device="cuda")
+    out, kept = torch.full_like(want, 7.0), torch.zeros(40, *want.shape, dtype=want.dtype, device="cuda")
+    turn = torch.zeros(1, dtype=torch.int64, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run_attention(ctx, pr, BF16, True, Hkv, 16, ws=ws, out=out)
+        kept.index_copy_(0, turn, out[None])
+        out.fill_(7.0)
+        ws.fill_(0xFF)
+        turn += 1
+    for _ in range(40):
+        graph.replay()
+    torch.cuda.synchronize()
+    ctx.check()
+    assert all(torch.equal(k, want) for k in kept)
+
+
 def test_two_graphs_that_share_a_workspace_in_turn(ctx):
     """Two captured calls with different lengths use one workspace one after the other."""
     import torch
