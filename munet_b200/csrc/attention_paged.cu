@@ -1155,8 +1155,9 @@ constexpr int MAX_WORKERS_PER_SM = 12;
 constexpr int MAX_PART_ROWS_PER_SM = 2 * 128;
 // Requests with this many rows (new tokens x heads of a group) or more go to the prompt-chunk kernel: below, a
 // tile of 256 rows would be mostly empty, and reading the keys once per 16 rows costs less (8 requests of 4096
-// keys, 4 KV heads of 128: 64 rows 45 us against 50, 96 rows 67 against 52, 128 rows 82 against 54).
-constexpr int TILE_KERNEL_ROWS = 81;
+// keys, 4 KV heads of 128: 64 rows 46 us against 50, 72 rows 51 against 51, 80 rows 60 against 51, 128 rows 83
+// against 53; of 64: 72 rows 41 against 44, 80 rows 43 against 44, 88 rows 49 against 45).
+constexpr int TILE_KERNEL_ROWS = 73;
 bool uses_tile_kernel(int n_tokens, int B, int G, int D, int dtype) {
   return dtype == BF16 && (D == 64 || D == 128) && n_tokens > B && B <= MU_PAGED_TILE_MAX_REQUESTS &&
          1ll * n_tokens * G >= TILE_KERNEL_ROWS;
