@@ -39,6 +39,21 @@ template <int D> struct PtCfg {
   static constexpr int TAIL = BARS * 8 + PT_SLOTS * 8 * 16 + PT_SLOTS * 32 + 16;
 };
 
+// Byte of 16-byte word `word` of row `row` of a query tile: blocks of 64 dimensions, 128 bytes a row, swizzled. Queries
+// and the output that is staged in their place both go through it, so a warp only ever touches its own rows' bytes and
+// needs no barrier with the others of its tile between an output and the next work's queries.
+__host__ __device__ constexpr int q_word(int row, int word) {
+  return (word >> 3) * (PT_BQ * 128) + row * 128 + (((word & 7) ^ (row & 7)) << 4);
+}
+template <int D> constexpr bool rows_apart() { // within the tile, and in their own row's 128 bytes of each block
+  for (int row = 0; row < PT_BQ; ++row)
+    for (int word = 0; word < D / 8; ++word)
+      if (q_word(row, word) < 0 || q_word(row, word) + 16 > PtCfg<D>::Q_BYTES || q_word(row, word) / 128 % PT_BQ != row)
+        return false;
+  return true;
+}
+static_assert(rows_apart<64>() && rows_apart<128>(), "rows of a query tile share bytes");
+
 // Row tile costs of one request: tile t counts first + t * slope units, no fewer than the keys it sees / 8.
 struct TileCosts {
   int tiles, slope;
@@ -553,8 +568,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_paged_tile_kernel(Pag
           for (int k = 0; k < 2; ++k) {
             const uint4 u = load8(c + k);
             auto two = [&](uint32_t w) { return f16x2(bf16_lo(w) * f, bf16_hi(w) * f); };
-            *reinterpret_cast<uint4 *>(sQ + x * Cfg::Q_BYTES + ((c + k) >> 3) * (PT_BQ * 128) + row * 128 +
-                                       ((((c + k) & 7) ^ (row & 7)) << 4)) = make_uint4(two(u.x), two(u.y), two(u.z), two(u.w));
+            *reinterpret_cast<uint4 *>(sQ + x * Cfg::Q_BYTES + q_word(row, c + k)) =
+                make_uint4(two(u.x), two(u.y), two(u.z), two(u.w));
           }
         fence_proxy_async();
         __syncwarp();
@@ -703,9 +718,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_paged_tile_kernel(Pag
       // wait on each other's latency.
       const float inv = g.slot >= 0 ? 1.f : l_run == 0.f ? 0.f : 1.f / l_run;
       const long long pr = 1ll * max(g.slot, 0) * a.rows_per_tile + x * PT_BQ + row;
-      uint8_t *stage = sQ + x * Cfg::Q_BYTES + q * 32 * D * 2; // 32 rows of D * 2 bytes
-      constexpr int ROW = D * 2, PER_ROW = ROW / 16;           // bytes, 16-byte words
-      auto cell = [&](int r, int c) { return reinterpret_cast<uint4 *>(stage + r * ROW + ((c ^ (r & 7)) << 4)); };
+      constexpr int PER_ROW = D / 8; // 16-byte words
+      auto cell = [&](int r, int c) { return reinterpret_cast<uint4 *>(sQ + x * Cfg::Q_BYTES + q_word(q * 32 + r, c)); };
       const long long my_out = live ? 1ll * (s.q0 + token) * a.out_ld + 1ll * head * D : -1;
       auto rows_out = [&](auto &&to) { // the staged rows, coalesced: to(row of the warp, word) takes 16 bytes
         __syncwarp();
