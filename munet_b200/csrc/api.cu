@@ -341,6 +341,8 @@ int mu_check(mu_ctx *ctx, void *stream) {
     return fail(ctx, MU_ERR_NOMEM, "page map: free pages, block table or slots exhausted");
   if (st == 113)
     return fail(ctx, MU_ERR_INDEX, "paged cache: request lengths out of range");
+  if (st == 114)
+    return fail(ctx, MU_ERR_CUDA, "paged cache: attention kernel's shared memory is misaligned, its rows are not written");
   return fail(ctx, MU_ERR_TIMEOUT, "device-side bounded wait ran out (code %d)", st);
 }
 

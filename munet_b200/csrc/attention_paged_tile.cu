@@ -193,9 +193,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_paged_tile_kernel(Pag
   long long *upto = reinterpret_cast<long long *>(smem + Cfg::SMEM + (Cfg::TAIL + 15) / 16 * 16);
   __shared__ long long warp_sum[PT_THREADS / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, me = blockIdx.x;
+  if (tid == 0)
+    a.notes[me] = make_int2(0, -1); // before any way out: the join reads every worker's
   if (smem_u32(smem) & 1023u) { // the swizzled operands need it
     if (tid == 0)
-      atomicCAS(a.status, 0, MU_DEV_BAD_INDEX);
+      atomicCAS(a.status, 0, MU_DEV_BAD_LAYOUT);
     return;
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); // the join waits for the whole grid anyway
@@ -234,7 +236,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_paged_tile_kernel(Pag
       upto[b] += before;
   }
   if (tid == 0) {
-    a.notes[me] = make_int2(0, -1);
     for (int x = 0; x < 2; ++x) {
       mbar_init(&q_full[x], 4), mbar_init(&q_empty[x], 1);
       mbar_init(&k_full[x], PT_LOADERS), mbar_init(&k_empty[x], 1);
@@ -302,7 +303,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_paged_tile_kernel(Pag
                       vd + static_cast<uint64_t>(((k / 4) * (DB * 8192) + (k % 4) * 2048) >> 4), idesc_pv,
                       (accumulate || k != 0) ? 1u : 0u);
       };
-      while (ok && walk.next(a, upto, g, s, true)) {
+      while (walk.next(a, upto, g, s, true)) {
+        if (!ok) // a wait ran out: other workers' notes still name the items that this one begins
+          continue;
         const int nk_x[2] = {tiles_of(0), tiles_of(1)}, nk = max(nk_x[0], nk_x[1]);
         if (nk == 0)
           continue;
@@ -310,7 +313,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_paged_tile_kernel(Pag
           if (nk_x[x] > 0)
             wait(&q_full[x], wq[x] & 1, MU_DEV_TIMEOUT_MMA);
         if (!wait(&k_full[kq & 1], (kq >> 1) & 1, MU_DEV_TIMEOUT_MMA))
-          break;
+          continue;
         tc_fence_after();
         for (int x = 0; x < 2; ++x)
           if (nk_x[x] > 0) {

@@ -22,6 +22,7 @@ enum : int {
   MU_DEV_BAD_PAGE = 111,   // page or slot outside the cache / block table
   MU_DEV_NO_PAGE = 112,    // free pages, block table or slots too few for the request lengths
   MU_DEV_BAD_LENGTH = 113, // negative or contradictory request lengths
+  MU_DEV_BAD_LAYOUT = 114, // a kernel's shared memory is not where its operands need it
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {
