@@ -581,8 +581,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_paged_tile_kernel(Pag
 
         for (int j = 0; j < nk && ok; ++j, ++st) {
           const int slot = (tile0 + j) & (PT_SLOTS - 1), lim = limit - (g.chunk0 + j) * PT_BK;
-          wait(&m_full[slot], ((tile0 + j) / PT_SLOTS) & 1, MU_DEV_TIMEOUT_EPILOGUE);
-          if (!wait(&s_full[x], st & 1, MU_DEV_TIMEOUT_EPILOGUE))
+          wait(&s_full[x], st & 1, MU_DEV_TIMEOUT_EPILOGUE);
+          // Behind the scores: a query tile that had no part in the key tiles before may be several of the slot's
+          // phases ahead, where its parity says nothing; now the scales are there, and those of tile + PT_SLOTS are not.
+          if (!wait(&m_full[slot], ((tile0 + j) / PT_SLOTS) & 1, MU_DEV_TIMEOUT_EPILOGUE))
             break;
           tc_fence_after();
           const float4 *sc = scales + slot * 8;

@@ -161,3 +161,26 @@ def test_several_works_per_cta(ctx, case, D, causal, aligned):
         assert torch.equal(out, first)
         assert aligned or ((wide[:, 0] == 7).all() and (wide[:, 1 + Hq * D:] == 7).all())
     ctx.check()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_query_tile_that_sits_out_long_works(ctx, D):
+    """Works of one query tile over many key tiles, then works of two: the second tile's warps come from far ahead of the
+    keys and values, with scales that differ from page to page."""
+    import torch
+    B, G, page = 240, 8, 16
+    news = [10 if b % 2 else 25 for b in range(B)]
+    lens = [1500 + 3 * b for b in range(B)]
+    works = works_of(lens, news, G, 1, True, ctx.num_sms)
+    # more than two turns of the four slots with one query tile, then two of them
+    assert sum(a[3] > 8 and news[a[0]] * G <= 128 and news[b[0]] * G > 128 for w in works for a, b in zip(w, w[1:])) > 20
+    rng = np.random.default_rng(D)
+    pr = make_problem(rng, BF16, B, G, 1, D, page, lens, news)
+    pr["ks"] *= np.exp2(rng.integers(-3, 2, pr["ks"].shape)).astype(np.float32)
+    pr["vs"] *= np.exp2(rng.integers(-6, 7, pr["vs"].shape)).astype(np.float32)
+    want, bound = expect(pr, True, page)
+    first = run_attention(ctx, pr, BF16, True, 1, page)
+    check(pr, first, want, bound)
+    for _ in range(10):
+        assert torch.equal(run_attention(ctx, pr, BF16, True, 1, page), first)
+    ctx.check()
