@@ -235,8 +235,8 @@ int mu_kv_cache_append(mu_ctx *ctx, const void *k, const void *v, long long ld, 
  * request is skipped. What lies in a page behind its request's last token is never read as a value. Scales
  * from 2^-64 to 2^64 keep every bit of their values (V scales below count as 2^-64). `out` must not overlap q.
  * workspace (16-byte aligned, mu_attention_paged_workspace_bytes) holds pieces of long requests during the
- * call only; calls that may overlap on the GPU need one each. At most MU_ATTENTION_PAGED_MAX_REQUESTS
- * requests. */
+ * call only; calls that may overlap on the GPU need one each. It never shrinks as n_tokens or B grow, so one made
+ * for a program's largest call serves its smaller ones. At most MU_ATTENTION_PAGED_MAX_REQUESTS requests. */
 #define MU_ATTENTION_PAGED_MAX_REQUESTS 16384
 size_t mu_attention_paged_workspace_bytes(const mu_ctx *ctx, int n_tokens, int B, int Hq, int Hkv,
                                           int D, int dtype);

@@ -1158,18 +1158,22 @@ constexpr int MAX_PART_ROWS_PER_SM = 2 * 128;
 // keys, 4 KV heads of 128: 64 rows 46 us against 50, 72 rows 51 against 51, 80 rows 60 against 51, 128 rows 83
 // against 53; of 64: 72 rows 41 against 44, 80 rows 43 against 44, 88 rows 49 against 45).
 constexpr int TILE_KERNEL_ROWS = 73;
+bool tile_kernel_shape(int n_tokens, int G, int D, int dtype) {
+  return dtype == BF16 && (D == 64 || D == 128) && 1ll * n_tokens * G >= TILE_KERNEL_ROWS;
+}
 bool uses_tile_kernel(int n_tokens, int B, int G, int D, int dtype) {
-  return dtype == BF16 && (D == 64 || D == 128) && n_tokens > B && B <= MU_PAGED_TILE_MAX_REQUESTS &&
-         1ll * n_tokens * G >= TILE_KERNEL_ROWS;
+  return tile_kernel_shape(n_tokens, G, D, dtype) && n_tokens > B && B <= MU_PAGED_TILE_MAX_REQUESTS;
 }
 // One kernel's part of the workspace: pieces, notes, split items.
 size_t part_bytes(size_t rows, int D, int workers) {
   return (rows * (sizeof(float) * D + sizeof(float2)) + (sizeof(SplitItem) + sizeof(int2)) * workers + 63) & ~size_t(63);
 }
 size_t tile_part_bytes(int num_sms, int D) { return part_bytes(2ull * PAGED_TILE_ROWS * num_sms, D, num_sms); }
-size_t paged_workspace_bytes(int num_sms, int n_tokens, int B, int G, int D, int dtype) {
+// Whatever the number of requests: a workspace for a program's largest call serves its smaller ones, among them those of
+// few requests that use the prompt-chunk kernel where the largest does not.
+size_t paged_workspace_bytes(int num_sms, int n_tokens, int G, int D, int dtype) {
   return part_bytes(1ull * MAX_PART_ROWS_PER_SM * num_sms, D, num_sms * MAX_WORKERS_PER_SM) +
-         (uses_tile_kernel(n_tokens, B, G, D, dtype) ? tile_part_bytes(num_sms, D) : 0) + 64;
+         (n_tokens > 1 && tile_kernel_shape(n_tokens, G, D, dtype) ? tile_part_bytes(num_sms, D) : 0) + 64;
 }
 void place_parts(PagedArgs &a, unsigned char *w, size_t rows, int workers) {
   a.part_o = reinterpret_cast<float *>(w);
@@ -1313,7 +1317,7 @@ int *mu_ctx_status_ptr(mu_ctx *ctx);
 size_t mu_attention_paged_workspace_bytes(const mu_ctx *ctx, int n_tokens, int B, int Hq, int Hkv, int D, int dtype) {
   if (!ctx || n_tokens <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0)
     return 0;
-  return mu::paged_workspace_bytes(mu_ctx_num_sms(ctx), n_tokens, B, Hq / Hkv, D, dtype);
+  return mu::paged_workspace_bytes(mu_ctx_num_sms(ctx), n_tokens, Hq / Hkv, D, dtype);
 }
 
 int mu_attention_paged(mu_ctx *ctx, const void *q, long long q_ld, void *out, long long out_ld, const void *k_cache,
