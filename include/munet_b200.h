@@ -233,7 +233,9 @@ int mu_kv_cache_append(mu_ctx *ctx, const void *k, const void *v, long long ld, 
  * `out` behind query_start[B] are left as they are. Keys on a page id outside the pool, or beyond
  * table_stride pages, are left out and latch MU_ERR_INDEX; so do contradictory row ranges, whose
  * request is skipped. What lies in a page behind its request's last token is never read as a value. Scales
- * from 2^-64 to 2^64 keep every bit of their values (V scales below count as 2^-64). `out` must not overlap q.
+ * from 2^-64 to 2^64 keep every bit of their values (V scales below count as 2^-64). At head sizes that
+ * are multiples of 16 a weight p_j * v_scale_j is held in fp16 (float32: two fp16 numbers), the row's largest at 2^7 or
+ * more (float32: 2^15): 11 (22) bits, but no step finer than 2^-31 (2^-39) of the largest. `out` must not overlap q.
  * workspace (16-byte aligned, mu_attention_paged_workspace_bytes) holds pieces of long requests during the
  * call only; calls that may overlap on the GPU need one each. It never shrinks as n_tokens or B grow, so one made
  * for a program's largest call serves its smaller ones. At most MU_ATTENTION_PAGED_MAX_REQUESTS requests. */
@@ -373,8 +375,8 @@ int mu_argmax(mu_ctx *ctx, const void *x, int32_t *idx, long long rows, int cols
  * uniform * (their sum); prob[r] = its share of that sum. temperature, top_k, top_p, min_p are one value
  * per row on the device, or NULL for none (temperature 1); prob may be NULL. A temperature <= 0 takes the
  * first maximum. NaN counts as -inf; a row with nothing above -inf gives idx -1, prob 0; +inf leaves
- * only infinite logits. Sums are exact (weights are integer multiples of 2^-42), so results do not
- * depend on the launch shape. */
+ * only infinite logits. Sums are exact (weights are integer multiples of 2^-42, so a logit whose weight is below
+ * 2^-43 is never drawn), and results do not depend on the launch shape. */
 #define MU_SAMPLE_MAX_COLS 1048576
 int mu_sample(mu_ctx *ctx, const void *logits, long long ld, const float *uniform,
               const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,

@@ -11,8 +11,10 @@
 // are. A worker walks its range as segments, one per (request, head, row tile). A segment that covers
 // all chunks writes its rows; one that does not leaves (running maximum, sum, weighted values) in the
 // workspace, and a second small kernel joins the pieces. No atomics: results do not depend on the order
-// in which workers run. Every item counts a few units more than its chunks, for what starting a segment
-// costs: without it the workers that got many short requests finished last.
+// in which workers run. (A causal row tile counts all of its request's chunks, those that it does not see among
+// them. Prompts that take this file's kernels, float32 or head sizes other than 64 and 128, are therefore shared out
+// unevenly: the workers of early rows have less to do.) Every item counts a few units more than its chunks,
+// for what starting a segment costs: without it the workers that got many short requests finished last.
 #include "../../include/munet_b200.h"
 #include "attention_paged.cuh"
 #include <climits>
@@ -1156,7 +1158,9 @@ constexpr int MAX_PART_ROWS_PER_SM = 2 * 128;
 // Requests with this many rows (new tokens x heads of a group) or more go to the prompt-chunk kernel: below, a
 // tile of 256 rows would be mostly empty, and reading the keys once per 16 rows costs less (8 requests of 4096
 // keys, 4 KV heads of 128: 64 rows 46 us against 50, 72 rows 51 against 51, 80 rows 60 against 51, 128 rows 83
-// against 53; of 64: 72 rows 41 against 44, 80 rows 43 against 44, 88 rows 49 against 45).
+// against 53; of 64: 72 rows 41 against 44, 80 rows 43 against 44, 88 rows 49 against 45: there the border lies 8 to 15
+// rows higher, and one number serves both at a cost of 1 to 3 us). The host cannot see lengths: a call of more tokens than
+// requests launches the prompt-chunk kernel whether or not a request has this many.
 constexpr int TILE_KERNEL_ROWS = 73;
 bool tile_kernel_shape(int n_tokens, int G, int D, int dtype) {
   return dtype == BF16 && (D == 64 || D == 128) && 1ll * n_tokens * G >= TILE_KERNEL_ROWS;

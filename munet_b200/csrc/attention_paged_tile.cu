@@ -2,8 +2,8 @@
 // many rows (new tokens x query heads of a KV head), bfloat16, head size 64 or 128.
 //
 // Bound by the softmax in front of the tensor pipe: eight requests of up to 8192 keys with chunks of up to 2048 new
-// tokens, 16 query and 4 KV heads of 128, take 687 us with the join (590 TFLOP/s; 730 between changes of work, which
-// cost 11 us each). Persistent, one CTA per SM, 16 warps:
+// tokens, 16 query and 4 KV heads of 128, take 691 us with the join (587 TFLOP/s; 730 between changes of work, which
+// cost 11 us each); with heads of 64, 587 us (346 TFLOP/s: as many weights for half the products). Persistent, one CTA per SM, 16 warps:
 //   warp 0      issues every tcgen05.mma (fp16 operands, fp32 accumulators in tensor memory)
 //   warps 1-7   bring keys and values in: e4m3 bytes from their pages, turned into fp16 (exact) and
 //               written where a TMA with 128-byte swizzle would have put them
@@ -28,7 +28,8 @@ namespace mu {
 constexpr int PT_BQ = 128, PT_BK = 128, PT_ROWS = 2 * PT_BQ; // a row tile is the pair A, B
 constexpr int PT_LOADERS = 7, PT_THREADS = 32 * (1 + PT_LOADERS + 8);
 constexpr int PT_UNIT = 8, PT_START = 112; // keys of a unit; units that beginning an item counts for: seven key tiles
-                                           // (16 units: 823 us for the mixed chunks above, 48: 770, 80: 717, 128: 712)
+                                           // (16 units: 823 us for the mixed chunks above, 48: 770, 80: 717, 128: 712;
+                                           // measured at head size 128 only)
 constexpr int PT_SLOTS = 4;               // key tiles whose page scales are kept
 constexpr float PT_W_EXP = 7.f;           // a row's reference weight is 2^7: with the 2^8 the maximum may lead, 2^15
 
