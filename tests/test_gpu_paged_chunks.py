@@ -184,3 +184,62 @@ def test_a_query_tile_that_sits_out_long_works(ctx, D):
     for _ in range(10):
         assert torch.equal(run_attention(ctx, pr, BF16, True, 1, page), first)
     ctx.check()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_captured_call_whose_lengths_change(ctx, D):
+    """Lengths, tables and row ranges are the device's: one captured call serves chunks, single tokens, an empty batch and
+    padded tokens."""
+    import torch
+    B, G, Hkv, page, cap = 6, 4, 2, 16, 400
+    rng = np.random.default_rng(D)
+    steps = [([300, 40, 1, 0, 30, 1], [900, 40, 700, 0, 31, 16]), ([1] * 6, [901, 41, 701, 1, 32, 17]), ([0] * 6, [901, 41, 701, 1, 32, 17]),
+             ([66, 66, 66, 66, 66, 66], [66, 1000, 300, 67, 2000, 80])]
+    width = 2000 // page + 2
+    pr = make_problem(rng, BF16, B, G * Hkv, Hkv, D, page, [2000] * B, [1] * B)
+    num = pr["kc"].shape[0]
+    pr["table"] = rng.permutation(num)[:B * (2000 // page)].reshape(B, -1).astype(np.int32)
+    pr["table"] = np.concatenate([pr["table"], np.full((B, width - pr["table"].shape[1]), -1, np.int32)], 1)
+    pr["q"], pr["n"] = torch.randn(cap, G * Hkv, D, device="cuda").to(torch.bfloat16), cap
+    pr["dev"] = [torch.from_numpy(pr[k]).cuda() for k in ("kc", "vc", "ks", "vs", "table", "qs", "seq")]
+    ws = torch.full((ctx.attention_paged_workspace_bytes(cap, B, G * Hkv, Hkv, D, BF16),), 0xFF, dtype=torch.uint8, device="cuda")
+    out = torch.full_like(pr["q"], 7.0)
+    run_attention(ctx, pr, BF16, True, Hkv, page, ws=ws, out=out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run_attention(ctx, pr, BF16, True, Hkv, page, ws=ws, out=out)
+    for news, lens in steps * 3:
+        pr["qs"], pr["seq"] = np.concatenate([[0], np.cumsum(news)]).astype(np.int32), np.asarray(lens, np.int32)
+        pr["dev"][5].copy_(torch.from_numpy(pr["qs"]))
+        pr["dev"][6].copy_(torch.from_numpy(pr["seq"]))
+        out.fill_(7.0)
+        graph.replay()
+        ctx.check()
+        if sum(news):
+            check(pr, out, *expect(pr, True, page))
+        assert (out[sum(news):] == 7).all()
+
+
+@pytest.mark.parametrize("D,new", [(128, 40), (64, 100), (100, 2)])
+def test_offsets_beyond_32_bits(ctx, D, new):
+    """Pages at the far end of a pool of more than 2^32 bytes, and rows of q and out over 2^33 elements."""
+    import torch
+    G, Hkv, page = 4, 2, 64
+    rng = np.random.default_rng(D)
+    pr = make_problem(rng, BF16, 2, G * Hkv, Hkv, D, page, [300, 150], [new, 1], pad_rows=0)
+    want = run_attention(ctx, pr, BF16, True, Hkv, page)
+    small = pr["dev"][:4]
+    P, num = small[0].shape[0], (9 << 29) // (Hkv * D * page)
+    big = [torch.empty((num,) + tuple(t.shape[1:]), dtype=t.dtype, device="cuda") for t in small]
+    for b, t in zip(big, small):
+        b[num - P:] = t
+    table = torch.from_numpy(np.where(pr["table"] >= 0, pr["table"] + num - P, -1).astype(np.int32)).cuda()
+    far = dict(pr, dev=[*big, table, *pr["dev"][5:]], kc=np.empty((num, 0)))
+    assert torch.equal(run_attention(ctx, far, BF16, True, Hkv, page), want)
+    del big, far
+    ld = 2 ** 33 // pr["n"] // 8 * 8
+    q, out = (torch.empty(pr["n"] * ld, dtype=torch.bfloat16, device="cuda").view(pr["n"], ld)[:, :G * Hkv * D] for _ in range(2))
+    q, out = (t.view(pr["n"], G * Hkv, D) for t in (q, out))
+    q.copy_(pr["q"])
+    assert torch.equal(run_attention(ctx, dict(pr, q=q), BF16, True, Hkv, page, out=out), want)
+    ctx.check()
